@@ -28,6 +28,8 @@ FKV_ERR_UNSUPPORTED = 5
 FKV_ERR_TIMEOUT = 6
 FKV_ERR_IO = 7
 
+FKV_DTYPE_BF16, FKV_DTYPE_FP16 = 0, 1
+
 
 class TransferDesc(ctypes.Structure):
     """Mirror of ``fkv_transfer_desc`` (field order and types must match)."""
@@ -191,6 +193,23 @@ _SIGNATURES = {
         [c_int, c_int, c_int, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64,
          c_i64, c_i64, c_i64, c_vp, c_int, c_int, c_int],
     ),
+    "fkv_fp4_write": (
+        c_int, [c_vp, c_int, c_i64, c_int, c_int, c_int, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64,
+                c_i64, c_int, c_vp, c_i64, c_vp]),
+    "fkv_fp4_read": (
+        c_int, [c_vp, c_int, c_i64, c_int, c_int, c_int, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64,
+                c_i64, c_int, c_vp, c_i64, c_vp]),
+    "fkv_fp4_pack_blocks": (
+        c_int, [c_int, c_vp, c_vp, c_int, c_int, c_int, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64,
+                c_int, c_vp, c_vp, c_i64, c_vp]),
+    "fkv_fp4_unpack_blocks": (
+        c_int, [c_int, c_vp, c_vp, c_int, c_int, c_int, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64,
+                c_int, c_vp, c_vp, c_i64, c_vp]),
+    "fkv_fp4_attention_workspace": (c_i64, [c_i64, c_int, c_int, c_int, c_int, c_int]),
+    "fkv_fp4_attention": (
+        c_int, [c_vp, c_i64, c_int, c_int, c_int, c_i64, c_i64, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64,
+                c_int, c_i64, c_int, c_vp, c_i64, c_int, c_vp, c_vp, c_int, c_int, ctypes.c_float, c_int,
+                c_vp, c_i64, c_vp]),
     "fkv_cache_index_create": (c_int, [c_int, c_i64, c_int, ctypes.POINTER(c_vp)]),
     "fkv_cache_index_destroy": (None, [c_vp]),
     "fkv_cache_index_match": (c_int, [c_vp, c_vp, c_vp, c_int, c_vp, c_vp, c_vp, c_vp]),

@@ -1,0 +1,321 @@
+// The KV cache in 4 bits: quantising tokens as they are written, reading
+// them back, and both for whole blocks of every layer (the 16-bit cache of an
+// inference engine on one side, 4-bit blocks for the host and SSD tiers on
+// the other).
+//
+// Format.  16 consecutive channels of one token and head are a group: 16
+// e2m1 values q and one scale s of 5 exponent and 3 mantissa bits (a half
+// without sign and low mantissa bits: code c is the half with bits c << 7).
+//   s = nearest(amax / 6), at most 10240;  q = nearest_e2m1(x / s)
+// both with ties to the even code; x' = q * s has at most 6 significant bits
+// and is exact in half and bfloat16.  16 tokens of one head are a unit of
+// 9 * D bytes: 16 rows of D / 2 payload bytes (even channel in the low four
+// bits), then 16 rows of D / 16 scale bytes.  A unit is one contiguous,
+// 16-byte aligned piece, so attention fetches it with one bulk copy; a block
+// holds its units head after head, so a head's share of a block (and a
+// tensor-parallel rank's) is one piece too.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "fkv_common.h"
+#include "fp4_format.cuh"
+
+namespace fkv {
+namespace {
+
+constexpr int kMaxLayers = 128;  // layers of one launch: their pointers travel in the kernel's parameters
+constexpr int kThreads = 256;
+constexpr int kUnroll = 4;
+
+struct RowsArgs {
+  int num_heads;
+  int kv_dim;
+  int tokens_per_block;
+  int64_t num_rows;       // tokens of the call (blocks * tokens_per_block for the block form)
+  int64_t num_slots;      // slots of the 4-bit layer
+  int64_t num_row_slots;  // slots of the 16-bit side (block form)
+  int64_t fp4_kv_stride, fp4_block_stride;
+  int64_t token_stride[2], head_stride[2];        // bytes, 16-bit side
+  int64_t row_block_stride;                        // bytes, block form
+  const int64_t *fp4_ids;                          // slots (token form) or blocks
+  const int64_t *row_ids;                          // blocks of the 16-bit side (block form)
+  uint8_t *fp4[kMaxLayers];
+  uint8_t *rows[2][kMaxLayers];
+};
+
+// 32 bytes in one access where the address allows it, else two of 16.
+template <bool WIDE>
+__device__ __forceinline__ void load_group(const uint8_t *p, uint32_t (&r)[8]) {
+  if (WIDE) {
+    asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "l"(p));
+  } else {
+    const uint4 a = *reinterpret_cast<const uint4 *>(p), b = *reinterpret_cast<const uint4 *>(p + 16);
+    r[0] = a.x, r[1] = a.y, r[2] = a.z, r[3] = a.w, r[4] = b.x, r[5] = b.y, r[6] = b.z, r[7] = b.w;
+  }
+}
+template <bool WIDE>
+__device__ __forceinline__ void store_group(uint8_t *p, const uint32_t (&r)[8]) {
+  if (WIDE) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4 *>(p)[0] = make_uint4(r[0], r[1], r[2], r[3]);
+    reinterpret_cast<uint4 *>(p)[1] = make_uint4(r[4], r[5], r[6], r[7]);
+  }
+}
+
+// One thread per group of 16 channels.  A CTA takes R consecutive rows of the
+// list (R = 16, or 1 for a call with fewer rows than 16) of one layer and
+// side, for every head; threads run over groups first, then rows, then heads,
+// so 32 lanes store 256 payload bytes and 32 scale bytes of one unit next to
+// each other.  NG: groups of a head, 0 = at run time.
+template <bool WRITE, bool BF16, bool BLOCKS, bool WIDE, int NG, int R>
+__global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constant__ RowsArgs a, int groups) {
+  const int ng = NG ? NG : groups;
+  const int layer = blockIdx.y / a.kv_dim, side = blockIdx.y % a.kv_dim;
+  const int64_t row0 = (int64_t)blockIdx.x * R;
+  const int work = a.num_heads * R * ng;
+  uint8_t *const fp4 = a.fp4[layer] + side * a.fp4_kv_stride;
+  uint8_t *const rows = a.rows[side][layer];
+  const int D = 16 * ng, tpb = a.tokens_per_block;
+  for (int w0 = threadIdx.x; w0 < work; w0 += kThreads * kUnroll) {
+    uint32_t x[kUnroll][8];
+    uint8_t *pay[kUnroll], *sc[kUnroll], *row[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int w = w0 + u * kThreads;
+      pay[u] = nullptr, row[u] = nullptr;
+      if (w < work) {
+        const int g = w % ng, t = (w / ng) % R, h = w / (ng * R);
+        const int64_t i = row0 + t;
+        if (i < a.num_rows) {
+          int64_t slot;
+          if (BLOCKS) {
+            const int64_t b = i / tpb, off = i % tpb;
+            const int64_t fb = a.fp4_ids[b], rb = a.row_ids[b];
+            slot = fb < 0 ? -1 : fb * tpb + off;
+            if (rb < 0 || rb >= a.num_row_slots) slot = -1;
+            row[u] = rows + rb * a.row_block_stride + off * a.token_stride[side] + h * a.head_stride[side] + g * 32;
+          } else {
+            slot = a.fp4_ids[i];
+            row[u] = rows + i * a.token_stride[side] + h * a.head_stride[side] + g * 32;
+          }
+          if (slot >= 0 && slot < a.num_slots) {
+            const int64_t b = slot / tpb;
+            const int off = (int)(slot - b * tpb);
+            uint8_t *unit = fp4 + b * a.fp4_block_stride + ((int64_t)h * (tpb / 16) + off / 16) * (9 * D);
+            pay[u] = unit + (off % 16) * (D / 2) + g * 8;
+            sc[u] = unit + 8 * D + (off % 16) * ng + g;
+          }
+          if (pay[u]) {
+            if (WRITE) {
+              load_group<WIDE>(row[u], x[u]);
+            } else {
+              const uint2 p = *reinterpret_cast<const uint2 *>(pay[u]);
+              x[u][0] = p.x, x[u][1] = p.y, x[u][2] = *sc[u];
+            }
+          } else if (!WRITE && !BLOCKS) {
+            x[u][0] = x[u][1] = x[u][2] = 0;  // a row without a slot reads as zeros
+          } else {
+            row[u] = nullptr;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      if (!row[u]) continue;
+      if (WRITE) {
+        if (!pay[u]) continue;
+        uint2 p;
+        const uint32_t code = quantise_group<BF16>(x[u], p);
+        *reinterpret_cast<uint2 *>(pay[u]) = p;
+        *sc[u] = (uint8_t)code;
+      } else {
+        uint32_t y[8];
+        dequantise_group<BF16>(make_uint2(x[u][0], x[u][1]), x[u][2], y);
+        store_group<WIDE>(row[u], y);
+      }
+    }
+  }
+}
+
+template <bool WRITE, bool BF16, bool BLOCKS, bool WIDE, int R>
+void launch_ng(const RowsArgs &a, dim3 grid, int ng, cudaStream_t s) {
+  switch (ng) {
+    case 4: fp4_rows_kernel<WRITE, BF16, BLOCKS, WIDE, 4, R><<<grid, kThreads, 0, s>>>(a, ng); break;
+    case 8: fp4_rows_kernel<WRITE, BF16, BLOCKS, WIDE, 8, R><<<grid, kThreads, 0, s>>>(a, ng); break;
+    default: fp4_rows_kernel<WRITE, BF16, BLOCKS, WIDE, 0, R><<<grid, kThreads, 0, s>>>(a, ng); break;
+  }
+}
+template <bool WRITE, bool BF16, bool BLOCKS, bool WIDE>
+void launch_r(const RowsArgs &a, int rows_at_once, dim3 grid, int ng, cudaStream_t s) {
+  if (rows_at_once == 16)
+    launch_ng<WRITE, BF16, BLOCKS, WIDE, 16>(a, grid, ng, s);
+  else
+    launch_ng<WRITE, BF16, BLOCKS, WIDE, 1>(a, grid, ng, s);
+}
+template <bool WRITE, bool BLOCKS>
+void launch_rows(const RowsArgs &a, bool bf16, bool wide, int r, dim3 grid, int ng, cudaStream_t s) {
+  if (bf16)
+    wide ? launch_r<WRITE, true, BLOCKS, true>(a, r, grid, ng, s) : launch_r<WRITE, true, BLOCKS, false>(a, r, grid, ng, s);
+  else
+    wide ? launch_r<WRITE, false, BLOCKS, true>(a, r, grid, ng, s) : launch_r<WRITE, false, BLOCKS, false>(a, r, grid, ng, s);
+}
+
+int check_geometry(const char *who, int kv_dim, int64_t num_blocks, int tpb, int heads, int head_size, int dtype) {
+  const std::string w(who);
+  if (kv_dim != 1 && kv_dim != 2) return fail(FKV_ERR_INVALID_ARG, w + ": kv_dim must be 1 or 2");
+  if (tpb <= 0 || tpb % 16) return fail(FKV_ERR_INVALID_ARG, w + ": tokens_per_block must be a positive multiple of 16");
+  if (head_size <= 0 || head_size % 16 || head_size > 65536)
+    return fail(FKV_ERR_INVALID_ARG, w + ": head_size must be a positive multiple of 16");
+  if (heads <= 0 || heads > 65536) return fail(FKV_ERR_INVALID_ARG, w + ": num_heads must be positive");
+  if ((int64_t)heads * head_size > (int64_t)1 << 24) return fail(FKV_ERR_INVALID_ARG, w + ": a token of more than 2^24 values");
+  if (num_blocks < 0 || num_blocks > INT64_MAX / tpb) return fail(FKV_ERR_INVALID_ARG, w + ": bad number of blocks");
+  if (dtype != FKV_DTYPE_BF16 && dtype != FKV_DTYPE_FP16)
+    return fail(FKV_ERR_UNSUPPORTED, w + ": the 16-bit side must be bfloat16 or half");
+  return FKV_OK;
+}
+
+bool aligned(int64_t v, int64_t to) { return v % to == 0; }
+bool aligned(const void *p, int64_t to) { return (uintptr_t)p % to == 0; }
+
+template <bool WRITE, bool BLOCKS>
+int run_rows(RowsArgs &a, int num_layers, int head_size, int dtype, bool wide, cudaStream_t s) {
+  const int ng = head_size / 16, r = a.num_rows < 16 ? 1 : 16;
+  // grid.x counts row groups: 2^31 - 1 of them is the launch limit
+  const int64_t gx = (a.num_rows + r - 1) / r;
+  if (gx > INT32_MAX) return fail(FKV_ERR_INVALID_ARG, "more than 2^31 groups of rows in one call");
+  launch_rows<WRITE, BLOCKS>(a, dtype == FKV_DTYPE_BF16, wide, r, dim3((unsigned)gx, num_layers * a.kv_dim), ng, s);
+  FKV_CUDA(cudaGetLastError());
+  note_launch();
+  return FKV_OK;
+}
+
+template <bool WRITE>
+int tokens_call(const char *who, void *layer, int kv_dim, int64_t num_blocks, int tpb, int heads, int head_size,
+                int64_t kv_stride, int64_t block_stride, const void *k, const void *v, int64_t k_token_stride,
+                int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, int dtype, const int64_t *slots,
+                int64_t num_tokens, void *stream) {
+  clear_error();
+  int rc = check_geometry(who, kv_dim, num_blocks, tpb, heads, head_size, dtype);
+  if (rc != FKV_OK) return rc;
+  const std::string w(who);
+  if (num_tokens < 0) return fail(FKV_ERR_INVALID_ARG, w + ": num_tokens must be non-negative");
+  if (num_tokens == 0) return FKV_OK;
+  if (!k || !slots || (kv_dim == 2 && !v) || (num_blocks > 0 && !layer))
+    return fail(FKV_ERR_INVALID_ARG, w + ": null pointer");
+  if (kv_dim == 1 && v) return fail(FKV_ERR_INVALID_ARG, w + ": a latent layer (kv_dim 1) has no values");
+  if (!aligned(layer, 16) || !aligned(kv_stride, 16) || !aligned(block_stride, 16))
+    return fail(FKV_ERR_MISALIGNED, w + ": the layer and its strides must be multiples of 16 bytes");
+  RowsArgs a{};
+  a.num_heads = heads, a.kv_dim = kv_dim, a.tokens_per_block = tpb;
+  a.num_rows = num_tokens, a.num_slots = num_blocks * tpb;
+  a.fp4_kv_stride = kv_stride, a.fp4_block_stride = block_stride;
+  a.token_stride[0] = k_token_stride, a.head_stride[0] = k_head_stride;
+  a.token_stride[1] = v_token_stride, a.head_stride[1] = v_head_stride;
+  a.fp4_ids = slots;
+  a.fp4[0] = (uint8_t *)layer;
+  a.rows[0][0] = (uint8_t *)k, a.rows[1][0] = (uint8_t *)v;
+  bool wide = true;
+  for (int i = 0; i < kv_dim; ++i) {
+    if (!aligned(a.rows[i][0], 16) || !aligned(a.token_stride[i], 16) || !aligned(a.head_stride[i], 16))
+      return fail(FKV_ERR_MISALIGNED, w + ": rows must start on 16-byte boundaries");
+    wide = wide && aligned(a.rows[i][0], 32) && aligned(a.token_stride[i], 32) && aligned(a.head_stride[i], 32);
+  }
+  return run_rows<WRITE, false>(a, 1, head_size, dtype, wide, (cudaStream_t)stream);
+}
+
+template <bool WRITE>
+int blocks_call(const char *who, int num_layers, void *const *fp4_layers, void *const *kv_layers, int kv_dim, int tpb,
+                int heads, int head_size, int64_t fp4_num_blocks, int64_t fp4_kv_stride, int64_t fp4_block_stride,
+                int64_t kv_num_blocks, int64_t kv_kv_stride, int64_t kv_block_stride, int dtype, const int64_t *fp4_ids,
+                const int64_t *kv_ids, int64_t num, void *stream) {
+  clear_error();
+  int rc = check_geometry(who, kv_dim, fp4_num_blocks, tpb, heads, head_size, dtype);
+  if (rc != FKV_OK) return rc;
+  const std::string w(who);
+  if (num < 0 || num_layers < 0 || kv_num_blocks < 0 || num > INT64_MAX / tpb)
+    return fail(FKV_ERR_INVALID_ARG, w + ": counts must be non-negative");
+  if (num == 0 || num_layers == 0) return FKV_OK;
+  if (!fp4_layers || !kv_layers || !fp4_ids || !kv_ids) return fail(FKV_ERR_INVALID_ARG, w + ": null pointer");
+  if (!aligned(fp4_kv_stride, 16) || !aligned(fp4_block_stride, 16) || !aligned(kv_kv_stride, 16) ||
+      !aligned(kv_block_stride, 16))
+    return fail(FKV_ERR_MISALIGNED, w + ": strides must be multiples of 16 bytes");
+  bool wide = aligned(kv_kv_stride, 32) && aligned(kv_block_stride, 32);
+  for (int l = 0; l < num_layers; ++l) {
+    if (!fp4_layers[l] || !kv_layers[l]) return fail(FKV_ERR_INVALID_ARG, w + ": null layer pointer");
+    if (!aligned(fp4_layers[l], 16) || !aligned(kv_layers[l], 16))
+      return fail(FKV_ERR_MISALIGNED, w + ": layers must start on 16-byte boundaries");
+    wide = wide && aligned(kv_layers[l], 32);
+  }
+  RowsArgs a{};
+  a.num_heads = heads, a.kv_dim = kv_dim, a.tokens_per_block = tpb;
+  a.num_rows = num * tpb, a.num_slots = fp4_num_blocks * tpb, a.num_row_slots = kv_num_blocks;
+  a.fp4_kv_stride = fp4_kv_stride, a.fp4_block_stride = fp4_block_stride;
+  a.row_block_stride = kv_block_stride;
+  for (int i = 0; i < 2; ++i) a.head_stride[i] = 2 * head_size, a.token_stride[i] = (int64_t)2 * head_size * heads;
+  a.fp4_ids = fp4_ids, a.row_ids = kv_ids;
+  for (int l0 = 0; l0 < num_layers; l0 += kMaxLayers) {
+    const int n = num_layers - l0 < kMaxLayers ? num_layers - l0 : kMaxLayers;
+    for (int l = 0; l < n; ++l) {
+      a.fp4[l] = (uint8_t *)fp4_layers[l0 + l];
+      a.rows[0][l] = (uint8_t *)kv_layers[l0 + l];
+      a.rows[1][l] = (uint8_t *)kv_layers[l0 + l] + kv_kv_stride;
+    }
+    if ((rc = run_rows<WRITE, true>(a, n, head_size, dtype, wide, (cudaStream_t)stream)) != FKV_OK) return rc;
+  }
+  return FKV_OK;
+}
+
+}  // namespace
+}  // namespace fkv
+
+extern "C" {
+
+int fkv_fp4_write(void *layer, int kv_dim, int64_t num_blocks, int tokens_per_block, int num_heads, int head_size,
+                  int64_t kv_stride_in_bytes, int64_t block_stride_in_bytes, const void *k, const void *v,
+                  int64_t k_token_stride_in_bytes, int64_t k_head_stride_in_bytes, int64_t v_token_stride_in_bytes,
+                  int64_t v_head_stride_in_bytes, int dtype, const int64_t *slots, int64_t num_tokens, void *stream) {
+  return fkv::tokens_call<true>("fkv_fp4_write", layer, kv_dim, num_blocks, tokens_per_block, num_heads, head_size,
+                                kv_stride_in_bytes, block_stride_in_bytes, k, v, k_token_stride_in_bytes,
+                                k_head_stride_in_bytes, v_token_stride_in_bytes, v_head_stride_in_bytes, dtype, slots,
+                                num_tokens, stream);
+}
+
+int fkv_fp4_read(const void *layer, int kv_dim, int64_t num_blocks, int tokens_per_block, int num_heads, int head_size,
+                 int64_t kv_stride_in_bytes, int64_t block_stride_in_bytes, void *k, void *v,
+                 int64_t k_token_stride_in_bytes, int64_t k_head_stride_in_bytes, int64_t v_token_stride_in_bytes,
+                 int64_t v_head_stride_in_bytes, int dtype, const int64_t *slots, int64_t num_tokens, void *stream) {
+  return fkv::tokens_call<false>("fkv_fp4_read", const_cast<void *>(layer), kv_dim, num_blocks, tokens_per_block,
+                                 num_heads, head_size, kv_stride_in_bytes, block_stride_in_bytes, k, v,
+                                 k_token_stride_in_bytes, k_head_stride_in_bytes, v_token_stride_in_bytes,
+                                 v_head_stride_in_bytes, dtype, slots, num_tokens, stream);
+}
+
+int fkv_fp4_pack_blocks(int num_layers, void *const *kv_layer_ptrs, void *const *fp4_layer_ptrs, int kv_dim,
+                        int tokens_per_block, int num_heads, int head_size, int64_t kv_num_blocks,
+                        int64_t kv_kv_stride_in_bytes, int64_t kv_block_stride_in_bytes, int64_t fp4_num_blocks,
+                        int64_t fp4_kv_stride_in_bytes, int64_t fp4_block_stride_in_bytes, int dtype,
+                        const int64_t *kv_block_ids, const int64_t *fp4_block_ids, int64_t num_blocks, void *stream) {
+  return fkv::blocks_call<true>("fkv_fp4_pack_blocks", num_layers, fp4_layer_ptrs, kv_layer_ptrs, kv_dim,
+                                tokens_per_block, num_heads, head_size, fp4_num_blocks, fp4_kv_stride_in_bytes,
+                                fp4_block_stride_in_bytes, kv_num_blocks, kv_kv_stride_in_bytes,
+                                kv_block_stride_in_bytes, dtype, fp4_block_ids, kv_block_ids, num_blocks, stream);
+}
+
+int fkv_fp4_unpack_blocks(int num_layers, void *const *fp4_layer_ptrs, void *const *kv_layer_ptrs, int kv_dim,
+                          int tokens_per_block, int num_heads, int head_size, int64_t fp4_num_blocks,
+                          int64_t fp4_kv_stride_in_bytes, int64_t fp4_block_stride_in_bytes, int64_t kv_num_blocks,
+                          int64_t kv_kv_stride_in_bytes, int64_t kv_block_stride_in_bytes, int dtype,
+                          const int64_t *fp4_block_ids, const int64_t *kv_block_ids, int64_t num_blocks, void *stream) {
+  return fkv::blocks_call<false>("fkv_fp4_unpack_blocks", num_layers, fp4_layer_ptrs, kv_layer_ptrs, kv_dim,
+                                 tokens_per_block, num_heads, head_size, fp4_num_blocks, fp4_kv_stride_in_bytes,
+                                 fp4_block_stride_in_bytes, kv_num_blocks, kv_kv_stride_in_bytes,
+                                 kv_block_stride_in_bytes, dtype, fp4_block_ids, kv_block_ids, num_blocks, stream);
+}
+
+}  // extern "C"

@@ -85,6 +85,17 @@ class KVCacheLayout:
     def get_total_elements(self) -> int:
         return prod(self.kv_shape)
 
+    def fp4(self) -> "KVCacheLayout":
+        """The same blocks held in 4 bits (fp4_cache): a layout of bytes
+        (uint8), head_size becoming the 9 / 16 byte a value that a token and
+        head take.  Its strides are those of the 4-bit layers and pools, for
+        every entry point that takes a layout or byte strides."""
+        if self.head_size % 16 or self.tokens_per_block % 16:
+            raise ValueError(f"head_size ({self.head_size}) and tokens_per_block "
+                             f"({self.tokens_per_block}) must be multiples of 16")
+        return KVCacheLayout(self.type, self.num_layer, self.num_block, self.tokens_per_block,
+                             self.num_head, self.head_size * 9 // 16, self.is_mla)
+
 
 def gpu_byte_strides(gpu_layout: KVCacheLayout, itemsize: int) -> dict:
     """Per-layer GPU strides as GPUCPUTransferWorker computes them

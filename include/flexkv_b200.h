@@ -574,6 +574,109 @@ int fkv_cache_index_take(fkv_cache_index *ci, int64_t num, int64_t *block_ids, i
  * length, snapshot offset, deleted table slots, table slots. */
 int fkv_cache_index_stats(fkv_cache_index *ci, int64_t *out, void *stream);
 
+/* ------------------------------------------------------------------------
+ * The KV cache in 4 bits: quantise tokens as they are written, read them
+ * back, convert whole blocks of every layer from and to a 16-bit cache, and
+ * attention that reads the 4-bit cache.  No counterpart in the reference,
+ * whose blocks keep the engine's type.
+ *
+ * 16 consecutive channels of one token and head form a group of 16 e2m1
+ * values (4 bits: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) and one
+ * scale byte c, which stands for the half-precision number with the bits
+ * c << 7: 4.5 bits a value.  scale = nearest(amax / 6), at most 10240; value =
+ * nearest(x / scale), both with ties to the even code.  Stored values are
+ * exact in bfloat16 and half.  NaN is stored as 0; what lies beyond +-61440,
+ * infinities too, saturates there.
+ *
+ * 16 tokens of one head are a unit of 9 * head_size bytes: 16 rows of
+ * head_size / 2 payload bytes (the even channel in the low four bits), then 16
+ * rows of head_size / 16 scale bytes.  A block of a layer is num_heads *
+ * tokens_per_block / 16 units, head by head: one chunk of tokens_per_block *
+ * num_heads * head_size * 9 / 16 bytes that every transfer entry point above
+ * moves as it is.  Side kv (0 keys, 1 values; kv_dim 1: one latent vector) of
+ * block b starts at layer + kv * kv_stride + b * block_stride.
+ * tokens_per_block and head_size are multiples of 16, the layer and its
+ * strides multiples of 16 bytes.
+ *
+ * All of these only enqueue work on `stream`, whose device must be current,
+ * allocate nothing and can be captured into a graph.  Ids, slots, tables and
+ * lengths are device memory and are checked in the kernels: what points
+ * outside a pool is skipped as described, never accessed.
+ * ---------------------------------------------------------------------- */
+#define FKV_DTYPE_BF16 0
+#define FKV_DTYPE_FP16 1
+
+/* Quantise num_tokens rows into their slots (slot = block *
+ * tokens_per_block + offset).  Row i of head h starts at k + i * token_stride
+ * + h * head_stride (bytes, multiples of 16) and holds head_size values of
+ * `dtype`; v likewise (NULL when kv_dim is 1).  A slot that is negative or
+ * past the pool drops its row.  The other slots must differ from one another:
+ * of rows given the same slot an unspecified mixture is stored. */
+int fkv_fp4_write(void *layer, int kv_dim, int64_t num_blocks, int tokens_per_block, int num_heads,
+                  int head_size, int64_t kv_stride_in_bytes, int64_t block_stride_in_bytes,
+                  const void *k, const void *v, int64_t k_token_stride_in_bytes,
+                  int64_t k_head_stride_in_bytes, int64_t v_token_stride_in_bytes,
+                  int64_t v_head_stride_in_bytes, int dtype, const int64_t *slots,
+                  int64_t num_tokens, void *stream);
+
+/* The rows of slots, as values of `dtype`; a slot that is negative or past
+ * the pool gives a row of zeros. */
+int fkv_fp4_read(const void *layer, int kv_dim, int64_t num_blocks, int tokens_per_block, int num_heads,
+                 int head_size, int64_t kv_stride_in_bytes, int64_t block_stride_in_bytes, void *k,
+                 void *v, int64_t k_token_stride_in_bytes, int64_t k_head_stride_in_bytes,
+                 int64_t v_token_stride_in_bytes, int64_t v_head_stride_in_bytes, int dtype,
+                 const int64_t *slots, int64_t num_tokens, void *stream);
+
+/* Blocks kv_block_ids[i] of a 16-bit cache (layers [kv_dim, blocks,
+ * tokens_per_block, num_heads, head_size], the block contiguous) into blocks
+ * fp4_block_ids[i] of the 4-bit cache, every layer in one launch (128 layers a
+ * launch).  The layer pointers are host arrays, the ids device memory.  A pair
+ * with an id outside its pool is skipped; fp4_block_ids must not repeat. */
+int fkv_fp4_pack_blocks(int num_layers, void *const *kv_layer_ptrs, void *const *fp4_layer_ptrs,
+                        int kv_dim, int tokens_per_block, int num_heads, int head_size,
+                        int64_t kv_num_blocks, int64_t kv_kv_stride_in_bytes,
+                        int64_t kv_block_stride_in_bytes, int64_t fp4_num_blocks,
+                        int64_t fp4_kv_stride_in_bytes, int64_t fp4_block_stride_in_bytes, int dtype,
+                        const int64_t *kv_block_ids, const int64_t *fp4_block_ids, int64_t num_blocks,
+                        void *stream);
+/* The other way: blocks fp4_block_ids[i] into blocks kv_block_ids[i], which
+ * must not repeat. */
+int fkv_fp4_unpack_blocks(int num_layers, void *const *fp4_layer_ptrs, void *const *kv_layer_ptrs,
+                          int kv_dim, int tokens_per_block, int num_heads, int head_size,
+                          int64_t fp4_num_blocks, int64_t fp4_kv_stride_in_bytes,
+                          int64_t fp4_block_stride_in_bytes, int64_t kv_num_blocks,
+                          int64_t kv_kv_stride_in_bytes, int64_t kv_block_stride_in_bytes, int dtype,
+                          const int64_t *fp4_block_ids, const int64_t *kv_block_ids, int64_t num_blocks,
+                          void *stream);
+
+/* Attention of new tokens over a 4-bit layer (kv_dim 2), head_size 64 or 128.
+ * q and out: num_q_tokens rows of num_q_heads vectors of `dtype` (token and
+ * head strides in bytes, multiples of 16); query head h reads key head h /
+ * (num_q_heads / num_kv_heads).  Sequence b owns the rows [cu_seqlens_q[b],
+ * cu_seqlens_q[b + 1]) (NULL: num_q_tokens / num_seqs rows each), has
+ * seq_lens[b] tokens in the cache, the new ones among them, and its token j in
+ * block block_tables[b * block_table_stride + j / tokens_per_block], of
+ * max_blocks entries.  Its row i sees the keys up to position seq_lens[b] -
+ * rows + i (causal != 0) or all of them.  A row that sees nothing gives zeros.
+ * Tokens past the table, or in a block outside the pool, count as hidden.
+ * Rows of no sequence are left as they were.  max_q_len: the most rows of a
+ * sequence, which only chooses the kernel.  lse (optional): float [num_q_tokens,
+ * num_q_heads], the natural logarithm of the sum of exponentials, -inf for a
+ * row that sees nothing.  workspace: device memory of at least
+ * fkv_fp4_attention_workspace bytes, 16-byte aligned, that nothing else uses
+ * until the call has run; its content does not matter. */
+int64_t fkv_fp4_attention_workspace(int64_t num_q_tokens, int num_q_heads, int num_kv_heads,
+                                    int head_size, int num_seqs, int max_q_len);
+int fkv_fp4_attention(const void *layer, int64_t num_blocks, int tokens_per_block, int num_kv_heads,
+                      int head_size, int64_t kv_stride_in_bytes, int64_t block_stride_in_bytes,
+                      const void *q, void *out, float *lse, int64_t q_token_stride_in_bytes,
+                      int64_t q_head_stride_in_bytes, int64_t out_token_stride_in_bytes,
+                      int64_t out_head_stride_in_bytes, int dtype, int64_t num_q_tokens,
+                      int num_q_heads, const int32_t *block_tables, int64_t block_table_stride,
+                      int max_blocks, const int32_t *seq_lens, const int32_t *cu_seqlens_q,
+                      int num_seqs, int max_q_len, float softmax_scale, int causal, void *workspace,
+                      int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
