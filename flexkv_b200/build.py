@@ -49,7 +49,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     tmp = LIB_PATH + ".tmp"
     cmd = [
         _nvcc(), *ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17",
-        "-Xcompiler", "-fPIC,-O3,-Wall", "-Xptxas", "-v", "-shared",
+        "-Xcompiler", "-fPIC,-O3,-Wall", "-Xptxas", "-v", "--threads", "0", "-shared",
         "-I", os.path.join(REPO_DIR, "include"),
         "-o", tmp, *[os.path.join(CSRC, s) for s in SOURCES], "-lpthread",
     ]

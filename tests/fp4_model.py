@@ -69,8 +69,8 @@ def write(layer: np.ndarray, rows, slots: np.ndarray) -> None:
 
 def attention(layer, q, tables, lens, cu, scale, causal, tpb):
     """q [tokens, Hq, D] in 64 bits.  Returns out, lse, the sum of weights times |v| (what errors of the
-    weights scale with) and the largest scale * sum |q| |k| of each row (what errors of the scores scale with);
-    rows of no sequence stay NaN."""
+    weights scale with; 2^-21 of the sum of |v| is in it, see attention_bounds) and the largest scale * sum |q| |k|
+    of each row (what errors of the scores scale with); rows of no sequence stay NaN."""
     h = layer.shape[2]
     n, hq, d = q.shape
     g = hq // h
@@ -97,7 +97,7 @@ def attention(layer, q, tables, lens, cu, scale, causal, tpb):
                 m = s.max()
                 p = np.exp(s - m)
                 out[lo + i, qh] = p @ vs / p.sum()
-                weight[lo + i, qh] = p @ np.abs(vs) / p.sum()
+                weight[lo + i, qh] = p @ np.abs(vs) / p.sum() + 2.0 ** -21 * np.abs(vs).sum(0)
                 lse[lo + i, qh] = m + np.log(p.sum())
                 size[lo + i, qh] = (np.abs(ks) @ np.abs(x)).max() * abs(scale)
     return out, lse, weight, size
