@@ -8,6 +8,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "fkv_common.h"
@@ -20,6 +21,8 @@ struct AttnArgs {
   const uint8_t *layer;
   int64_t num_blocks, kv_stride, block_stride;
   int tokens_per_block, kv_heads, group;
+  int upb;             // units of a block
+  uint64_t upb_magic;  // u / upb = (u * upb_magic) >> 40 for u < 2^28, upb <= 2^12
   const uint8_t *q;
   int64_t q_token_stride, q_head_stride;  // bytes
   uint8_t *out;
@@ -30,7 +33,9 @@ struct AttnArgs {
   int64_t table_stride;
   int max_blocks;
   const int32_t *seq_lens;
-  const int32_t *cu;  // null: num_q / num_seqs rows each
+  const int32_t *cu;  // null: rows_each rows each
+  int rows_each;
+  int table_tokens;  // tokens that a table's width holds
   int num_seqs;
   float scale;
   int causal;
@@ -40,24 +45,33 @@ __device__ __forceinline__ float natural_lse(float m, float l) {  // m: in power
   return l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
 }
 
-// Four channels from c on of (token, head) row `row` of a sequence.
-template <bool BF16>
-__device__ __forceinline__ void store_row(const AttnArgs &a, int64_t first, int h, int64_t row, int64_t nrows, int c, float4 v,
-                                          float m, float l) {
+// N channels from c on of (token, head) row `row` of a sequence.
+template <bool BF16, int N>
+__device__ __forceinline__ void store_row(const AttnArgs &a, int64_t first, int h, int row, int nrows, int c,
+                                          const float (&v)[N], float m, float l) {
   if (row >= nrows) return;
-  const int64_t tok = first + row / a.group;
-  const int qh = h * a.group + (int)(row % a.group);
+  const int i = row / a.group, qh = h * a.group + row - i * a.group;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  uint2 w;
-  if (BF16) {
-    __nv_bfloat162 x = __floats2bfloat162_rn(v.x * inv, v.y * inv), y = __floats2bfloat162_rn(v.z * inv, v.w * inv);
-    w.x = *reinterpret_cast<uint32_t *>(&x), w.y = *reinterpret_cast<uint32_t *>(&y);
-  } else {
-    __half2 x = __floats2half2_rn(v.x * inv, v.y * inv), y = __floats2half2_rn(v.z * inv, v.w * inv);
-    w.x = *reinterpret_cast<uint32_t *>(&x), w.y = *reinterpret_cast<uint32_t *>(&y);
+  uint32_t w[N / 2];
+#pragma unroll
+  for (int k = 0; k < N / 2; ++k) {
+    if (BF16) {
+      const __nv_bfloat162 x = __floats2bfloat162_rn(v[2 * k] * inv, v[2 * k + 1] * inv);
+      w[k] = *reinterpret_cast<const uint32_t *>(&x);
+    } else {
+      const __half2 x = __floats2half2_rn(v[2 * k] * inv, v[2 * k + 1] * inv);
+      w[k] = *reinterpret_cast<const uint32_t *>(&x);
+    }
   }
-  *reinterpret_cast<uint2 *>(a.out + tok * a.o_token_stride + qh * a.o_head_stride + 2 * c) = w;
-  if (a.lse && c == 0) a.lse[tok * (a.kv_heads * a.group) + qh] = natural_lse(m, l);
+  uint8_t *dst = a.out + (first + i) * a.o_token_stride + qh * a.o_head_stride + 2 * c;
+  if constexpr (N >= 8) {
+#pragma unroll
+    for (int k = 0; k < N / 8; ++k)
+      reinterpret_cast<uint4 *>(dst)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+  } else {
+    *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
+  }
+  if (a.lse && c == 0) a.lse[(first + i) * (a.kv_heads * a.group) + qh] = natural_lse(m, l);
 }
 
 // ---- few rows: decoding, and checking a handful of proposed tokens ----------
@@ -83,16 +97,23 @@ __device__ __forceinline__ void store_row(const AttnArgs &a, int64_t first, int 
 // sum of weights is taken before the rounding, in 32 bits).
 //
 // The sequences' units (16 tokens) x key heads x blocks of R rows form one
-// line of work that is cut into equal pieces, one for each CTA, whatever the
-// lengths are; they are read on the device, so a captured launch follows them.
-// Within a CTA every warp has its own ring of bulk copies, takes chunks of up
-// to kUps units in turn and keeps its own running maximum, sum and O; they are
-// joined once for each (sequence, head), and pieces of one (sequence, head) in
-// several CTAs by a second small kernel, in a fixed order.
+// line of work that is cut into equal pieces, one for each warp of the GPU,
+// whatever the lengths are; they are read on the device, so a captured launch
+// follows them.  A warp walks through its piece by itself, with its own ring
+// of asynchronous copies that runs ahead over the borders of sequences and
+// heads, and its own running sum, maximum and O.  What it holds whole it
+// writes out; the rest is joined once at the end within the CTA, and pieces of
+// one (sequence, head) in several CTAs by a second small kernel, both in a
+// fixed order.
 
-constexpr int kWarps = 8;
-constexpr int kUps = 2;     // units of a chunk
-constexpr int kStages = 4;  // chunks of a warp's ring
+// Warps of a CTA, units of a chunk and chunks of a warp's ring, for NT row tiles.
+template <int NT>
+struct DecodeShape {
+  static constexpr int kWarps = NT == 1 ? 12 : NT == 2 ? 8 : 4;
+  static constexpr int kUps = 2;
+  static constexpr int kStages = NT == 4 ? 4 : 3;
+};
+
 constexpr float kNone = -1e30f;  // a row's base before any key
 // A weight is 2^(score - base).  The base is set 7 below the largest score and
 // moves when one passes it by 15: the largest weight of a row lies between
@@ -100,13 +121,13 @@ constexpr float kNone = -1e30f;  // a row's base before any key
 // at most 2^-32 of the sum of weights from any weight, however small.
 constexpr float kLift = 7.0f, kMove = 15.0f;
 
-struct Item {  // what a CTA needs of one sequence
-  int64_t len;      // tokens that can be seen: the table's end at most
-  int64_t len_q;    // tokens as given: positions count from here
-  int64_t first;    // first row in q
-  int rows;         // new tokens
-  int blocks;       // blocks of R (token, head) rows
-  int64_t units;    // units to pass, at least one where there are rows
+struct Item {     // what a warp needs of one sequence
+  int len;        // tokens that can be seen: the table's end at most
+  int len_q;      // tokens as given: positions count from here
+  int64_t first;  // first row in q
+  int rows;       // new tokens
+  int blocks;     // blocks of R (token, head) rows
+  int units;      // units to pass, at least one where there are rows
 };
 
 template <int R>
@@ -116,57 +137,66 @@ __device__ __forceinline__ Item item_of(const AttnArgs &a, int b) {
     const int64_t lo = min((int64_t)max(a.cu[b], 0), a.num_q), hi = min((int64_t)max(a.cu[b + 1], 0), a.num_q);
     it.first = lo, it.rows = (int)max(hi - lo, (int64_t)0);
   } else {
-    it.rows = (int)(a.num_q / a.num_seqs);
-    it.first = (int64_t)b * it.rows;
+    it.rows = a.rows_each;
+    it.first = (int64_t)b * a.rows_each;
   }
   it.len_q = a.seq_lens[b];
-  it.len = min(max(it.len_q, (int64_t)0), (int64_t)a.max_blocks * a.tokens_per_block);
-  it.blocks = (int)(((int64_t)it.rows * a.group + R - 1) / R);
-  it.units = it.rows ? max((it.len + 15) / 16, (int64_t)1) : 0;
+  it.len = min(max(it.len_q, 0), a.table_tokens);
+  it.blocks = (it.rows * a.group + R - 1) / R;
+  it.units = it.rows ? max((it.len + 15) >> 4, 1) : 0;
   return it;
 }
 
-// Where a CTA's piece starts, found by every CTA for itself.
-struct Start {
-  int64_t total;   // units of all work
+// The cut of all work into pieces, and where this CTA's starts; every CTA
+// finds it for itself.
+struct Cut {
+  int64_t each, more;  // a CTA has each + 1 units, from CTA `more` on each
   int64_t begin, end;
-  int ctas;
   int b;           // sequence of `begin`
   int64_t before;  // units before sequence b
+  __device__ int cta_of(int64_t x) const {
+    return (int)(x < (each + 1) * more ? x / (each + 1) : more + (x - (each + 1) * more) / each);
+  }
 };
 
-template <int R>
-__device__ void find_start(const AttnArgs &a, int ctas, Start *out, int64_t *scratch /* kWarps */) {
-  const int per = (a.num_seqs + kWarps * 32 - 1) / (kWarps * 32);
-  const int b0 = min(threadIdx.x * per, a.num_seqs), b1 = min(b0 + per, a.num_seqs);
+template <int R, int kWarps>
+__device__ void find_cut(const AttnArgs &a, Cut *out, int64_t *scratch /* kWarps */) {
+  const int per = (a.num_seqs + kWarps * 32 - 1) / (kWarps * 32), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b0 = min((int)threadIdx.x * per, a.num_seqs), b1 = min(b0 + per, a.num_seqs);
   int64_t mine = 0;
   for (int b = b0; b < b1; ++b) {
     const Item it = item_of<R>(a, b);
-    mine += it.units * it.blocks * a.kv_heads;
+    mine += (int64_t)it.units * (it.blocks * a.kv_heads);
   }
   int64_t upto = mine;
 #pragma unroll
   for (int i = 1; i < 32; i <<= 1) {
     const int64_t o = __shfl_up_sync(~0u, upto, i);
-    if ((threadIdx.x & 31) >= i) upto += o;
+    if (lane >= i) upto += o;
   }
-  if ((threadIdx.x & 31) == 31) scratch[threadIdx.x >> 5] = upto;
+  if (lane == 31) scratch[warp] = upto;
   __syncthreads();
   int64_t total = 0;
+#pragma unroll
   for (int w = 0; w < kWarps; ++w) {
-    if (w < (threadIdx.x >> 5)) upto += scratch[w];
+    if (w < warp) upto += scratch[w];
     total += scratch[w];
   }
   const int64_t want = (total + kWarps - 1) / kWarps;  // a unit for each warp, at least
-  const int n = (int)(want < ctas ? want : ctas);
-  const int64_t begin = blockIdx.x < n ? blockIdx.x * total / n : total;
-  const int64_t end = blockIdx.x < n ? (blockIdx.x + 1) * total / n : total;
-  if (threadIdx.x == 0) out->total = total, out->begin = begin, out->end = end, out->ctas = n;
+  const uint32_t n = want < gridDim.x ? (uint32_t)want : gridDim.x;
+  int64_t each = 0, more = 0;
+  if (n) {
+    each = total >> 32 ? total / n : (uint32_t)total / n;
+    more = total - each * n;
+  }
+  const int64_t c = blockIdx.x;
+  const int64_t begin = c < n ? c * each + min(c, more) : total, end = c < n ? begin + each + (c < more) : total;
   int64_t at = upto - mine;
+  if (threadIdx.x == 0) out->each = each, out->more = more, out->begin = begin, out->end = end;
   if (begin >= at && begin < upto) {
     for (int b = b0; b < b1; ++b) {
       const Item it = item_of<R>(a, b);
-      const int64_t w = it.units * it.blocks * a.kv_heads;
+      const int64_t w = (int64_t)it.units * (it.blocks * a.kv_heads);
       if (begin < at + w) {
         out->b = b, out->before = at;
         break;
@@ -177,81 +207,80 @@ __device__ void find_start(const AttnArgs &a, int ctas, Start *out, int64_t *scr
   __syncthreads();
 }
 
-// A walk over a CTA's piece: segments (the part of one (sequence, head, row
-// block) in it), and a warp's chunks in them.
-template <int R>
+// A walk over a warp's part of the line of work: segments (the part of one
+// (sequence, head, row block) in it), and chunks of kUps units in them.
+template <int R, int kUps>
 struct Walk {
-  int64_t left;      // units of the piece from u0 on
-  int b, idx;        // sequence; (head, row block) in it
+  int left;      // units of the part from u0 on
+  int b, idx;    // sequence; (head, row block) in it
+  int h, rb;
   Item it;
-  int64_t u0, u1;    // units of the segment
-  int64_t at;        // this warp's next chunk
-  int step;          // units of a chunk
+  int u0, u1;    // units of the segment
+  int at;        // the next chunk
 
-  __device__ void start(const AttnArgs &a, const Start &s, int warp) {
-    left = s.end - s.begin;
-    if (left <= 0) return;
-    b = s.b;
-    it = item_of<R>(a, b);
-    const int64_t off = s.begin - s.before;
-    idx = (int)(off / it.units);
-    u0 = off - (int64_t)idx * it.units;
-    open(warp);
+  // `off`: the part's start, from that of sequence `seq` on
+  __device__ void start(const AttnArgs &a, int seq, int64_t off, int units) {
+    left = units;
+    b = seq;
+    for (;;) {
+      it = item_of<R>(a, b);
+      const int64_t w = (int64_t)it.units * (it.blocks * a.kv_heads);
+      if (off < w) break;
+      off -= w, ++b;  // the part has units, so this ends
+    }
+    idx = (int)(off >> 32 ? off / it.units : (uint32_t)off / (uint32_t)it.units);
+    u0 = (int)(off - (int64_t)idx * it.units);
+    open();
   }
-  __device__ void open(int warp) {
+  __device__ void open() {
+    h = it.blocks == 1 ? idx : idx / it.blocks, rb = idx - h * it.blocks;
     u1 = min(it.units, u0 + left);
-    const int64_t share = (u1 - u0 + kWarps - 1) / kWarps;
-    step = (int)min(share, (int64_t)kUps);
-    at = u0 + (int64_t)warp * step;
+    at = u0;
   }
-  // To the next segment; false at the end of the piece.
-  __device__ bool next_segment(const AttnArgs &a, int warp) {
+  // To the next segment; false at the end of the part.
+  __device__ bool next_segment(const AttnArgs &a) {
     left -= u1 - u0;
     if (left <= 0) return false;
     u0 = 0;
     if (++idx == it.blocks * a.kv_heads) {
       idx = 0;
       do it = item_of<R>(a, ++b);
-      while (it.units * it.blocks == 0);  // there is work left, so this ends
+      while (it.blocks == 0);  // there is work left, so this ends
     }
-    open(warp);
+    open();
     return true;
   }
-  __device__ void next_chunk() { at += kWarps * step; }
+  __device__ void next_chunk() { at += kUps; }
   __device__ bool has_chunk() const { return at < u1; }
-  __device__ int chunk_units() const { return (int)min((int64_t)step, u1 - at); }
+  __device__ int chunk_units() const { return min(kUps, u1 - at); }
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void mbar_init(uint64_t *m, int count) {
-  asm volatile("mbarrier.init.shared.b64 [%0], %1;" ::"r"(smem_addr(m)), "r"(count) : "memory");
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void mbar_expect(uint64_t *m, int bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared.b64 _, [%0], %1;" ::"r"(smem_addr(m)), "r"(bytes) : "memory");
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ bool mbar_try(uint64_t *m, int parity) {
-  int ok;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared.b64 p, [%1], %2, %3;\n selp.b32 %0, 1, 0, p;\n}"
-      : "=r"(ok)
-      : "r"(smem_addr(m)), "r"(parity), "r"(1000000)
-      : "memory");
-  return ok;
+template <int WORDS>
+__device__ __forceinline__ void load_shared(uint32_t (&w)[WORDS], uint32_t at) {
+  if constexpr (WORDS == 4)
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
+  else if constexpr (WORDS == 2)
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at));
+  else
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(at));
 }
-__device__ __forceinline__ void bulk_load(void *dst, const void *src, int bytes, uint64_t *m) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   smem_addr(dst)),
-               "l"(src), "r"(bytes), "r"(smem_addr(m))
-               : "memory");
-}
-// Waits with a limit (a try waits up to a millisecond by itself): one that
-// runs out is counted, and the data is taken as it is.
-__device__ unsigned long long g_wait_timeouts;
-__device__ __forceinline__ bool mbar_wait(uint64_t *m, int parity, int tries) {
-  for (int i = 0; i < tries; ++i)
-    if (mbar_try(m, parity)) return true;
-  if ((threadIdx.x & 31) == 0) atomicAdd(&g_wait_timeouts, 1ull);
-  return false;
+template <int BYTES>
+__device__ __forceinline__ uint32_t load_scales(uint32_t at) {
+  uint32_t r;
+  if constexpr (BYTES == 2)
+    asm volatile("{\n .reg .b16 h;\n ld.shared.b16 h, [%1];\n cvt.u32.u16 %0, h;\n}" : "=r"(r) : "r"(at));
+  else
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(r) : "r"(at));
+  return r;
 }
 
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -291,179 +320,217 @@ struct SplitMeta {  // of a CTA: the (sequence, head, row block) that starts in 
   int b, idx;
 };
 
+// What a warp has of a (sequence, head, row block) that it does not hold whole.
+template <int D, int NT>
+struct Part {
+  static constexpr int kPad = D + 4;  // floats of a row: quads store 16-byte pieces of rows 2 t and 2 t + 1
+  alignas(16) float o[8 * NT][kPad];
+  float m[8 * NT], l[8 * NT];
+};
+struct PartMeta {
+  int there, starts, ends, b, idx;
+  int64_t last;  // the (sequence, head, row block)'s last unit in the line of work, where it starts here
+};
+
 template <int D, int NT>
 struct DecodeSmem {
-  static constexpr int kUnit = 9 * D;
-  static constexpr int kPad = D + 4;  // floats of a row in the join: quads store 16-byte pieces of rows 2 t and 2 t + 1
-  alignas(128) uint8_t ring[kWarps][kStages][kUps][2][kUnit];
-  alignas(16) float o[kWarps][8][kPad];
-  float m[kWarps][8 * NT], l[kWarps][8 * NT];
-  uint64_t full[kWarps][kStages];
-  Start start;
+  static constexpr int kWarps = DecodeShape<NT>::kWarps, kUps = DecodeShape<NT>::kUps, kStages = DecodeShape<NT>::kStages;
+  alignas(128) uint8_t ring[kWarps][kStages][kUps][2][9 * D];  // at the end: the part that starts in the warp
+  Part<D, NT> part[kWarps];                                     // the part that goes on from the warp before
+  PartMeta meta[kWarps][2];
+  Cut cut;
   int64_t scratch[kWarps];
+  static_assert(sizeof(Part<D, NT>) <= sizeof(ring[0]), "a part has to fit a warp's ring");
 };
 
 template <int D>
 __host__ __device__ constexpr int slot_floats(int rows) { return rows * (D + 2); }
 
 template <int D, int NT, bool BF16>
-__global__ void __launch_bounds__(kWarps * 32, 1)
+__global__ void __launch_bounds__(DecodeShape<NT>::kWarps * 32, 1)
 fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ parts, SplitMeta *__restrict__ meta) {
   constexpr int R = 8 * NT, KS = D / 16, KW = D / 32, VB = D / 16;  // k-steps; words of a lane's K row; bytes of its V row
-  extern __shared__ uint8_t smem_raw[];
+  constexpr int kWarps = DecodeShape<NT>::kWarps, kUps = DecodeShape<NT>::kUps, kStages = DecodeShape<NT>::kStages;
+  constexpr int kUnit = 9 * D, kSlot = kUps * 2 * kUnit, kBatch = 32 / kUps;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
   auto &sm = *reinterpret_cast<DecodeSmem<D, NT> *>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   // the next kernel only starts its CTAs early; it waits for this one's end before it reads
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (lane == 0) {
-    for (int s = 0; s < kStages; ++s) mbar_init(&sm.full[warp][s], 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  find_start<R>(a, gridDim.x, &sm.start, sm.scratch);
-  const Start st = sm.start;
   if (threadIdx.x == 0) meta[blockIdx.x].last = -1;
-  if (st.begin >= st.end) return;
+  if (lane < 2) sm.meta[warp][lane].there = 0;
+  find_cut<R, kWarps>(a, &sm.cut, sm.scratch);
+  const int64_t begin = sm.cut.begin;
+  const int units_here = (int)(sm.cut.end - begin);
+  if (units_here <= 0) return;
+  const int from = (int)((int64_t)units_here * warp / kWarps), to = (int)((int64_t)units_here * (warp + 1) / kWarps);
 
-  Walk<R> in, cur;  // the copies' walk runs ahead
-  in.start(a, st, warp);
-  cur = in;
-  bool more = true;
-  int64_t page = -1;
-  const int units_per_block = a.tokens_per_block / 16;
-  auto settle = [&] {  // to a segment with a chunk for this warp, and on to its pages
-    while (more && !in.has_chunk()) more = in.next_segment(a, warp);
-    if (more && lane < 2 * in.chunk_units()) {
-      const int64_t u = in.at + (lane >> 1), e = u / units_per_block;
-      page = e < a.max_blocks ? a.tables[in.b * a.table_stride + e] : -1;
-    }
-  };
-  uint32_t valid = 0;  // bit kUps * stage + unit: the unit's page is in the pool and its copy was started
-  int alive = 1000;    // tries of a wait; after one ran out, a single one
-  auto issue = [&](int stage) {
-    const int n = more ? in.chunk_units() : 0;
-    if (n == 0) return;
-    const bool good = lane < 2 * n && page >= 0 && page < a.num_blocks;
-    const uint32_t ok = __ballot_sync(~0u, good);
-    uint32_t mask = 0;
+  if (from < to) {
+    Walk<R, kUps> in, cur;  // the copies' walk runs ahead
+    in.start(a, sm.cut.b, begin + from - sm.cut.before, to - from);
+    cur = in;
+    const uint32_t ring = smem_addr(sm.ring[warp]);
+    bool more = true;
+    // Where the segment's next 32 units lie, one for each lane: bytes from the layer's start, -1 for a page
+    // outside the pool; and the pages of the 32 after them, on their way.
+    int64_t where = -1;
+    int next_page = -1, turn = 0;
+    auto page_of = [&](int u) {
+      const int e = (int)(((uint64_t)u * a.upb_magic) >> 40);  // u / units of a block
+      return u < in.u1 && e < a.max_blocks ? a.tables[in.b * a.table_stride + e] : -1;
+    };
+    auto take_batch = [&] {
+      const int u = in.at + lane, e = (int)(((uint64_t)u * a.upb_magic) >> 40);
+      where = next_page < 0 || next_page >= a.num_blocks
+                  ? -1
+                  : next_page * a.block_stride + ((int64_t)in.h * a.upb + u - e * a.upb) * kUnit;
+      next_page = page_of(u + 32);
+      turn = 0;
+    };
+    uint32_t valid = 0;  // bit kUps * stage + unit: the unit's page is in the pool and its copy was started
+    auto issue = [&](int stage) {
+      if (more) {
+        const int n = in.chunk_units();
+        uint32_t mask = 0;
 #pragma unroll
-    for (int u = 0; u < kUps; ++u) mask |= ((ok >> (2 * u)) & 1) << u;
-    valid = (valid & ~(((1u << kUps) - 1) << (kUps * stage))) | (mask << (kUps * stage));
-    if (lane == 0) mbar_expect(&sm.full[warp][stage], __popc(ok) * 9 * D);
-    __syncwarp();
-    if (good) {
-      const int64_t u = in.at + (lane >> 1);
-      const int h = in.idx / in.it.blocks;
-      const uint8_t *src = a.layer + (lane & 1) * a.kv_stride + page * a.block_stride +
-                           ((int64_t)h * units_per_block + u % units_per_block) * (9 * D);
-      bulk_load(sm.ring[warp][stage][lane >> 1][lane & 1], src, 9 * D, &sm.full[warp][stage]);
-    }
-    in.next_chunk();
-    settle();
-  };
-  settle();
+        for (int u = 0; u < kUps; ++u) {
+          const int64_t off = __shfl_sync(~0u, where, turn * kUps + u);
+          if (u < n && off >= 0) {
+            mask |= 1u << u;
+            const uint32_t dst = ring + stage * kSlot + u * 2 * kUnit + lane * 16;
+            const uint8_t *src = a.layer + off + lane * 16, *srcv = src + a.kv_stride;
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) issue(s);
-  int stage = 0, phase = 0;
-
-  for (;;) {  // segments
-    const int h = cur.idx / cur.it.blocks, rb = cur.idx % cur.it.blocks;
-    const int64_t row0 = (int64_t)rb * R;  // of the sequence's (token, head) rows
-    const int64_t nrows = (int64_t)cur.it.rows * a.group;
-    // queries, n = g, channels D / 4 * t on; multiplier and end of the rows 2 t, 2 t + 1
-    uint32_t qf[NT][KS][2];
-    float mul[NT][2];
-    int64_t end[NT][2], lowest = INT64_MAX, highest = 0;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int64_t r = row0 + n * 8 + g;
-      float x[D / 4];
-      float amax = 0;
-      if (r < nrows) {
-        const uint8_t *p = a.q + (cur.it.first + r / a.group) * a.q_token_stride +
-                           (h * a.group + r % a.group) * a.q_head_stride + t * (D / 2);
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          const uint4 v = reinterpret_cast<const uint4 *>(p)[i];
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 f = pair_to_float2<BF16>(w[j]);
-            x[8 * i + 2 * j] = f.x, x[8 * i + 2 * j + 1] = f.y;
-            amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+            for (int i = 0; i < kUnit / 512; ++i) {
+              copy16(dst + i * 512, src + i * 512);
+              copy16(dst + kUnit + i * 512, srcv + i * 512);
+            }
+            if (lane < kUnit % 512 / 16) {
+              copy16(dst + kUnit / 512 * 512, src + kUnit / 512 * 512);
+              copy16(dst + kUnit + kUnit / 512 * 512, srcv + kUnit / 512 * 512);
+            }
           }
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < D / 4; ++i) x[i] = 0;
+        valid = (valid & ~(((1u << kUps) - 1) << (kUps * stage))) | (mask << (kUps * stage));
+        in.next_chunk();
+        if (!in.has_chunk()) {
+          more = in.next_segment(a);
+          if (more) {
+            next_page = page_of(in.at + lane);
+            take_batch();
+          }
+        } else if (++turn == kBatch) {
+          take_batch();
+        }
       }
-      amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
-      amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
-      const float f = row_factor(amax);
+      copies_commit();
+    };
+    next_page = page_of(in.at + lane);
+    take_batch();
 #pragma unroll
-      for (int k = 0; k < KS; ++k)
+    for (int s = 0; s < kStages - 1; ++s) issue(s);
+    int stage = 0;
+    // a lane's places in a unit: its pieces of keys and values and of their scales
+    const int tok = (g & 1) ? ((g >> 1) ^ 1) + 4 : (g >> 1);  // S^T: rows g, g + 8 are tokens tok, tok + 8
+    const int tk[2] = {t, (t ^ 1) + 4};                       // tokens of rows 2 t, 2 t + 1
+    const uint32_t at_k = tok * (D / 2) + t * (D / 8), at_ks = 8 * D + tok * (D / 16) + t * (D / 64);
+    const uint32_t at_v[2] = {kUnit + tk[0] * (D / 2) + g * VB, kUnit + tk[1] * (D / 2) + g * VB};
+    const uint32_t at_vs[2] = {kUnit + 8 * D + tk[0] * (D / 16) + g * D / 128,
+                               kUnit + 8 * D + tk[1] * (D / 16) + g * D / 128};
+
+    for (;;) {  // segments
+      const int h = cur.h;
+      const int row0 = cur.rb * R, nrows = cur.it.rows * a.group;  // of the sequence's (token, head) rows
+      // queries, n = g, channels D / 4 * t on; multiplier and end of the rows 2 t, 2 t + 1
+      uint32_t qf[NT][KS][2];
+      float mul[NT][2], bar[NT][2];  // bar: the sum q k past which the row's base moves
+      int end[NT][2], lowest = INT32_MAX, highest = 0;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) qf[n][k][j] = pack_half2(x[4 * k + 2 * j] * f, x[4 * k + 2 * j + 1] * f);
-      const float mine = a.scale * 1.4426950408889634f * (1.0f / f);
+      for (int n = 0; n < NT; ++n) {
+        const int r = row0 + n * 8 + g;
+        uint32_t x[D / 8];
+        float amax = 0;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        mul[n][j] = __shfl_sync(~0u, mine, (2 * t + j) * 4);
-        const int64_t rr = row0 + n * 8 + 2 * t + j;
-        int64_t e = 0;
-        if (rr < nrows) e = a.causal ? min(cur.it.len, cur.it.len_q - cur.it.rows + rr / a.group + 1) : cur.it.len;
-        end[n][j] = e;
-        if (rr < nrows) lowest = min(lowest, e);
-        highest = max(highest, e);
+        for (int i = 0; i < D / 8; ++i) x[i] = 0;
+        if (r < nrows) {
+          const int i0 = r / a.group;
+          const uint8_t *p = a.q + (cur.it.first + i0) * a.q_token_stride +
+                             (h * a.group + r - i0 * a.group) * a.q_head_stride + t * (D / 2);
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) {
+            const uint4 v = reinterpret_cast<const uint4 *>(p)[i];
+            x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const float2 f = pair_to_float2<BF16>(x[i]);
+          amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
+        // a negative softmax_scale goes into the queries: the multiplier is positive, and so that no score is 0 * inf
+        const float f = row_factor(amax), fs = a.scale < 0.0f ? -f : f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float2 y = pair_to_float2<BF16>(x[2 * k + j]);
+            qf[n][k][j] = pack_half2(y.x * fs, y.y * fs);
+          }
+        const float mine = fmaxf(fabsf(a.scale) * 1.4426950408889634f * (1.0f / f), 1e-37f);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          mul[n][j] = __shfl_sync(~0u, mine, (2 * t + j) * 4);
+          bar[n][j] = -INFINITY;
+          const int rr = row0 + n * 8 + 2 * t + j;
+          int e = 0;
+          if (rr < nrows) {
+            e = cur.it.len;
+            if (a.causal) e = max(min(e, cur.it.len_q - cur.it.rows + rr / a.group + 1), 0);
+            lowest = min(lowest, e);
+          }
+          end[n][j] = e;
+          highest = max(highest, e);
+        }
       }
-    }
 #pragma unroll
-    for (int i = 1; i < 4; i <<= 1) {
-      lowest = min(lowest, __shfl_xor_sync(~0u, lowest, i));
-      highest = max(highest, __shfl_xor_sync(~0u, highest, i));
-    }
+      for (int i = 1; i < 4; i <<= 1) {
+        lowest = min(lowest, __shfl_xor_sync(~0u, lowest, i));
+        highest = max(highest, __shfl_xor_sync(~0u, highest, i));
+      }
 
-    float o[NT][KS][4], m[NT][2], l[NT][2];
+      float o[NT][KS][4], m[NT][2], l[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+      for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int k = 0; k < KS; ++k)
+        for (int k = 0; k < KS; ++k)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[n][k][i] = 0;
-      m[n][0] = m[n][1] = kNone;
-      l[n][0] = l[n][1] = 0;
-    }
+          for (int i = 0; i < 4; ++i) o[n][k][i] = 0;
+        m[n][0] = m[n][1] = kNone;
+        l[n][0] = l[n][1] = 0;
+      }
 
-    for (; cur.has_chunk(); cur.next_chunk()) {
-      const uint32_t ok = (valid >> (kUps * stage)) & ((1u << kUps) - 1);
-      if (!mbar_wait(&sm.full[warp][stage], phase, alive)) alive = 1;
-      __syncwarp();  // and every lane is done with the chunk before, whose slot is the next to fill
-      issue((stage + kStages - 1) % kStages);
-      float s[kUps][NT][4];
-      // S^T: rows g, g + 8 are tokens tok, tok + 8
-      const int tok = (g & 1) ? ((g >> 1) ^ 1) + 4 : (g >> 1);
-#pragma unroll
-      for (int u = 0; u < kUps; ++u) {
-        const uint8_t *K = sm.ring[warp][stage][u][0];
+      auto unit = [&](uint32_t slot, int base, bool there) {
+        float s[NT][4];
         uint32_t w[2][KW], sc[2][(D + 127) / 128 * 2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint8_t *row = K + (tok + 8 * i) * (D / 2) + t * (D / 8);
-          if constexpr (D == 128) {
-            const uint4 v = *reinterpret_cast<const uint4 *>(row);
-            w[i][0] = v.x, w[i][1] = v.y, w[i][2] = v.z, w[i][3] = v.w;
-            const uint32_t c = *reinterpret_cast<const uint16_t *>(K + 8 * D + (tok + 8 * i) * (D / 16) + 2 * t);
-            sc[i][0] = __byte_perm(c, 0, 0x0404) >> 1;
-            sc[i][1] = __byte_perm(c, 0, 0x1414) >> 1;
-          } else {
-            const uint2 v = *reinterpret_cast<const uint2 *>(row);
-            w[i][0] = v.x, w[i][1] = v.y;
-            const uint32_t c = K[8 * D + (tok + 8 * i) * (D / 16) + t];
-            sc[i][0] = __byte_perm(c, 0, 0x0404) >> 1;
-          }
+          load_shared(w[i], slot + at_k + 8 * i * (D / 2));
+          const uint32_t c = load_scales<D / 64>(slot + at_ks + 8 * i * (D / 16));
+          sc[i][0] = __byte_perm(c, 0, 0x0404) >> 1;
+          if constexpr (D == 128) sc[i][1] = __byte_perm(c, 0, 0x1414) >> 1;
+        }
+        // V^T: lane g takes channels D / 8 * g on, of the tokens of rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+        uint32_t vw[4][VB / 4], vc[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          load_shared(vw[i], slot + at_v[i & 1] + 8 * (i >> 1) * (D / 2));
+          vc[i] = load_scales<1>(slot + at_vs[i & 1] + 8 * (i >> 1) * (D / 16));
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[u][n][i] = 0;
+          for (int i = 0; i < 4; ++i) s[n][i] = 0;
 #pragma unroll
         for (int j = 0; j < KW; ++j) {
           uint32_t x[2][4];
@@ -477,96 +544,64 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ parts,
           for (int k = 0; k < 2; ++k) {
             const uint32_t f[4] = {x[0][2 * k], x[1][2 * k], x[0][2 * k + 1], x[1][2 * k + 1]};
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma(s[u][n], f, qf[n][2 * j + k][0], qf[n][2 * j + k][1]);
+            for (int n = 0; n < NT; ++n) mma(s[n], f, qf[n][2 * j + k][0], qf[n][2 * j + k][1]);
           }
         }
-      }
-      // scores in powers of two; hidden ones to -inf
-      bool hide[kUps];
-      bool grow = false;
-#pragma unroll
-      for (int u = 0; u < kUps; ++u) {
-        const int64_t base = (cur.at + u) * 16;
-        hide[u] = !((ok >> u) & 1) || base + 16 > lowest;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[u][n][i] *= mul[n][i & 1];
-        if (hide[u]) {
+        if (!there || base + 16 > lowest) {  // hidden scores to -inf
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int64_t j = base + tok + 8 * (i >> 1);
-              if (!((ok >> u) & 1) || j >= end[n][i & 1]) s[u][n][i] = -INFINITY;
+            for (int i = 0; i < 4; ++i)
+              if (!there || base + tok + 8 * (i >> 1) >= end[n][i & 1]) s[n][i] = -INFINITY;
+          // what no row sees may be anything: its scale counts as zero
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (!there || base + tk[i & 1] + 8 * (i >> 1) >= highest) vc[i] = 0;
+        }
+        bool grow = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) grow |= fmaxf(s[n][i], s[n][i + 2]) > bar[n][i];
+        if (__any_sync(~0u, grow)) {  // rare after the first units
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float x = fmaxf(s[n][j], s[n][j + 2]);
+#pragma unroll
+              for (int i = 4; i < 32; i <<= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, i));
+              if (x > bar[n][j]) {  // others stay: a row does not depend on its neighbours
+                const float to = x * mul[n][j] - kLift, f = exp2_fast(m[n][j] - to);
+                m[n][j] = to;
+                bar[n][j] = __fdividef(to + kMove, mul[n][j]);
+                l[n][j] *= f;
+#pragma unroll
+                for (int k = 0; k < KS; ++k) o[n][k][j] *= f, o[n][k][j + 2] *= f;
+              }
             }
         }
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) grow |= s[u][n][i] > m[n][i & 1] + kMove;
-      }
-      if (__any_sync(~0u, grow)) {  // rare after the first chunks
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float x = kNone;
-#pragma unroll
-            for (int u = 0; u < kUps; ++u) x = fmaxf(x, fmaxf(s[u][n][j], s[u][n][j + 2]));
-#pragma unroll
-            for (int i = 4; i < 32; i <<= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, i));
-            const float to = x > m[n][j] + kMove ? x - kLift : m[n][j];  // others stay: a row does not depend on its neighbours
-            const float f = exp2_fast(m[n][j] - to);
-            m[n][j] = to;
-            l[n][j] *= f;
-#pragma unroll
-            for (int k = 0; k < KS; ++k) o[n][k][j] *= f, o[n][k][j + 2] *= f;
-          }
-      }
-#pragma unroll
-      for (int u = 0; u < kUps; ++u) {
         uint32_t p[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float x = exp2_fast(s[u][n][2 * i] - m[n][0]), y = exp2_fast(s[u][n][2 * i + 1] - m[n][1]);
+            const float x = exp2_fast(fmaf(s[n][2 * i], mul[n][0], -m[n][0]));
+            const float y = exp2_fast(fmaf(s[n][2 * i + 1], mul[n][1], -m[n][1]));
             l[n][0] += x, l[n][1] += y;
             p[n][i] = transpose8(pack_half2(x, y));
           }
-        // V^T: lane g takes channels D / 8 * g on, of the tokens of rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-        const uint8_t *V = sm.ring[warp][stage][u][1];
-        const int tk[2] = {t, (t ^ 1) + 4};
-        uint32_t w[4][VB / 4], sc[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t c[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int tt = tk[j] + 8 * i;
-            if constexpr (D == 128) {
-              const uint2 v = *reinterpret_cast<const uint2 *>(V + tt * (D / 2) + g * VB);
-              w[2 * i + j][0] = v.x, w[2 * i + j][1] = v.y;
-            } else {
-              w[2 * i + j][0] = *reinterpret_cast<const uint32_t *>(V + tt * (D / 2) + g * VB);
-            }
-            c[j] = V[8 * D + tt * (D / 16) + g * D / 128];
-            // what no row sees may be anything: its scale counts as zero
-            if (hide[u] && (!((ok >> u) & 1) || (cur.at + u) * 16 + tt >= highest)) c[j] = 0;
-          }
-          sc[i] = (c[0] << 7) | (c[1] << 23);
-        }
+        const uint32_t vs[2] = {(vc[0] << 7) | (vc[1] << 23), (vc[2] << 7) | (vc[3] << 23)};
 #pragma unroll
         for (int j = 0; j < VB / 4; ++j) {
           uint32_t x[2][2][4];  // token pair, channel parity, channel pair
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const uint32_t w0 = w[2 * i][j], w1 = w[2 * i + 1][j];
+            const uint32_t w0 = vw[2 * i][j], w1 = vw[2 * i + 1][j];
             e2m1x8_to_half2((w0 & 0x0F0F0F0Fu) | ((w1 << 4) & 0xF0F0F0F0u), x[i][0]);
             e2m1x8_to_half2(((w0 >> 4) & 0x0F0F0F0Fu) | (w1 & 0xF0F0F0F0u), x[i][1]);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[i][0][k] = hmul2(x[i][0][k], sc[i]), x[i][1][k] = hmul2(x[i][1][k], sc[i]);
+            for (int k = 0; k < 4; ++k) x[i][0][k] = hmul2(x[i][0][k], vs[i]), x[i][1][k] = hmul2(x[i][1][k], vs[i]);
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -575,109 +610,145 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ parts,
             for (int n = 0; n < NT; ++n) mma(o[n][4 * j + k], f, p[n][0], p[n][1]);
           }
         }
-      }
-      if (++stage == kStages) stage = 0, phase ^= 1;
-    }
+      };
 
-    // join the warps' parts: row r of the block, channel c
-    const bool starts = cur.u0 == 0, ends = cur.u1 == cur.it.units;
-    float *slot = parts + (int64_t)(2 * blockIdx.x + (starts ? 1 : 0)) * slot_floats<D>(R);
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int i = 4; i < 32; i <<= 1) l[n][j] += __shfl_xor_sync(~0u, l[n][j], i);
-#pragma unroll
-        for (int k = 0; k < KS; k += 2)
-          *reinterpret_cast<float4 *>(&sm.o[warp][2 * t + j][g * (D / 8) + 2 * k]) =
-              make_float4(o[n][k][j], o[n][k][j + 2], o[n][k + 1][j], o[n][k + 1][j + 2]);
-        if (g == 0) sm.m[warp][n * 8 + 2 * t + j] = m[n][j], sm.l[warp][n * 8 + 2 * t + j] = l[n][j];
+      for (; cur.has_chunk(); cur.next_chunk()) {
+        const uint32_t ok = valid >> (kUps * stage);
+        const int units = cur.chunk_units();
+        copies_wait<kStages - 2>();
+        __syncwarp();  // the chunk is there, and every lane is done with the one before, whose slot is the next to fill
+        issue(stage == 0 ? kStages - 1 : stage - 1);
+#pragma unroll 1
+        for (int u = 0; u < units; ++u)
+          unit(ring + stage * kSlot + u * 2 * kUnit, (cur.at + u) * 16, (ok >> u) & 1);
+        if (++stage == kStages) stage = 0;
       }
-      __syncthreads();
-      for (int i = threadIdx.x; i < 8 * (D / 4); i += kWarps * 32) {
-        const int r = i / (D / 4), c = i % (D / 4) * 4, rr = n * 8 + r;
-        float M = kNone, L = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm.m[w][rr]);
-        float4 acc = make_float4(0, 0, 0, 0);
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float f = exp2_fast(sm.m[w][rr] - M);
-          const float4 v = *reinterpret_cast<const float4 *>(&sm.o[w][r][c]);
-          L += sm.l[w][rr] * f;
-          acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
-        }
-        if (starts && ends) {
-          store_row<BF16>(a, cur.it.first, h, row0 + rr, nrows, c, acc, M, L);
-        } else {
-          *reinterpret_cast<float4 *>(slot + rr * D + c) = acc;
-          if (c == 0) slot[R * D + 2 * rr] = M, slot[R * D + 2 * rr + 1] = L;
-        }
+
+      const bool starts = cur.u0 == 0, ends = cur.u1 == cur.it.units;
+      if (starts && !ends) {  // the part's last segment: the ring is free once its last copies are in
+        copies_wait<0>();
+        __syncwarp();
       }
-      __syncthreads();
+      Part<D, NT> &part = starts ? *reinterpret_cast<Part<D, NT> *>(sm.ring[warp]) : sm.part[warp];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float sum = l[n][j];
+#pragma unroll
+          for (int i = 4; i < 32; i <<= 1) sum += __shfl_xor_sync(~0u, sum, i);
+          const int rr = n * 8 + 2 * t + j;
+          if (starts && ends) {
+            float v[D / 8];
+#pragma unroll
+            for (int k = 0; k < KS; ++k) v[2 * k] = o[n][k][j], v[2 * k + 1] = o[n][k][j + 2];
+            store_row<BF16>(a, cur.it.first, h, row0 + rr, nrows, g * (D / 8), v, m[n][j], sum);
+          } else {
+#pragma unroll
+            for (int k = 0; k < KS; k += 2)
+              *reinterpret_cast<float4 *>(&part.o[rr][g * (D / 8) + 2 * k]) =
+                  make_float4(o[n][k][j], o[n][k][j + 2], o[n][k + 1][j], o[n][k + 1][j + 2]);
+            if (g == 0) part.m[rr] = m[n][j], part.l[rr] = sum;
+          }
+        }
+      if (!(starts && ends) && lane == 0)
+        sm.meta[warp][starts] = {1, starts, ends, cur.b, cur.idx, begin + to - (cur.u1 - cur.u0) + cur.it.units - 1};
+      if (!cur.next_segment(a)) break;
     }
-    if (starts && !ends && threadIdx.x == 0) {
-      // the global index of the item's last unit gives the CTA that holds it
-      const int64_t x = st.end - (cur.u1 - cur.u0) + cur.it.units - 1;
-      meta[blockIdx.x].b = cur.b;
-      meta[blockIdx.x].idx = cur.idx;
-      meta[blockIdx.x].last = (int)(((x + 1) * st.ctas - 1) / st.total);
+  }
+
+  // Join the warps' parts of each (sequence, head, row block), in their order.
+  __syncthreads();
+  int first = -1;
+  for (int p = 0; p < 2 * kWarps; ++p) {
+    const PartMeta pm = sm.meta[p >> 1][p & 1];
+    if (pm.there && first < 0) first = p;
+    bool flush = pm.there && pm.ends;
+    if (p == 2 * kWarps - 1) flush = first >= 0;
+    if (!flush) continue;
+    const PartMeta head = sm.meta[first >> 1][first & 1];
+    int lastp = p;
+    while (!sm.meta[lastp >> 1][lastp & 1].there) --lastp;
+    const bool whole = head.starts && sm.meta[lastp >> 1][lastp & 1].ends;
+    const Item it = item_of<R>(a, head.b);
+    const int h = head.idx / it.blocks, row0 = (head.idx - h * it.blocks) * R, nrows = it.rows * a.group;
+    float *slot = parts + (int64_t)(2 * blockIdx.x + (head.starts ? 1 : 0)) * slot_floats<D>(R);
+    for (int i = threadIdx.x; i < R * (D / 4); i += kWarps * 32) {
+      const int r = i / (D / 4), c = i % (D / 4) * 4;
+      float M = kNone, L = 0, acc[4] = {};
+      for (int q = first; q <= p; ++q)
+        if (sm.meta[q >> 1][q & 1].there) {
+          const auto &x = (q & 1) ? *reinterpret_cast<const Part<D, NT> *>(sm.ring[q >> 1]) : sm.part[q >> 1];
+          M = fmaxf(M, x.m[r]);
+        }
+      for (int q = first; q <= p; ++q)
+        if (sm.meta[q >> 1][q & 1].there) {
+          const auto &x = (q & 1) ? *reinterpret_cast<const Part<D, NT> *>(sm.ring[q >> 1]) : sm.part[q >> 1];
+          const float f = exp2_fast(x.m[r] - M);
+          const float4 v = *reinterpret_cast<const float4 *>(&x.o[r][c]);
+          L += x.l[r] * f;
+          acc[0] += v.x * f, acc[1] += v.y * f, acc[2] += v.z * f, acc[3] += v.w * f;
+        }
+      if (whole) {
+        store_row<BF16>(a, it.first, h, row0 + r, nrows, c, acc, M, L);
+      } else {
+        *reinterpret_cast<float4 *>(slot + r * D + c) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        if (c == 0) slot[R * D + 2 * r] = M, slot[R * D + 2 * r + 1] = L;
+      }
     }
-    if (!cur.next_segment(a, warp)) break;
+    if (head.starts && !whole && threadIdx.x == 0)
+      meta[blockIdx.x] = {sm.cut.cta_of(head.last), head.b, head.idx};
+    first = -1;
   }
 }
 
 // Joins the pieces of the (sequence, head, row block) that starts in CTA
-// blockIdx.x of the kernel above, for row blockIdx.y of it.
+// blockIdx.x of the kernel above, for row blockIdx.y of it: a thread sums four
+// channels of every kJoin-th piece.
+constexpr int kJoin = 8;
 template <int D, int NT, bool BF16>
-__global__ void __launch_bounds__(D) fp4_join_kernel(const __grid_constant__ AttnArgs a, const float *__restrict__ parts,
-                                                     const SplitMeta *__restrict__ meta) {
-  constexpr int R = 8 * NT, kMost = 1024;
-  __shared__ float w[kMost];
-  __shared__ float red[2][D / 32];
+__global__ void __launch_bounds__(kJoin * D / 4) fp4_join_kernel(const __grid_constant__ AttnArgs a,
+                                                                 const float *__restrict__ parts,
+                                                                 const SplitMeta *__restrict__ meta) {
+  constexpr int R = 8 * NT, T = D / 4;
+  __shared__ float4 part[kJoin][T];
+  __shared__ float sum[kJoin];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int c = blockIdx.x, r = blockIdx.y, last = meta[c].last;
   if (last < 0) return;
-  const int n = last - c + 1;
-  auto slot = [&](int i) { return parts + (int64_t)(2 * (c + i) + (i == 0 ? 1 : 0)) * slot_floats<D>(R); };
-  float M = kNone;
-  for (int i = threadIdx.x; i < n; i += D) M = fmaxf(M, slot(i)[R * D + 2 * r]);
-#pragma unroll
-  for (int i = 1; i < 32; i <<= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, i));
-  if ((threadIdx.x & 31) == 0) red[0][threadIdx.x >> 5] = M;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) M = fmaxf(M, red[0][i]);
-  float L = 0;
-  for (int i = threadIdx.x; i < n; i += D) {
-    const float f = exp2_fast(slot(i)[R * D + 2 * r] - M);
-    w[i] = f;
-    L += slot(i)[R * D + 2 * r + 1] * f;
-  }
-#pragma unroll
-  for (int i = 1; i < 32; i <<= 1) L += __shfl_xor_sync(~0u, L, i);
-  if ((threadIdx.x & 31) == 0) red[1][threadIdx.x >> 5] = L;
-  __syncthreads();
-  L = 0;
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) L += red[1][i];
-  float acc = 0;
-#pragma unroll 8
-  for (int i = 0; i < n; ++i) acc += slot(i)[r * D + threadIdx.x] * w[i];
+  const int n = last - c + 1, x = threadIdx.x % T, y = threadIdx.x / T, lane = threadIdx.x & 31;
   const Item it = item_of<R>(a, meta[c].b);
   const int h = meta[c].idx / it.blocks, rb = meta[c].idx % it.blocks;
-  const int64_t row = (int64_t)rb * R + r;
-  if (row >= (int64_t)it.rows * a.group) return;
-  const int64_t tok = it.first + row / a.group;
-  const int qh = h * a.group + (int)(row % a.group);
-  uint8_t *dst = a.out + tok * a.o_token_stride + qh * a.o_head_stride + threadIdx.x * 2;
-  const float v = acc * (L == 0 ? 0.0f : 1.0f / L);
-  if (BF16)
-    *reinterpret_cast<__nv_bfloat16 *>(dst) = __float2bfloat16_rn(v);
-  else
-    *reinterpret_cast<__half *>(dst) = __float2half_rn(v);
-  if (a.lse && threadIdx.x == 0) a.lse[tok * (a.kv_heads * a.group) + qh] = natural_lse(M, L);
+  const int row = rb * R + r, nrows = it.rows * a.group;
+  if (row >= nrows) return;
+  auto slot = [&](int i) { return parts + (int64_t)(2 * (c + i) + (i == 0 ? 1 : 0)) * slot_floats<D>(R); };
+  // every warp finds the largest base for itself
+  float M = kNone;
+  for (int i = lane; i < n; i += 32) M = fmaxf(M, slot(i)[R * D + 2 * r]);
+#pragma unroll
+  for (int i = 1; i < 32; i <<= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, i));
+  float4 acc = make_float4(0, 0, 0, 0);
+  float L = 0;
+#pragma unroll 4
+  for (int i = y; i < n; i += kJoin) {
+    const float *p = slot(i);
+    const float f = exp2_fast(p[R * D + 2 * r] - M);
+    const float4 v = *reinterpret_cast<const float4 *>(p + r * D + 4 * x);
+    L += p[R * D + 2 * r + 1] * f;
+    acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+  }
+  part[y][x] = acc;
+  if (x == 0) sum[y] = L;
+  __syncthreads();
+  if (y) return;
+  L = 0;
+  float v[4] = {};
+#pragma unroll
+  for (int i = 0; i < kJoin; ++i) {
+    L += sum[i];
+    v[0] += part[i][x].x, v[1] += part[i][x].y, v[2] += part[i][x].z, v[3] += part[i][x].w;
+  }
+  store_row<BF16>(a, it.first, h, row, nrows, 4 * x, v, M, L);
 }
 
 template <int D, int NT>
@@ -696,10 +767,10 @@ int launch_decode(const AttnArgs &a, int ctas, void *workspace, cudaStream_t s) 
   FKV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   float *parts = (float *)workspace;
   SplitMeta *meta = (SplitMeta *)(parts + (int64_t)ctas * 2 * slot_floats<D>(8 * NT));
-  kernel<<<ctas, kWarps * 32, smem, s>>>(a, parts, meta);
+  kernel<<<ctas, DecodeShape<NT>::kWarps * 32, smem, s>>>(a, parts, meta);
   FKV_CUDA(cudaGetLastError());
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(ctas, 8 * NT), cfg.blockDim = dim3(D), cfg.stream = s;
+  cfg.gridDim = dim3(ctas, 8 * NT), cfg.blockDim = dim3(kJoin * D / 4), cfg.stream = s;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
@@ -745,6 +816,7 @@ int fkv_fp4_attention(const void *layer, int64_t num_blocks, int tokens_per_bloc
   const char *w = "fkv_fp4_attention: ";
   auto bad = [&](const char *m) { return fail(FKV_ERR_INVALID_ARG, std::string(w) + m); };
   if (tokens_per_block <= 0 || tokens_per_block % 16) return bad("tokens_per_block must be a positive multiple of 16");
+  if (tokens_per_block > 65536) return bad("tokens_per_block must be at most 65536");
   if (head_size != 64 && head_size != 128)
     return fail(FKV_ERR_UNSUPPORTED, std::string(w) + "head_size must be 64 or 128");
   if (dtype != FKV_DTYPE_BF16 && dtype != FKV_DTYPE_FP16)
@@ -754,6 +826,7 @@ int fkv_fp4_attention(const void *layer, int64_t num_blocks, int tokens_per_bloc
   if (num_blocks < 0 || num_q_tokens < 0 || num_seqs < 0 || max_blocks < 0) return bad("counts must be non-negative");
   if (!std::isfinite(softmax_scale)) return bad("softmax_scale must be finite");
   if (num_q_tokens == 0 || num_seqs == 0) return FKV_OK;
+  if (num_q_tokens * num_q_heads >= INT32_MAX) return bad("2^31 (token, head) rows or more in one call");
   if (!q || !out || !seq_lens || (max_blocks > 0 && !block_tables) || (num_blocks > 0 && !layer)) return bad("null pointer");
   if (!cu_seqlens_q && num_q_tokens % num_seqs) return bad("without cu_seqlens_q every sequence has the same number of new tokens");
   if ((uintptr_t)layer % 16 || kv_stride_in_bytes % 16 || block_stride_in_bytes % 16 || (uintptr_t)q % 16 ||
@@ -764,11 +837,14 @@ int fkv_fp4_attention(const void *layer, int64_t num_blocks, int tokens_per_bloc
   a.layer = (const uint8_t *)layer, a.num_blocks = num_blocks, a.kv_stride = kv_stride_in_bytes;
   a.block_stride = block_stride_in_bytes, a.tokens_per_block = tokens_per_block, a.kv_heads = num_kv_heads;
   a.group = num_q_heads / num_kv_heads;
+  a.upb = tokens_per_block / 16, a.upb_magic = ((uint64_t)1 << 40) / a.upb + 1;
   a.q = (const uint8_t *)q, a.q_token_stride = q_token_stride_in_bytes, a.q_head_stride = q_head_stride_in_bytes;
   a.out = (uint8_t *)out, a.o_token_stride = out_token_stride_in_bytes, a.o_head_stride = out_head_stride_in_bytes;
   a.lse = lse, a.num_q = num_q_tokens, a.tables = block_tables, a.table_stride = block_table_stride;
   a.max_blocks = max_blocks, a.seq_lens = seq_lens, a.cu = cu_seqlens_q, a.num_seqs = num_seqs;
   a.scale = softmax_scale, a.causal = causal;
+  a.rows_each = (int)(num_q_tokens / num_seqs);
+  a.table_tokens = (int)std::min<int64_t>((int64_t)max_blocks * tokens_per_block, INT32_MAX - 15);
   ThreadDeviceCtx *ctx;
   const int rc = get_ctx(-1, &ctx);
   if (rc != FKV_OK) return rc;
