@@ -9,7 +9,9 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
+#include <random>
 
 #include "fkv_common.h"
 #include "fp4_format.cuh"
@@ -103,7 +105,7 @@ __device__ __forceinline__ void store_row(const AttnArgs &a, int64_t first, int 
 // of asynchronous copies that runs ahead over the borders of sequences and
 // heads, and its own running sum, maximum and O.  What it holds whole it
 // writes out; the rest is joined once at the end within the CTA, and pieces of
-// one (sequence, head) in several CTAs by a second small kernel, both in a
+// one (sequence, head) in several CTAs by the CTA that comes last, both in a
 // fixed order.
 
 // Warps of a CTA, units of a chunk and chunks of a warp's ring, for NT row tiles.
@@ -147,7 +149,7 @@ __device__ __forceinline__ Item item_of(const AttnArgs &a, int b) {
   return it;
 }
 
-// The cut of all work into pieces, and where this CTA's starts; every CTA
+// The cut of all work into pieces, and where this CTA's starts; every warp
 // finds it for itself.
 struct Cut {
   int64_t each, more;  // a CTA has each + 1 units, from CTA `more` on each
@@ -155,56 +157,53 @@ struct Cut {
   int b;           // sequence of `begin`
   int64_t before;  // units before sequence b
   __device__ int cta_of(int64_t x) const {
-    return (int)(x < (each + 1) * more ? x / (each + 1) : more + (x - (each + 1) * more) / each);
+    const int64_t y = (each + 1) * more;
+    const int64_t n = x < y ? x : x - y, d = x < y ? each + 1 : each;
+    return (int)((x < y ? 0 : more) + ((n | d) >> 32 ? n / d : (uint32_t)n / (uint32_t)d));
   }
 };
 
 template <int R, int kWarps>
-__device__ void find_cut(const AttnArgs &a, Cut *out, int64_t *scratch /* kWarps */) {
-  const int per = (a.num_seqs + kWarps * 32 - 1) / (kWarps * 32), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int b0 = min((int)threadIdx.x * per, a.num_seqs), b1 = min(b0 + per, a.num_seqs);
-  int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) {
+__device__ __forceinline__ Cut find_cut(const AttnArgs &a) {
+  const int lane = threadIdx.x & 31;
+  auto work_of = [&](int b) {
     const Item it = item_of<R>(a, b);
-    mine += (int64_t)it.units * (it.blocks * a.kv_heads);
-  }
-  int64_t upto = mine;
-#pragma unroll
-  for (int i = 1; i < 32; i <<= 1) {
-    const int64_t o = __shfl_up_sync(~0u, upto, i);
-    if (lane >= i) upto += o;
-  }
-  if (lane == 31) scratch[warp] = upto;
-  __syncthreads();
+    return (int64_t)it.units * (it.blocks * a.kv_heads);
+  };
+  Cut cut;
   int64_t total = 0;
+  for (int b = lane; b < a.num_seqs; b += 32) total += work_of(b);
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) upto += scratch[w];
-    total += scratch[w];
-  }
+  for (int i = 1; i < 32; i <<= 1) total += __shfl_xor_sync(~0u, total, i);
   const int64_t want = (total + kWarps - 1) / kWarps;  // a unit for each warp, at least
   const uint32_t n = want < gridDim.x ? (uint32_t)want : gridDim.x;
-  int64_t each = 0, more = 0;
-  if (n) {
-    each = total >> 32 ? total / n : (uint32_t)total / n;
-    more = total - each * n;
+  if (blockIdx.x >= n) {
+    cut.begin = cut.end = total;
+    return cut;
   }
+  cut.each = total >> 32 ? total / n : (uint32_t)total / n;
+  cut.more = total - cut.each * n;
   const int64_t c = blockIdx.x;
-  const int64_t begin = c < n ? c * each + min(c, more) : total, end = c < n ? begin + each + (c < more) : total;
-  int64_t at = upto - mine;
-  if (threadIdx.x == 0) out->each = each, out->more = more, out->begin = begin, out->end = end;
-  if (begin >= at && begin < upto) {
-    for (int b = b0; b < b1; ++b) {
-      const Item it = item_of<R>(a, b);
-      const int64_t w = (int64_t)it.units * (it.blocks * a.kv_heads);
-      if (begin < at + w) {
-        out->b = b, out->before = at;
-        break;
-      }
-      at += w;
+  cut.begin = c * cut.each + min(c, cut.more), cut.end = cut.begin + cut.each + (c < cut.more);
+  // the sequence of `begin`, 32 at a time
+  int64_t before = 0;
+  for (int b0 = 0;; b0 += 32) {
+    const int64_t mine = b0 + lane < a.num_seqs ? work_of(b0 + lane) : 0;
+    int64_t upto = mine;
+#pragma unroll 1
+    for (int i = 1; i < 32; i <<= 1) {
+      const int64_t o = __shfl_up_sync(~0u, upto, i);
+      if (lane >= i) upto += o;
     }
+    const uint32_t past = __ballot_sync(~0u, before + upto > cut.begin);
+    if (past) {  // `begin` lies before the total, so this comes
+      const int l = __ffs(past) - 1;
+      cut.b = b0 + l;
+      cut.before = before + __shfl_sync(~0u, upto - mine, l);
+      return cut;
+    }
+    before += __shfl_sync(~0u, upto, 31);
   }
-  __syncthreads();
 }
 
 // A walk over a warp's part of the line of work: segments (the part of one
@@ -315,11 +314,6 @@ __device__ __forceinline__ float row_factor(float amax) {
   return __uint_as_float((uint32_t)(k + 127) << 23);
 }
 
-struct SplitMeta {  // of a CTA: the (sequence, head, row block) that starts in it and ends in another
-  int last;         // the CTA it ends in; -1: none
-  int b, idx;
-};
-
 // What a warp has of a (sequence, head, row block) that it does not hold whole.
 template <int D, int NT>
 struct Part {
@@ -327,9 +321,12 @@ struct Part {
   alignas(16) float o[8 * NT][kPad];
   float m[8 * NT], l[8 * NT];
 };
+// The rows a part belongs to, and its place in the line of work.
 struct PartMeta {
-  int there, starts, ends, b, idx;
-  int64_t last;  // the (sequence, head, row block)'s last unit in the line of work, where it starts here
+  int there, starts, ends;
+  int h, row0, nrows;      // key head; first (token, head) row, and how many the sequence has
+  int64_t first;           // the sequence's first row in q
+  int64_t begin, last;     // first and last unit of the whole (sequence, head, row block)
 };
 
 template <int D, int NT>
@@ -338,36 +335,76 @@ struct DecodeSmem {
   alignas(128) uint8_t ring[kWarps][kStages][kUps][2][9 * D];  // at the end: the part that starts in the warp
   Part<D, NT> part[kWarps];                                     // the part that goes on from the warp before
   PartMeta meta[kWarps][2];
-  Cut cut;
-  int64_t scratch[kWarps];
+  PartMeta open[2];  // parts of the CTA that others share: 0 goes on from another CTA, 1 starts here
+  int is_last;
   static_assert(sizeof(Part<D, NT>) <= sizeof(ring[0]), "a part has to fit a warp's ring");
 };
 
 template <int D>
 __host__ __device__ constexpr int slot_floats(int rows) { return rows * (D + 2); }
 
+// Joins `count` consecutive warps' parts from that of warp w0 on, whose part
+// is the one in its ring when `ring`: into rows of the output, or into a slot
+// of the workspace.
+template <int D, int NT, bool BF16>
+__device__ __forceinline__ void join_parts(const AttnArgs &a, const DecodeSmem<D, NT> &sm, int w0, bool ring, int count,
+                                           const PartMeta &pm, float *slot) {
+  constexpr int R = 8 * NT, kWarps = DecodeShape<NT>::kWarps;
+  auto part = [&](int k) -> const Part<D, NT> & {
+    return k == 0 && ring ? *reinterpret_cast<const Part<D, NT> *>(sm.ring[w0]) : sm.part[w0 + k];
+  };
+  for (int i = threadIdx.x; i < R * (D / 4); i += kWarps * 32) {
+    const int r = i / (D / 4), c = i % (D / 4) * 4;
+    float M = kNone, L = 0, acc[4] = {};
+#pragma unroll 4
+    for (int k = 0; k < count; ++k) M = fmaxf(M, part(k).m[r]);
+#pragma unroll 2
+    for (int k = 0; k < count; ++k) {
+      const float f = exp2_fast(part(k).m[r] - M);
+      const float4 v = *reinterpret_cast<const float4 *>(&part(k).o[r][c]);
+      L += part(k).l[r] * f;
+      acc[0] += v.x * f, acc[1] += v.y * f, acc[2] += v.z * f, acc[3] += v.w * f;
+    }
+    if (slot) {
+      *reinterpret_cast<float4 *>(slot + r * D + c) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      if (c == 0) slot[R * D + 2 * r] = M, slot[R * D + 2 * r + 1] = L;
+    } else {
+      store_row<BF16>(a, pm.first, pm.h, pm.row0 + r, pm.nrows, c, acc, M, L);
+    }
+  }
+}
+
+// Counts an arrival at a word of the workspace and says how many there were.
+// What the word held before does not matter: a call (or a captured launch,
+// which leaves its words at 0) knows its own counts by its number.
+__device__ __forceinline__ int arrive(unsigned long long *word, unsigned long long call) {
+  const unsigned long long old = *(volatile unsigned long long *)word;
+  if ((old >> 16) != call) atomicCAS(word, old, call << 16);  // where it fails another arrival has done it
+  return (int)((atomicAdd(word, 1ull) + 1) & 0xFFFF);
+}
+
 template <int D, int NT, bool BF16>
 __global__ void __launch_bounds__(DecodeShape<NT>::kWarps * 32, 1)
-fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ parts, SplitMeta *__restrict__ meta) {
+fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots, unsigned long long *__restrict__ arrived,
+                  unsigned long long call) {
   constexpr int R = 8 * NT, KS = D / 16, KW = D / 32, VB = D / 16;  // k-steps; words of a lane's K row; bytes of its V row
   constexpr int kWarps = DecodeShape<NT>::kWarps, kUps = DecodeShape<NT>::kUps, kStages = DecodeShape<NT>::kStages;
   constexpr int kUnit = 9 * D, kSlot = kUps * 2 * kUnit, kBatch = 32 / kUps;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   auto &sm = *reinterpret_cast<DecodeSmem<D, NT> *>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  // the next kernel only starts its CTAs early; it waits for this one's end before it reads
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (threadIdx.x == 0) meta[blockIdx.x].last = -1;
   if (lane < 2) sm.meta[warp][lane].there = 0;
-  find_cut<R, kWarps>(a, &sm.cut, sm.scratch);
-  const int64_t begin = sm.cut.begin;
-  const int units_here = (int)(sm.cut.end - begin);
+  const Cut cut = find_cut<R, kWarps>(a);
+  const int64_t begin = cut.begin;
+  const int units_here = (int)(cut.end - begin);
   if (units_here <= 0) return;
-  const int from = (int)((int64_t)units_here * warp / kWarps), to = (int)((int64_t)units_here * (warp + 1) / kWarps);
+  // the first warps have a unit more, or all there are
+  const int share = units_here / kWarps, rest = units_here - share * kWarps;
+  const int from = warp * share + min(warp, rest), to = from + share + (warp < rest);
 
   if (from < to) {
     Walk<R, kUps> in, cur;  // the copies' walk runs ahead
-    in.start(a, sm.cut.b, begin + from - sm.cut.before, to - from);
+    in.start(a, cut.b, begin + from - cut.before, to - from);
     cur = in;
     const uint32_t ring = smem_addr(sm.ring[warp]);
     bool more = true;
@@ -651,109 +688,103 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ parts,
             if (g == 0) part.m[rr] = m[n][j], part.l[rr] = sum;
           }
         }
-      if (!(starts && ends) && lane == 0)
-        sm.meta[warp][starts] = {1, starts, ends, cur.b, cur.idx, begin + to - (cur.u1 - cur.u0) + cur.it.units - 1};
+      if (!(starts && ends) && lane == 0) {
+        const int64_t unit0 = begin + to - cur.left - cur.u0;
+        sm.meta[warp][starts] = {1, starts, ends, h, row0, nrows, cur.it.first, unit0, unit0 + cur.it.units - 1};
+      }
       if (!cur.next_segment(a)) break;
     }
   }
 
   // Join the warps' parts of each (sequence, head, row block), in their order.
+  if (threadIdx.x < 2) sm.open[threadIdx.x].there = 0;
   __syncthreads();
-  int first = -1;
-  for (int p = 0; p < 2 * kWarps; ++p) {
-    const PartMeta pm = sm.meta[p >> 1][p & 1];
-    if (pm.there && first < 0) first = p;
-    bool flush = pm.there && pm.ends;
-    if (p == 2 * kWarps - 1) flush = first >= 0;
-    if (!flush) continue;
-    const PartMeta head = sm.meta[first >> 1][first & 1];
-    int lastp = p;
-    while (!sm.meta[lastp >> 1][lastp & 1].there) --lastp;
-    const bool whole = head.starts && sm.meta[lastp >> 1][lastp & 1].ends;
-    const Item it = item_of<R>(a, head.b);
-    const int h = head.idx / it.blocks, row0 = (head.idx - h * it.blocks) * R, nrows = it.rows * a.group;
-    float *slot = parts + (int64_t)(2 * blockIdx.x + (head.starts ? 1 : 0)) * slot_floats<D>(R);
-    for (int i = threadIdx.x; i < R * (D / 4); i += kWarps * 32) {
-      const int r = i / (D / 4), c = i % (D / 4) * 4;
-      float M = kNone, L = 0, acc[4] = {};
-      for (int q = first; q <= p; ++q)
-        if (sm.meta[q >> 1][q & 1].there) {
-          const auto &x = (q & 1) ? *reinterpret_cast<const Part<D, NT> *>(sm.ring[q >> 1]) : sm.part[q >> 1];
-          M = fmaxf(M, x.m[r]);
-        }
-      for (int q = first; q <= p; ++q)
-        if (sm.meta[q >> 1][q & 1].there) {
-          const auto &x = (q & 1) ? *reinterpret_cast<const Part<D, NT> *>(sm.ring[q >> 1]) : sm.part[q >> 1];
-          const float f = exp2_fast(x.m[r] - M);
-          const float4 v = *reinterpret_cast<const float4 *>(&x.o[r][c]);
-          L += x.l[r] * f;
-          acc[0] += v.x * f, acc[1] += v.y * f, acc[2] += v.z * f, acc[3] += v.w * f;
-        }
-      if (whole) {
-        store_row<BF16>(a, it.first, h, row0 + r, nrows, c, acc, M, L);
-      } else {
-        *reinterpret_cast<float4 *>(slot + r * D + c) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-        if (c == 0) slot[R * D + 2 * r] = M, slot[R * D + 2 * r + 1] = L;
-      }
+  const bool there = lane < 2 * kWarps && sm.meta[lane >> 1][lane & 1].there;
+  uint32_t parts = __ballot_sync(~0u, there);
+  const uint32_t ends = __ballot_sync(~0u, there && sm.meta[lane >> 1][lane & 1].ends);
+  while (parts) {
+    const int p0 = __ffs(parts) - 1;
+    const uint32_t e = ends & ~((1u << p0) - 1);
+    const int p1 = e ? __ffs(e) - 1 : 31 - __clz(parts);  // the part that ends it, or the last
+    parts &= ~((2u << p1) - 1);
+    const PartMeta pm = sm.meta[p0 >> 1][p0 & 1];
+    const bool whole = pm.starts && e;
+    join_parts<D, NT, BF16>(a, sm, p0 >> 1, p0 & 1, (p1 >> 1) - (p0 >> 1) + 1, pm,
+                            whole ? nullptr : slots + (int64_t)(2 * blockIdx.x + pm.starts) * slot_floats<D>(R));
+    if (!whole && threadIdx.x == 0) sm.open[pm.starts] = pm;
+  }
+
+  // The CTA that comes last joins what several CTAs have of one, in their order.
+  __threadfence();
+  __syncthreads();
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) {
+    const PartMeta pm = sm.open[i];
+    if (!pm.there) continue;
+    const int c0 = cut.cta_of(pm.begin), n = cut.cta_of(pm.last) - c0 + 1;
+    if (threadIdx.x == 0) {
+      const bool last = arrive(arrived + c0, call) == n;
+      if (last) arrived[c0] = 0;  // for a replay of this launch
+      __threadfence();
+      sm.is_last = last;
     }
-    if (head.starts && !whole && threadIdx.x == 0)
-      meta[blockIdx.x] = {sm.cut.cta_of(head.last), head.b, head.idx};
-    first = -1;
+    __syncthreads();
+    if (sm.is_last) {
+      // a warp gathers every kWarps-th CTA's slot, 8 rows at a time, into its part
+      const int groups = min(n, kWarps);
+      if (warp < groups) {
+        Part<D, NT> &mine = sm.part[warp];
+        for (int n8 = 0; n8 < NT; ++n8) {
+          constexpr int kLanes = D / 4, kRows = 32 / kLanes;  // D 64: two rows at a time
+          const int c = lane % kLanes * 4;
+          float acc[8 / kRows][4], M[8 / kRows], L[8 / kRows];
+#pragma unroll
+          for (int r = 0; r < 8 / kRows; ++r) M[r] = kNone, L[r] = 0, acc[r][0] = acc[r][1] = acc[r][2] = acc[r][3] = 0;
+#pragma unroll 2
+          for (int k = warp; k < n; k += kWarps) {
+            const float *slot = slots + (int64_t)(2 * (c0 + k) + (k == 0)) * slot_floats<D>(R);
+#pragma unroll
+            for (int r = 0; r < 8 / kRows; ++r) {
+              const int rr = n8 * 8 + r * kRows + lane / kLanes;
+              const float2 ml = __ldcg(reinterpret_cast<const float2 *>(slot + R * D + 2 * rr));
+              const float4 v = __ldcg(reinterpret_cast<const float4 *>(slot + rr * D + c));
+              const float to = fmaxf(M[r], ml.x), f = exp2_fast(M[r] - to), y = exp2_fast(ml.x - to);
+              M[r] = to;
+              L[r] = L[r] * f + ml.y * y;
+              acc[r][0] = acc[r][0] * f + v.x * y, acc[r][1] = acc[r][1] * f + v.y * y;
+              acc[r][2] = acc[r][2] * f + v.z * y, acc[r][3] = acc[r][3] * f + v.w * y;
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 8 / kRows; ++r) {
+            const int rr = n8 * 8 + r * kRows + lane / kLanes;
+            *reinterpret_cast<float4 *>(&mine.o[rr][c]) = make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
+            if (c == 0) mine.m[rr] = M[r], mine.l[rr] = L[r];
+          }
+        }
+      }
+      __syncthreads();
+      join_parts<D, NT, BF16>(a, sm, 0, false, groups, pm, nullptr);
+    }
+    __syncthreads();
   }
 }
 
-// Joins the pieces of the (sequence, head, row block) that starts in CTA
-// blockIdx.x of the kernel above, for row blockIdx.y of it: a thread sums four
-// channels of every kJoin-th piece.
-constexpr int kJoin = 8;
-template <int D, int NT, bool BF16>
-__global__ void __launch_bounds__(kJoin * D / 4) fp4_join_kernel(const __grid_constant__ AttnArgs a,
-                                                                 const float *__restrict__ parts,
-                                                                 const SplitMeta *__restrict__ meta) {
-  constexpr int R = 8 * NT, T = D / 4;
-  __shared__ float4 part[kJoin][T];
-  __shared__ float sum[kJoin];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int c = blockIdx.x, r = blockIdx.y, last = meta[c].last;
-  if (last < 0) return;
-  const int n = last - c + 1, x = threadIdx.x % T, y = threadIdx.x / T, lane = threadIdx.x & 31;
-  const Item it = item_of<R>(a, meta[c].b);
-  const int h = meta[c].idx / it.blocks, rb = meta[c].idx % it.blocks;
-  const int row = rb * R + r, nrows = it.rows * a.group;
-  if (row >= nrows) return;
-  auto slot = [&](int i) { return parts + (int64_t)(2 * (c + i) + (i == 0 ? 1 : 0)) * slot_floats<D>(R); };
-  // every warp finds the largest base for itself
-  float M = kNone;
-  for (int i = lane; i < n; i += 32) M = fmaxf(M, slot(i)[R * D + 2 * r]);
-#pragma unroll
-  for (int i = 1; i < 32; i <<= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, i));
-  float4 acc = make_float4(0, 0, 0, 0);
-  float L = 0;
-#pragma unroll 4
-  for (int i = y; i < n; i += kJoin) {
-    const float *p = slot(i);
-    const float f = exp2_fast(p[R * D + 2 * r] - M);
-    const float4 v = *reinterpret_cast<const float4 *>(p + r * D + 4 * x);
-    L += p[R * D + 2 * r + 1] * f;
-    acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+// A number of 48 bits for each launch, from a start that differs between processes.
+unsigned long long next_call() {
+  static std::atomic<unsigned long long> last{[] {
+    std::random_device r;
+    return ((unsigned long long)r() << 32) ^ r();
+  }()};
+  for (;;) {
+    const unsigned long long n = (last.fetch_add(1, std::memory_order_relaxed) + 1) & 0xFFFFFFFFFFFFull;
+    if (n) return n;  // 0 is what a finished launch leaves
   }
-  part[y][x] = acc;
-  if (x == 0) sum[y] = L;
-  __syncthreads();
-  if (y) return;
-  L = 0;
-  float v[4] = {};
-#pragma unroll
-  for (int i = 0; i < kJoin; ++i) {
-    L += sum[i];
-    v[0] += part[i][x].x, v[1] += part[i][x].y, v[2] += part[i][x].z, v[3] += part[i][x].w;
-  }
-  store_row<BF16>(a, it.first, h, row, nrows, 4 * x, v, M, L);
 }
 
 template <int D, int NT>
 int64_t decode_workspace(int ctas) {
-  return (int64_t)ctas * 2 * slot_floats<D>(8 * NT) * 4 + (int64_t)ctas * sizeof(SplitMeta);
+  return (int64_t)ctas * 2 * slot_floats<D>(8 * NT) * 4 + (int64_t)ctas * 8;
 }
 int64_t decode_workspace(int D, int nt, int ctas) {
   return D == 128 ? (nt == 1 ? decode_workspace<128, 1>(ctas) : nt == 2 ? decode_workspace<128, 2>(ctas) : decode_workspace<128, 4>(ctas))
@@ -765,18 +796,11 @@ int launch_decode(const AttnArgs &a, int ctas, void *workspace, cudaStream_t s) 
   const int smem = sizeof(DecodeSmem<D, NT>);
   auto kernel = fp4_decode_kernel<D, NT, BF16>;
   FKV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  float *parts = (float *)workspace;
-  SplitMeta *meta = (SplitMeta *)(parts + (int64_t)ctas * 2 * slot_floats<D>(8 * NT));
-  kernel<<<ctas, DecodeShape<NT>::kWarps * 32, smem, s>>>(a, parts, meta);
+  float *slots = (float *)workspace;
+  auto *arrived = (unsigned long long *)(slots + (int64_t)ctas * 2 * slot_floats<D>(8 * NT));
+  kernel<<<ctas, DecodeShape<NT>::kWarps * 32, smem, s>>>(a, slots, arrived, next_call());
   FKV_CUDA(cudaGetLastError());
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(ctas, 8 * NT), cfg.blockDim = dim3(kJoin * D / 4), cfg.stream = s;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at, cfg.numAttrs = 1;
-  FKV_CUDA(cudaLaunchKernelEx(&cfg, fp4_join_kernel<D, NT, BF16>, a, (const float *)parts, (const SplitMeta *)meta));
-  note_launch(2);
+  note_launch();
   return FKV_OK;
 }
 template <int D, bool BF16>
