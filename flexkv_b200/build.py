@@ -20,6 +20,8 @@ REPO_DIR = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_DIR = os.path.join(PKG_DIR, "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libflexkv_b200.so")
+BINDING = os.path.join(CSRC, "fp4_binding.cpp")  # the 4-bit cache's operators on torch tensors
+BINDING_PATH = os.path.join(LIB_DIR, "_fp4.so")
 SOURCES = ["fkv_common.cpp", "transfer.cu", "tp_group.cpp", "xxh64.cu", "engine.cpp", "ipc.cpp", "ssd.cpp",
            "block_index.cu", "fp4_cache.cu", "fp4_attention.cu"]
 HEADERS = [os.path.join(CSRC, "fkv_common.h"), os.path.join(CSRC, "fp4_format.cuh"),
@@ -42,7 +44,49 @@ def _stale() -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _build_binding(verbose: bool) -> None:
+    """The CPython module of the 4-bit cache's operators, against this
+    interpreter and the installed torch."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    inc = [sysconfig.get_paths()["include"], *include_paths()]
+    tmp = BINDING_PATH + ".tmp"
+    # The C++ library has to be the shared one that torch uses: a second copy, linked statically as some
+    # compilers' defaults have it, ends the process at the first stream or exception that meets the other.
+    cmd = [
+        _nvcc(), "-O2", "-std=c++17", "-Xcompiler", "-fPIC,-Wall", "-shared",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        *[a for d in inc for a in ("-isystem", d)], "-o", tmp, BINDING, f"-L{torch_lib}", "-ltorch_python", "-ltorch",
+        "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Xlinker", f"-rpath={torch_lib}", "-Xlinker", "-l:libstdc++.so.6",
+        "-cudart", "none",
+    ]
+    if verbose:
+        print(" ".join(cmd))
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed ({res.returncode}):\n{res.stderr[-4000:]}")
+    os.replace(tmp, BINDING_PATH)
+
+
+def _binding_stale() -> bool:
+    if not os.path.exists(BINDING_PATH):
+        return True
+    deps = [BINDING, os.path.join(REPO_DIR, "include", "flexkv_b200.h"), os.path.abspath(__file__)]
+    return any(os.path.getmtime(d) > os.path.getmtime(BINDING_PATH) for d in deps)
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
+    lib = _build_lib(force, verbose)
+    if force or _binding_stale():
+        _build_binding(verbose)
+    return lib
+
+
+def _build_lib(force: bool, verbose: bool) -> str:
     if not force and not _stale():
         return LIB_PATH
     os.makedirs(LIB_DIR, exist_ok=True)

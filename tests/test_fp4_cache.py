@@ -148,3 +148,12 @@ def test_python_refuses_host_tensors():
         fp4_cache.fp4_pack_blocks([], [], slots, slots)
     with pytest.raises(RuntimeError, match="uint8"):
         fp4_cache.fp4_read(layer.float(), slots)
+    with pytest.raises(RuntimeError, match=r"got \[2, 4, 2, 1, 540\]"):
+        fp4_cache.fp4_read(layer[..., :540], slots)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        fp4_cache.fp4_read(layer[:, :, :, :, ::1].transpose(1, 2), slots)
+    for args in ((layer,), (layer, x, x, slots, slots)):
+        with pytest.raises(TypeError):
+            fp4_cache._native().write(*args)
+    with pytest.raises(RuntimeError, match="torch.Tensor"):
+        fp4_cache.fp4_write([layer], x, x, slots)
