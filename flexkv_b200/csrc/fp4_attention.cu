@@ -770,6 +770,473 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
   }
 }
 
+// ---- many rows: prompts behind a cached prefix ------------------------------
+//
+// With hundreds of rows for each key the products bound the kernel, so they go
+// to tcgen05.  A CTA takes kTiles * 128 (token, head) rows of one sequence and
+// key head through the keys, kKeys = 128 at a time, as separate warps:
+//  * four warps bring K and V in: 4-bit bytes from global memory into
+//    registers (a chunk ahead), to half, into shared memory in the 128-byte
+//    swizzled layout.  K as it lies is K-major for S = Q K^T, V is MN-major
+//    for O = P V: no transpose;
+//  * one thread issues the products: S of a tile of 128 rows into tensor
+//    memory, and O += P V with P read from tensor memory;
+//  * four warps for each tile of rows take S, a thread a row: weights
+//    2^(score - base) in half go back over S as P, their sum stays in the
+//    thread.  The base moves only when a score passes it by kMove, as in the
+//    kernel above: then the weights are taken again and O is scaled in place.
+// Two tiles of rows alternate: while one is in softmax the tensor core works
+// on the other, and K and V are converted once for both.
+// Tensor memory (512 columns): O of both tiles, S of both; P lies over S.
+
+constexpr int kTiles = 2, kKeys = 128;
+constexpr int kFillWarps = 4;
+constexpr int kManyThreads = (4 * kTiles + kFillWarps + 1) * 32;
+
+template <int D>
+struct ManySmem {
+  static constexpr int kBlock = 128 * 128;  // 128 rows of 64 halves, swizzled
+  alignas(1024) uint8_t q[kTiles][D / 64][kBlock];
+  alignas(1024) uint8_t k[2][D / 64][kBlock];
+  alignas(1024) uint8_t v[2][D / 64][kBlock];
+  uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[kTiles], p_full[kTiles], o_done[kTiles];
+  alignas(4) uint8_t bad[4][kFillWarps];  // of a chunk of keys, a warp's two units: whose page is outside the pool
+  uint32_t tmem;
+};
+
+__device__ __forceinline__ void mbar_init(uint64_t *m, int count) {
+  asm volatile("mbarrier.init.shared.b64 [%0], %1;" ::"r"(smem_addr(m)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t *m) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(smem_addr(m)) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint64_t *m, int parity) {
+  int ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2, %3;\n selp.b32 %0, 1, 0, p;\n}"
+      : "=r"(ok)
+      : "r"(smem_addr(m)), "r"(parity), "r"(1000000)
+      : "memory");
+  return ok;
+}
+// A wait has a limit (a try lasts up to a millisecond by itself).  One that
+// runs out is counted and the kernel goes on as if it had come, each later wait
+// with a single try: it ends, and its output is not to be used.
+__device__ unsigned long long g_wait_timeouts;
+struct Patience {
+  int tries = 2000;
+  __device__ __forceinline__ void wait(uint64_t *m, int parity) {
+    for (int i = 0; i < tries; ++i)
+      if (mbar_try(m, parity)) return;
+    if (tries > 1) atomicAdd(&g_wait_timeouts, 1ull);
+    tries = 1;
+  }
+};
+
+// A shared memory operand in the 128-byte swizzled layout.  K-major: 8 rows of
+// 128 bytes every 1024 bytes.  MN-major: 8 rows along K every 1024 bytes, the
+// next 64 columns a block of 128 rows further.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, bool mn_major) {
+  return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)(mn_major ? (128 * 128) >> 4 : 1) << 16 | (uint64_t)(1024 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// 128 rows, N columns, half operands, float sums.
+__host__ __device__ constexpr uint32_t mma_desc(int n, bool b_mn_major) {
+  return 1u << 4 | (b_mn_major ? 1u << 16 : 0) | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(desc), "r"((int)add)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, bool add) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(desc), "r"((int)add)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t *m) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(m)) : "memory");
+}
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+#define FKV_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+#define FKV_W8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+// 16 or 32 columns of the warp's 32 lanes.
+__device__ __forceinline__ void tmem_load16(uint32_t (&r)[16], uint32_t at) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : FKV_R8(r, 0), FKV_R8(r, 8)
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
+               FKV_W8(r, 0), FKV_W8(r, 8)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_load32(uint32_t (&r)[32], uint32_t at) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : FKV_R8(r, 0), FKV_R8(r, 8), FKV_R8(r, 16), FKV_R8(r, 24)
+      : "r"(at)
+      : "memory");
+}
+// What was loaded may be used from here on: the registers go through the wait.
+#define FKV_RW8(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7])
+__device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : FKV_RW8(r, 0), FKV_RW8(r, 8) : : "memory");
+}
+__device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : FKV_RW8(r, 0), FKV_RW8(r, 8), FKV_RW8(r, 16), FKV_RW8(r, 24)
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_constant__ AttnArgs a) {
+  constexpr int R = kTiles * 128;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  auto &sm = *reinterpret_cast<ManySmem<D> *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = blockIdx.y;
+
+  // the sequence and its block of rows: the last CTAs of a sequence have most keys, so they come first
+  int b = -1, rb = 0;
+  Item it;
+  {
+    int want = gridDim.x - 1 - blockIdx.x, before = 0;
+    for (int b0 = 0; b0 < a.num_seqs; b0 += 32) {
+      const int mine = b0 + lane < a.num_seqs ? item_of<R>(a, b0 + lane).blocks : 0;
+      int upto = mine;
+#pragma unroll 1
+      for (int i = 1; i < 32; i <<= 1) {
+        const int o = __shfl_up_sync(~0u, upto, i);
+        if (lane >= i) upto += o;
+      }
+      const uint32_t past = __ballot_sync(~0u, before + upto > want);
+      if (past) {
+        const int l = __ffs(past) - 1;
+        b = b0 + l;
+        rb = want - before - __shfl_sync(~0u, upto - mine, l);
+        break;
+      }
+      before += __shfl_sync(~0u, upto, 31);
+    }
+    if (b < 0) return;  // the grid is an upper bound
+    it = item_of<R>(a, b);
+  }
+  const int row0 = rb * R, nrows = it.rows * a.group;
+  const int tiles = nrows - row0 > 128 ? 2 : 1;
+  auto end_of = [&](int row) {  // the keys that a row sees
+    int e = it.len;
+    if (a.causal) e = max(min(e, it.len_q - it.rows + row / a.group + 1), 0);
+    return e;
+  };
+  const int most = end_of(min(nrows - 1, row0 + R - 1));
+  const int chunks = (most + kKeys - 1) / kKeys;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&sm.q_full, 128 * tiles);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.k_full[i], kFillWarps * 32), mbar_init(&sm.v_full[i], kFillWarps * 32);
+      mbar_init(&sm.k_empty[i], 1), mbar_init(&sm.v_empty[i], 1);
+    }
+    for (int t = 0; t < kTiles; ++t) mbar_init(&sm.s_full[t], 1), mbar_init(&sm.p_full[t], 128), mbar_init(&sm.o_done[t], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 4 * kTiles + kFillWarps) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sm.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = sm.tmem;
+  auto o_at = [&](int t) { return tmem + t * 128; };
+  auto s_at = [&](int t) { return tmem + (kTiles + t) * 128; };
+  Patience patience;
+
+  if (warp < 4 * kTiles) {
+    // ---- a thread for each row ----
+    const int t = warp >> 2, r = (warp & 3) * 32 + lane, row = row0 + t * 128 + r;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // the warp's 32 lanes of tensor memory
+    if (t < tiles) {
+      const bool valid = row < nrows;
+      const int i0 = valid ? row / a.group : 0;
+      float mul = 0;
+      {
+        const uint8_t *p = a.q + (it.first + i0) * a.q_token_stride + (h * a.group + row - i0 * a.group) * a.q_head_stride;
+        float amax = 0;
+        uint4 x[D / 8];
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) x[i] = valid ? reinterpret_cast<const uint4 *>(p)[i] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = pair_to_float2<BF16>(w[j]);
+            amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+        }
+        const float f = row_factor(amax), fs = a.scale < 0.0f ? -f : f;
+        mul = fmaxf(fabsf(a.scale) * 1.4426950408889634f * (1.0f / f), 1e-37f);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+          uint32_t y[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 z = pair_to_float2<BF16>(w[j]);
+            y[j] = pack_half2(z.x * fs, z.y * fs);
+          }
+          *reinterpret_cast<uint4 *>(&sm.q[t][i / 8][r * 128 + ((i % 8) ^ (r & 7)) * 16]) = make_uint4(y[0], y[1], y[2], y[3]);
+        }
+      }
+      fence_async();
+      mbar_arrive(&sm.q_full);
+
+      const int end = valid ? end_of(row) : 0;
+      const int lowest = __reduce_min_sync(~0u, valid ? end : INT32_MAX);
+      float base = kNone, bar = -INFINITY, l[2] = {0, 0};
+      for (int j = 0; j < chunks; ++j) {
+        patience.wait(&sm.s_full[t], j & 1);
+        fence_after();
+        const uint32_t S = s_at(t) + lanes;
+        const uint32_t bad = *(volatile uint32_t *)sm.bad[j & 3];
+        const bool hide = (j + 1) * kKeys > lowest || bad;
+        auto hidden = [&](uint32_t(&x)[32], int c) {  // scores of columns 32 c on that the row does not see
+          const uint32_t gone = bad >> (8 * c);
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (((gone >> (i / 16)) & 1) || j * kKeys + 32 * c + i >= end) x[i] = 0xFF800000u;
+        };
+        uint32_t x[2][32];
+        // the largest score first: P is going to lie over S
+        float top[2] = {-INFINITY, -INFINITY};
+        tmem_load32(x[0], S);
+#pragma unroll
+        for (int c = 0; c < kKeys / 32; ++c) {
+          tmem_wait_load(x[c & 1]);
+          tmem_load32(x[(c + 1) & 1], S + 32 * ((c + 1) % (kKeys / 32)));  // the last: the next pass's first
+          if (hide) hidden(x[c & 1], c);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) top[i & 1] = fmaxf(top[i & 1], __uint_as_float(x[c & 1][i]));
+        }
+        const float most_here = fmaxf(top[0], top[1]);
+        if (__any_sync(~0u, most_here > bar)) {  // rare after the first chunks
+          float f = 1.0f;
+          if (most_here > bar) {  // other rows stay: a row does not depend on its neighbours
+            const float to = most_here * mul - kLift;
+            f = exp2_fast(base - to);
+            base = to;
+            bar = __fdividef(to + kMove, mul);
+          }
+          l[0] *= f, l[1] *= f;
+          if (j > 0) {  // the product before is done: this chunk's S came after it
+            patience.wait(&sm.o_done[t], (j - 1) & 1);
+            fence_after();
+            tmem_wait_load(x[0]);
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t y[16];
+              tmem_load16(y, o_at(t) + lanes + 16 * c);
+              tmem_wait_load(y);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
+              tmem_store16(o_at(t) + lanes + 16 * c, y);
+            }
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < kKeys / 32; ++c) {
+          tmem_wait_load(x[c & 1]);
+          if (c + 1 < kKeys / 32) tmem_load32(x[(c + 1) & 1], S + 32 * (c + 1));
+          if (hide) hidden(x[c & 1], c);
+          uint32_t p[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float u = exp2_fast(fmaf(__uint_as_float(x[c & 1][2 * i]), mul, -base));
+            const float v = exp2_fast(fmaf(__uint_as_float(x[c & 1][2 * i + 1]), mul, -base));
+            l[0] += u, l[1] += v;
+            p[i] = pack_half2(u, v);
+          }
+          tmem_store16(S + 16 * c, p);  // over columns that have been read
+        }
+        tmem_wait_store();
+        fence_before();
+        mbar_arrive(&sm.p_full[t]);
+      }
+
+      // O / l
+      if (chunks) {
+        patience.wait(&sm.o_done[t], (chunks - 1) & 1);
+        fence_after();
+      }
+      const int tok_head = h * a.group + row - i0 * a.group;
+      const float sum = l[0] + l[1], inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      uint8_t *dst = a.out + (it.first + i0) * a.o_token_stride + tok_head * a.o_head_stride;
+#pragma unroll 1
+      for (int c = 0; c < D / 16; ++c) {
+        uint32_t x[16];
+        if (chunks) {
+          tmem_load16(x, o_at(t) + lanes + 16 * c);
+          tmem_wait_load(x);
+        }
+        if (valid) {
+          uint32_t y[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float u = sum == 0.0f ? 0.0f : __uint_as_float(x[2 * k]) * inv;
+            const float v = sum == 0.0f ? 0.0f : __uint_as_float(x[2 * k + 1]) * inv;
+            if (BF16) {
+              const __nv_bfloat162 z = __floats2bfloat162_rn(u, v);
+              y[k] = *reinterpret_cast<const uint32_t *>(&z);
+            } else {
+              y[k] = pack_half2(u, v);
+            }
+          }
+          reinterpret_cast<uint4 *>(dst)[2 * c] = make_uint4(y[0], y[1], y[2], y[3]);
+          reinterpret_cast<uint4 *>(dst)[2 * c + 1] = make_uint4(y[4], y[5], y[6], y[7]);
+        }
+      }
+      if (a.lse && valid) a.lse[(it.first + i0) * (a.kv_heads * a.group) + tok_head] = natural_lse(base, sum);
+    }
+  } else if (warp < 4 * kTiles + kFillWarps) {
+    // ---- K and V into shared memory ----
+    // Warp w brings units 2 w and 2 w + 1 of a chunk, 8 tokens at a time, a quarter of a row a lane.
+    const int w = warp - 4 * kTiles, tok = lane >> 2, quarter = lane & 3;
+    constexpr int kWords = D / 32;  // of a lane's piece, 8 channels each
+    auto page_of = [&](int u) {     // block and place of a unit, -1: none
+      const int e = (int)(((uint64_t)u * a.upb_magic) >> 40);
+      const int page = u * 16 < most && e < a.max_blocks ? a.tables[b * a.table_stride + e] : -1;
+      return page;
+    };
+    auto unit_at = [&](int u, int page) {
+      const int e = (int)(((uint64_t)u * a.upb_magic) >> 40);
+      return a.layer + page * a.block_stride + ((int64_t)h * a.upb + u - e * a.upb) * (9 * D);
+    };
+    uint32_t x[4][kWords], sc[4];  // pieces of one side of a chunk, on their way
+    int page[2], next_page[2];
+    uint32_t bad = 0;
+    auto fetch = [&](int j, int side) {
+      bad = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int u = j * (kKeys / 16) + 2 * w + i / 2, tt = (i & 1) * 8 + tok;
+        const bool good = page[i / 2] >= 0 && page[i / 2] < a.num_blocks;
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) x[i][k] = 0;
+        sc[i] = 0;  // what no row sees may be anything: its scale counts as zero
+        if (good) {
+          const uint8_t *p = unit_at(u, page[i / 2]) + side * a.kv_stride;
+          const uint8_t *row = p + tt * (D / 2) + quarter * (D / 8), *scale = p + 8 * D + tt * (D / 16) + quarter * (D / 64);
+          if constexpr (D == 128) {
+            const uint4 y = __ldg(reinterpret_cast<const uint4 *>(row));
+            x[i][0] = y.x, x[i][1] = y.y, x[i][2] = y.z, x[i][3] = y.w;
+          } else {
+            const uint2 y = __ldg(reinterpret_cast<const uint2 *>(row));
+            x[i][0] = y.x, x[i][1] = y.y;
+          }
+          if (u * 16 + tt < most) sc[i] = D == 128 ? __ldg(reinterpret_cast<const uint16_t *>(scale)) : __ldg(scale);
+        } else if (u * 16 < most) {
+          bad |= 1u << (i / 2);
+        }
+      }
+    };
+    auto put = [&](uint8_t (*dst)[ManySmem<D>::kBlock]) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = (2 * w + i / 2) * 16 + (i & 1) * 8 + tok;
+        const uint32_t s[2] = {__byte_perm(sc[i], 0, 0x0404) >> 1, __byte_perm(sc[i], 0, 0x1414) >> 1};
+#pragma unroll
+        for (int k0 = 0; k0 < kWords; ++k0) {
+          // D 128: lanes of the upper 64 channels go in another order, so that 8 lanes meet all banks
+          const bool swap = D == 128 && (quarter & 2);
+          const int k1 = k0 ^ 2;
+          const uint32_t word = D == 128 && swap ? x[i][k1 & (kWords - 1)] : x[i][k0];
+          const uint32_t scale = D == 128 ? (swap ? s[(k1 >> 1) & 1] : s[k0 >> 1]) : s[0];
+          const int k = swap ? k1 : k0;
+          uint32_t y[4];
+          e2m1x8_to_half2(word, y);
+#pragma unroll
+          for (int m = 0; m < 4; ++m) y[m] = hmul2(y[m], scale);
+          const int chunk = quarter * kWords + k;  // of 8 channels
+          *reinterpret_cast<uint4 *>(&dst[chunk >> 3][key * 128 + ((chunk & 7) ^ (key & 7)) * 16]) =
+              make_uint4(y[0], y[1], y[2], y[3]);
+        }
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < 2; ++i) page[i] = page_of(2 * w + i), next_page[i] = page_of(kKeys / 16 + 2 * w + i);
+    if (chunks) fetch(0, 0);
+    for (int j = 0; j < chunks; ++j) {
+      const int st = j & 1;
+      if (j >= 2) patience.wait(&sm.k_empty[st], ((j >> 1) + 1) & 1);
+      put(sm.k[st]);
+      if (lane == 0) sm.bad[j & 3][w] = (uint8_t)bad;  // read before chunk j + 4 gets here
+      fetch(j, 1);
+      fence_async();
+      mbar_arrive(&sm.k_full[st]);
+      if (j >= 2) patience.wait(&sm.v_empty[st], ((j >> 1) + 1) & 1);
+      put(sm.v[st]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) page[i] = next_page[i], next_page[i] = page_of((j + 2) * (kKeys / 16) + 2 * w + i);
+      if (j + 1 < chunks) fetch(j + 1, 0);
+      fence_async();
+      mbar_arrive(&sm.v_full[st]);
+    }
+  } else if (lane == 0 && chunks) {
+    // ---- the products ----
+    constexpr uint32_t kQK = mma_desc(kKeys, false), kPV = mma_desc(D, true);
+    auto score = [&](int t, int st) {
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k)
+        mma_ss(s_at(t), smem_desc(smem_addr(sm.q[t][k / 4]) + (k % 4) * 32, false),
+               smem_desc(smem_addr(sm.k[st][k / 4]) + (k % 4) * 32, false), kQK, k > 0);
+      mma_commit(&sm.s_full[t]);
+    };
+    patience.wait(&sm.q_full, 0);
+    patience.wait(&sm.k_full[0], 0);
+    fence_after();
+    for (int t = 0; t < tiles; ++t) score(t, 0);
+    mma_commit(&sm.k_empty[0]);
+    for (int j = 0; j < chunks; ++j) {
+      const int st = j & 1, next = (j + 1) & 1;
+      for (int t = 0; t < tiles; ++t) {
+        patience.wait(&sm.p_full[t], j & 1);
+        if (t == 0) patience.wait(&sm.v_full[st], (j >> 1) & 1);
+        fence_after();
+#pragma unroll
+        for (int k = 0; k < kKeys / 16; ++k)
+          mma_ts(o_at(t), s_at(t) + 8 * k, smem_desc(smem_addr(sm.v[st][0]) + k * 16 * 128, true), kPV, j > 0 || k > 0);
+        mma_commit(&sm.o_done[t]);
+        if (t == tiles - 1) mma_commit(&sm.v_empty[st]);
+        if (j + 1 < chunks) {
+          if (t == 0) patience.wait(&sm.k_full[next], ((j + 1) >> 1) & 1);
+          patience.wait(&sm.o_done[t], j & 1);  // P lies where S goes
+          fence_after();
+          score(t, next);
+          if (t == tiles - 1) mma_commit(&sm.k_empty[next]);
+        }
+      }
+    }
+  }
+
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 4 * kTiles + kFillWarps)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
 // A number of 48 bits for each launch, from a start that differs between processes.
 unsigned long long next_call() {
   static std::atomic<unsigned long long> last{[] {
@@ -812,6 +1279,21 @@ int launch_decode(const AttnArgs &a, int nt, int ctas, void *workspace, cudaStre
   }
 }
 
+template <int D, bool BF16>
+int launch_many(const AttnArgs &a, cudaStream_t s) {
+  const int smem = sizeof(ManySmem<D>) + 1024;
+  auto kernel = fp4_many_kernel<D, BF16>;
+  FKV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  // a bound of the blocks of rows: the sequences' lengths are on the device
+  const int64_t blocks = a.num_q * a.group / (kTiles * 128) + a.num_seqs;
+  kernel<<<dim3((unsigned)blocks, a.kv_heads), kManyThreads, smem, s>>>(a);
+  FKV_CUDA(cudaGetLastError());
+  note_launch();
+  return FKV_OK;
+}
+
+constexpr int kFewRows = 64;  // rows of a key head up to which the few-rows kernel runs
+
 // Tiles of 8 rows that go through the cache together.
 int row_tiles(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
 
@@ -826,6 +1308,7 @@ int64_t fkv_fp4_attention_workspace(int64_t num_q_tokens, int num_q_heads, int n
                                     int max_q_len) {
   ThreadDeviceCtx *ctx;
   if (num_kv_heads <= 0 || get_ctx(-1, &ctx) != FKV_OK) return 0;
+  if ((int64_t)max_q_len * (num_q_heads / num_kv_heads) > kFewRows) return 0;
   return decode_workspace(head_size, row_tiles((int64_t)max_q_len * (num_q_heads / num_kv_heads)), ctx->num_sms);
 }
 
@@ -872,11 +1355,15 @@ int fkv_fp4_attention(const void *layer, int64_t num_blocks, int tokens_per_bloc
   ThreadDeviceCtx *ctx;
   const int rc = get_ctx(-1, &ctx);
   if (rc != FKV_OK) return rc;
+  cudaStream_t s = (cudaStream_t)stream;
+  const bool bf16 = dtype == FKV_DTYPE_BF16;
+  if ((int64_t)max_q_len * a.group > kFewRows) {
+    if (head_size == 128) return bf16 ? launch_many<128, true>(a, s) : launch_many<128, false>(a, s);
+    return bf16 ? launch_many<64, true>(a, s) : launch_many<64, false>(a, s);
+  }
   const int nt = row_tiles((int64_t)max_q_len * a.group);
   if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < decode_workspace(head_size, nt, ctx->num_sms))
     return bad("the workspace is too small or not aligned");
-  cudaStream_t s = (cudaStream_t)stream;
-  const bool bf16 = dtype == FKV_DTYPE_BF16;
   if (head_size == 128)
     return bf16 ? launch_decode<128, true>(a, nt, ctx->num_sms, workspace, s) : launch_decode<128, false>(a, nt, ctx->num_sms, workspace, s);
   return bf16 ? launch_decode<64, true>(a, nt, ctx->num_sms, workspace, s) : launch_decode<64, false>(a, nt, ctx->num_sms, workspace, s);
