@@ -791,7 +791,10 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
 
 constexpr int kTiles = 2, kKeys = 128;
 constexpr int kFillWarps = 4;
-constexpr int kManyThreads = (4 * kTiles + kFillWarps + 1) * 32;
+constexpr int kManyThreads = (4 * kTiles + kFillWarps + 4) * 32;  // the last four: one issues the products
+// Registers of a thread of each kind; launched with 128, so the sum over all may be 512 * 128.
+constexpr int kRowRegs = 184, kFillRegs = 96, kIssueRegs = 40;
+static_assert(kRowRegs * 128 * kTiles + kFillRegs * 128 + kIssueRegs * 128 <= kManyThreads * 128, "register split");
 
 template <int D>
 struct ManySmem {
@@ -862,6 +865,36 @@ __device__ __forceinline__ void mma_commit(uint64_t *m) {
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Two floats in a register pair, as the packed instructions take them.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 #define FKV_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
 #define FKV_W8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
@@ -964,6 +997,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
 
   if (warp < 4 * kTiles) {
     // ---- a thread for each row ----
+    more_registers<kRowRegs>();
     const int t = warp >> 2, r = (warp & 3) * 32 + lane, row = row0 + t * 128 + r;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // the warp's 32 lanes of tensor memory
     if (t < tiles) {
@@ -1004,32 +1038,37 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
 
       const int end = valid ? end_of(row) : 0;
       const int lowest = __reduce_min_sync(~0u, valid ? end : INT32_MAX);
-      float base = kNone, bar = -INFINITY, l[2] = {0, 0};
+      float base = kNone, bar = -INFINITY, l[4] = {0, 0, 0, 0};
       for (int j = 0; j < chunks; ++j) {
         patience.wait(&sm.s_full[t], j & 1);
         fence_after();
         const uint32_t S = s_at(t) + lanes;
         const uint32_t bad = *(volatile uint32_t *)sm.bad[j & 3];
         const bool hide = (j + 1) * kKeys > lowest || bad;
-        auto hidden = [&](uint32_t(&x)[32], int c) {  // scores of columns 32 c on that the row does not see
-          const uint32_t gone = bad >> (8 * c);
+        uint32_t x[4][32];
+        tmem_load32(x[0], S), tmem_load32(x[1], S + 32);
+        tmem_wait_load(x[0]), tmem_wait_load(x[1]);
+        tmem_load32(x[2], S + 64), tmem_load32(x[3], S + 96);
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        auto half = [&](int c0) {  // what the row sees of 64 columns, and the largest of it
+          if (hide) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (((gone >> (i / 16)) & 1) || j * kKeys + 32 * c + i >= end) x[i] = 0xFF800000u;
+            for (int c = c0; c < c0 + 2; ++c) {
+              const uint32_t gone = bad >> (8 * c);
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (((gone >> (i / 16)) & 1) || j * kKeys + 32 * c + i >= end) x[c][i] = 0xFF800000u;
+            }
+          }
+#pragma unroll
+          for (int c = c0; c < c0 + 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[c][i]));
         };
-        uint32_t x[2][32];
-        // the largest score first: P is going to lie over S
-        float top[2] = {-INFINITY, -INFINITY};
-        tmem_load32(x[0], S);
-#pragma unroll
-        for (int c = 0; c < kKeys / 32; ++c) {
-          tmem_wait_load(x[c & 1]);
-          tmem_load32(x[(c + 1) & 1], S + 32 * ((c + 1) % (kKeys / 32)));  // the last: the next pass's first
-          if (hide) hidden(x[c & 1], c);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) top[i & 1] = fmaxf(top[i & 1], __uint_as_float(x[c & 1][i]));
-        }
-        const float most_here = fmaxf(top[0], top[1]);
+        half(0);
+        tmem_wait_load(x[2]), tmem_wait_load(x[3]);
+        half(2);
+        const float most_here = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         if (__any_sync(~0u, most_here > bar)) {  // rare after the first chunks
           float f = 1.0f;
           if (most_here > bar) {  // other rows stay: a row does not depend on its neighbours
@@ -1038,11 +1077,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
             base = to;
             bar = __fdividef(to + kMove, mul);
           }
-          l[0] *= f, l[1] *= f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) l[i] *= f;
           if (j > 0) {  // the product before is done: this chunk's S came after it
             patience.wait(&sm.o_done[t], (j - 1) & 1);
             fence_after();
-            tmem_wait_load(x[0]);
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
               uint32_t y[16];
@@ -1054,21 +1093,25 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
             }
           }
         }
+        const uint64_t mul2 = pair(mul, mul), base2 = pair(-base, -base);
+        uint64_t l01 = pair(l[0], l[1]), l23 = pair(l[2], l[3]);
 #pragma unroll
-        for (int c = 0; c < kKeys / 32; ++c) {
-          tmem_wait_load(x[c & 1]);
-          if (c + 1 < kKeys / 32) tmem_load32(x[(c + 1) & 1], S + 32 * (c + 1));
-          if (hide) hidden(x[c & 1], c);
+        for (int c = 0; c < 4; ++c) {
           uint32_t p[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float u = exp2_fast(fmaf(__uint_as_float(x[c & 1][2 * i]), mul, -base));
-            const float v = exp2_fast(fmaf(__uint_as_float(x[c & 1][2 * i + 1]), mul, -base));
-            l[0] += u, l[1] += v;
+            const float2 y = unpair(fma2(pair(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])), mul2, base2));
+            const float u = exp2_fast(y.x), v = exp2_fast(y.y);
+            if (i & 1)
+              l23 = add2(l23, pair(u, v));
+            else
+              l01 = add2(l01, pair(u, v));
             p[i] = pack_half2(u, v);
           }
-          tmem_store16(S + 16 * c, p);  // over columns that have been read
+          tmem_store16(S + 16 * c, p);
         }
+        const float2 la = unpair(l01), lb = unpair(l23);
+        l[0] = la.x, l[1] = la.y, l[2] = lb.x, l[3] = lb.y;
         tmem_wait_store();
         fence_before();
         mbar_arrive(&sm.p_full[t]);
@@ -1080,7 +1123,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
         fence_after();
       }
       const int tok_head = h * a.group + row - i0 * a.group;
-      const float sum = l[0] + l[1], inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const float sum = (l[0] + l[1]) + (l[2] + l[3]), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
       uint8_t *dst = a.out + (it.first + i0) * a.o_token_stride + tok_head * a.o_head_stride;
 #pragma unroll 1
       for (int c = 0; c < D / 16; ++c) {
@@ -1110,6 +1153,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
     }
   } else if (warp < 4 * kTiles + kFillWarps) {
     // ---- K and V into shared memory ----
+    fewer_registers<kFillRegs>();
     // Warp w brings units 2 w and 2 w + 1 of a chunk, 8 tokens at a time, a quarter of a row a lane.
     const int w = warp - 4 * kTiles, tok = lane >> 2, quarter = lane & 3;
     constexpr int kWords = D / 32;  // of a lane's piece, 8 channels each
@@ -1192,8 +1236,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
       fence_async();
       mbar_arrive(&sm.v_full[st]);
     }
-  } else if (lane == 0 && chunks) {
+  } else {
     // ---- the products ----
+    fewer_registers<kIssueRegs>();
+    if (warp == 4 * kTiles + kFillWarps && lane == 0 && chunks) {
     constexpr uint32_t kQK = mma_desc(kKeys, false), kPV = mma_desc(D, true);
     auto score = [&](int t, int st) {
 #pragma unroll
@@ -1226,6 +1272,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
           if (t == tiles - 1) mma_commit(&sm.k_empty[next]);
         }
       }
+    }
     }
   }
 
