@@ -937,13 +937,30 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   auto &sm = *reinterpret_cast<ManySmem<D> *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = blockIdx.y;
+  const int h = blockIdx.x % a.kv_heads, at = blockIdx.x / a.kv_heads;  // a block's heads run together
 
-  // the sequence and its block of rows: the last CTAs of a sequence have most keys, so they come first
+  // The sequence and its block of rows.  The last blocks of a sequence have most keys, so they come first; with up
+  // to 32 sequences the last of each come before the second last of any.
   int b = -1, rb = 0;
   Item it;
-  {
-    int want = gridDim.x - 1 - blockIdx.x, before = 0;
+  if (a.num_seqs <= 32) {
+    const int want = at, blocks = lane < a.num_seqs ? item_of<R>(a, lane).blocks : 0;
+    int lo = 0, hi = __reduce_max_sync(~0u, blocks);  // the depth d with sum min(blocks, d) <= want < that of d + 1
+    if (want >= __reduce_add_sync(~0u, blocks)) return;  // the grid is an upper bound
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if ((int)__reduce_add_sync(~0u, min(blocks, mid)) <= want)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    const int nth = want - (int)__reduce_add_sync(~0u, min(blocks, lo));
+    const uint32_t have = __ballot_sync(~0u, blocks > lo);
+    b = (int)__fns(have, 0, nth + 1);
+    rb = __shfl_sync(~0u, blocks, b) - 1 - lo;
+  } else {
+    const int want = gridDim.x / a.kv_heads - 1 - at;
+    int before = 0;
     for (int b0 = 0; b0 < a.num_seqs; b0 += 32) {
       const int mine = b0 + lane < a.num_seqs ? item_of<R>(a, b0 + lane).blocks : 0;
       int upto = mine;
@@ -961,9 +978,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
       }
       before += __shfl_sync(~0u, upto, 31);
     }
-    if (b < 0) return;  // the grid is an upper bound
-    it = item_of<R>(a, b);
+    if (b < 0) return;
   }
+  it = item_of<R>(a, b);
   const int row0 = rb * R, nrows = it.rows * a.group;
   const int tiles = nrows - row0 > 128 ? 2 : 1;
   auto end_of = [&](int row) {  // the keys that a row sees
@@ -1154,85 +1171,89 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
   } else if (warp < 4 * kTiles + kFillWarps) {
     // ---- K and V into shared memory ----
     fewer_registers<kFillRegs>();
-    // Warp w brings units 2 w and 2 w + 1 of a chunk, 8 tokens at a time, a quarter of a row a lane.
-    const int w = warp - 4 * kTiles, tok = lane >> 2, quarter = lane & 3;
+    // Warp w brings units 2 w and 2 w + 1 of a chunk, 8 tokens at a time, a quarter of a row a lane: 8 lanes
+    // that store together have 8 rows, so the swizzle spreads them over all banks.
+    const int w = warp - 4 * kTiles, tok = lane & 7, quarter = lane >> 3;
     constexpr int kWords = D / 32;  // of a lane's piece, 8 channels each
-    auto page_of = [&](int u) {     // block and place of a unit, -1: none
-      const int e = (int)(((uint64_t)u * a.upb_magic) >> 40);
-      const int page = u * 16 < most && e < a.max_blocks ? a.tables[b * a.table_stride + e] : -1;
-      return page;
-    };
-    auto unit_at = [&](int u, int page) {
-      const int e = (int)(((uint64_t)u * a.upb_magic) >> 40);
-      return a.layer + page * a.block_stride + ((int64_t)h * a.upb + u - e * a.upb) * (9 * D);
+    const int at_row = tok * (D / 2) + quarter * (D / 8), at_scale = 8 * D + tok * (D / 16) + quarter * (D / 64);
+    uint32_t at_chunk[kWords];  // a lane's pieces of a row in shared memory
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) {
+      const int c = quarter * kWords + k;
+      at_chunk[k] = (c >> 3) * ManySmem<D>::kBlock + w * 32 * 128 + tok * 128 + ((c & 7) ^ tok) * 16;
+    }
+    auto page_of = [&](int j, int i) {
+      const int u = j * (kKeys / 16) + 2 * w + i, e = (int)(((uint64_t)u * a.upb_magic) >> 40);
+      return u * 16 < most && e < a.max_blocks ? a.tables[b * a.table_stride + e] : -1;
     };
     uint32_t x[4][kWords], sc[4];  // pieces of one side of a chunk, on their way
-    int page[2], next_page[2];
+    const uint8_t *unit[2];        // the chunk's units; any place where there is none, and no scale is taken
+    int page[2];
     uint32_t bad = 0;
-    auto fetch = [&](int j, int side) {
+    auto find = [&](int j) {  // the units of chunk j, and the pages of the chunk after it
       bad = 0;
 #pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int u = j * (kKeys / 16) + 2 * w + i, e = (int)(((uint64_t)u * a.upb_magic) >> 40);
+        const bool good = page[i] >= 0 && page[i] < a.num_blocks;
+        unit[i] = good ? a.layer + page[i] * a.block_stride + ((int64_t)h * a.upb + u - e * a.upb) * (9 * D) : nullptr;
+        bad |= !good && u * 16 < most ? 1u << i : 0;
+        page[i] = page_of(j + 1, i);
+      }
+    };
+    auto fetch = [&](int j, int64_t side) {
+#pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int u = j * (kKeys / 16) + 2 * w + i / 2, tt = (i & 1) * 8 + tok;
-        const bool good = page[i / 2] >= 0 && page[i / 2] < a.num_blocks;
+        const uint8_t *p = unit[i >> 1];
+        sc[i] = 0;  // what no row sees may be anything: its scale counts as zero
 #pragma unroll
         for (int k = 0; k < kWords; ++k) x[i][k] = 0;
-        sc[i] = 0;  // what no row sees may be anything: its scale counts as zero
-        if (good) {
-          const uint8_t *p = unit_at(u, page[i / 2]) + side * a.kv_stride;
-          const uint8_t *row = p + tt * (D / 2) + quarter * (D / 8), *scale = p + 8 * D + tt * (D / 16) + quarter * (D / 64);
+        if (p) {
+          p += side + (i & 1) * 8 * (D / 2);
           if constexpr (D == 128) {
-            const uint4 y = __ldg(reinterpret_cast<const uint4 *>(row));
+            const uint4 y = __ldg(reinterpret_cast<const uint4 *>(p + at_row));
             x[i][0] = y.x, x[i][1] = y.y, x[i][2] = y.z, x[i][3] = y.w;
           } else {
-            const uint2 y = __ldg(reinterpret_cast<const uint2 *>(row));
+            const uint2 y = __ldg(reinterpret_cast<const uint2 *>(p + at_row));
             x[i][0] = y.x, x[i][1] = y.y;
           }
-          if (u * 16 + tt < most) sc[i] = D == 128 ? __ldg(reinterpret_cast<const uint16_t *>(scale)) : __ldg(scale);
-        } else if (u * 16 < most) {
-          bad |= 1u << (i / 2);
+          p += at_scale - (i & 1) * 8 * (D / 2 - D / 16);
+          if (j * kKeys + (2 * w + (i >> 1)) * 16 + (i & 1) * 8 + tok < most)
+            sc[i] = D == 128 ? __ldg(reinterpret_cast<const uint16_t *>(p)) : __ldg(p);
         }
       }
     };
-    auto put = [&](uint8_t (*dst)[ManySmem<D>::kBlock]) {
+    auto put = [&](uint32_t dst) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int key = (2 * w + i / 2) * 16 + (i & 1) * 8 + tok;
         const uint32_t s[2] = {__byte_perm(sc[i], 0, 0x0404) >> 1, __byte_perm(sc[i], 0, 0x1414) >> 1};
 #pragma unroll
-        for (int k0 = 0; k0 < kWords; ++k0) {
-          // D 128: lanes of the upper 64 channels go in another order, so that 8 lanes meet all banks
-          const bool swap = D == 128 && (quarter & 2);
-          const int k1 = k0 ^ 2;
-          const uint32_t word = D == 128 && swap ? x[i][k1 & (kWords - 1)] : x[i][k0];
-          const uint32_t scale = D == 128 ? (swap ? s[(k1 >> 1) & 1] : s[k0 >> 1]) : s[0];
-          const int k = swap ? k1 : k0;
+        for (int k = 0; k < kWords; ++k) {
           uint32_t y[4];
-          e2m1x8_to_half2(word, y);
+          e2m1x8_to_half2(x[i][k], y);
 #pragma unroll
-          for (int m = 0; m < 4; ++m) y[m] = hmul2(y[m], scale);
-          const int chunk = quarter * kWords + k;  // of 8 channels
-          *reinterpret_cast<uint4 *>(&dst[chunk >> 3][key * 128 + ((chunk & 7) ^ (key & 7)) * 16]) =
-              make_uint4(y[0], y[1], y[2], y[3]);
+          for (int m = 0; m < 4; ++m) y[m] = hmul2(y[m], s[D == 128 ? k >> 1 : 0]);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + at_chunk[k] + i * 8 * 128), "r"(y[0]), "r"(y[1]),
+                       "r"(y[2]), "r"(y[3])
+                       : "memory");
         }
       }
     };
-#pragma unroll
-    for (int i = 0; i < 2; ++i) page[i] = page_of(2 * w + i), next_page[i] = page_of(kKeys / 16 + 2 * w + i);
-    if (chunks) fetch(0, 0);
+    const uint32_t k_at = smem_addr(sm.k[0]), v_at = smem_addr(sm.v[0]);
+    constexpr uint32_t kStage = D / 64 * ManySmem<D>::kBlock;
+    page[0] = page_of(0, 0), page[1] = page_of(0, 1);
+    if (chunks) find(0), fetch(0, 0);
     for (int j = 0; j < chunks; ++j) {
       const int st = j & 1;
       if (j >= 2) patience.wait(&sm.k_empty[st], ((j >> 1) + 1) & 1);
-      put(sm.k[st]);
+      put(k_at + st * kStage);
       if (lane == 0) sm.bad[j & 3][w] = (uint8_t)bad;  // read before chunk j + 4 gets here
-      fetch(j, 1);
+      fetch(j, a.kv_stride);
       fence_async();
       mbar_arrive(&sm.k_full[st]);
       if (j >= 2) patience.wait(&sm.v_empty[st], ((j >> 1) + 1) & 1);
-      put(sm.v[st]);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) page[i] = next_page[i], next_page[i] = page_of((j + 2) * (kKeys / 16) + 2 * w + i);
-      if (j + 1 < chunks) fetch(j + 1, 0);
+      put(v_at + st * kStage);
+      if (j + 1 < chunks) find(j + 1), fetch(j + 1, 0);
       fence_async();
       mbar_arrive(&sm.v_full[st]);
     }
@@ -1333,7 +1354,8 @@ int launch_many(const AttnArgs &a, cudaStream_t s) {
   FKV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   // a bound of the blocks of rows: the sequences' lengths are on the device
   const int64_t blocks = a.num_q * a.group / (kTiles * 128) + a.num_seqs;
-  kernel<<<dim3((unsigned)blocks, a.kv_heads), kManyThreads, smem, s>>>(a);
+  if (blocks * a.kv_heads > INT32_MAX) return fail(FKV_ERR_INVALID_ARG, "fkv_fp4_attention: 2^31 blocks of rows or more");
+  kernel<<<(unsigned)(blocks * a.kv_heads), kManyThreads, smem, s>>>(a);
   FKV_CUDA(cudaGetLastError());
   note_launch();
   return FKV_OK;
