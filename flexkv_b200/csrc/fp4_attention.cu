@@ -847,20 +847,32 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, bool mn_major) {
 __host__ __device__ constexpr uint32_t mma_desc(int n, bool b_mn_major) {
   return 1u << 4 | (b_mn_major ? 1u << 16 : 0) | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add) {
+// The whole warp goes through the issuing code, so that operands stay in uniform
+// registers; `one` picks the thread that issues.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add, uint32_t one) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-      "l"(a), "l"(b), "r"(desc), "r"((int)add)
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(desc), "r"((int)add), "r"(one)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, bool add) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, bool add, uint32_t one) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-      "r"(a), "l"(b), "r"(desc), "r"((int)add)
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(desc), "r"((int)add), "r"(one)
       : "memory");
 }
-__device__ __forceinline__ void mma_commit(uint64_t *m) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(m)) : "memory");
+__device__ __forceinline__ void mma_commit(uint64_t *m, uint32_t one) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(smem_addr(m)), "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t one;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.b32 %0, 1, 0, p;\n}" : "=r"(one));
+  return one;
 }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -1260,40 +1272,60 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
   } else {
     // ---- the products ----
     fewer_registers<kIssueRegs>();
-    if (warp == 4 * kTiles + kFillWarps && lane == 0 && chunks) {
-    constexpr uint32_t kQK = mma_desc(kKeys, false), kPV = mma_desc(D, true);
-    auto score = [&](int t, int st) {
+    if (warp == 4 * kTiles + kFillWarps && chunks) {
+      constexpr uint32_t kQK = mma_desc(kKeys, false), kPV = mma_desc(D, true);
+      constexpr uint32_t kTile = D / 64 * ManySmem<D>::kBlock / 16, kBlock16 = ManySmem<D>::kBlock / 16;  // in descriptors
+      const uint32_t one = elect_one();
+      const uint32_t mem = __shfl_sync(~0u, tmem, 0);
+      const uint64_t q_desc = smem_desc(smem_addr(sm.q), false), k_desc = smem_desc(smem_addr(sm.k), false),
+                     v_desc = smem_desc(smem_addr(sm.v), true);
+      // loops and not straight code: this warp shares its instruction cache with three busier ones
+      auto score = [&](int t, uint64_t kk) {
+        uint64_t q = q_desc + t * kTile;
+        const uint32_t d = mem + (kTiles + t) * 128;
+#pragma unroll 1
+        for (int k = 0; k < D / 64; ++k, q += kBlock16, kk += kBlock16) {
+          mma_ss(d, q, kk, kQK, k > 0, one);
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k)
-        mma_ss(s_at(t), smem_desc(smem_addr(sm.q[t][k / 4]) + (k % 4) * 32, false),
-               smem_desc(smem_addr(sm.k[st][k / 4]) + (k % 4) * 32, false), kQK, k > 0);
-      mma_commit(&sm.s_full[t]);
-    };
-    patience.wait(&sm.q_full, 0);
-    patience.wait(&sm.k_full[0], 0);
-    fence_after();
-    for (int t = 0; t < tiles; ++t) score(t, 0);
-    mma_commit(&sm.k_empty[0]);
-    for (int j = 0; j < chunks; ++j) {
-      const int st = j & 1, next = (j + 1) & 1;
-      for (int t = 0; t < tiles; ++t) {
-        patience.wait(&sm.p_full[t], j & 1);
-        if (t == 0) patience.wait(&sm.v_full[st], (j >> 1) & 1);
-        fence_after();
-#pragma unroll
-        for (int k = 0; k < kKeys / 16; ++k)
-          mma_ts(o_at(t), s_at(t) + 8 * k, smem_desc(smem_addr(sm.v[st][0]) + k * 16 * 128, true), kPV, j > 0 || k > 0);
-        mma_commit(&sm.o_done[t]);
-        if (t == tiles - 1) mma_commit(&sm.v_empty[st]);
-        if (j + 1 < chunks) {
-          if (t == 0) patience.wait(&sm.k_full[next], ((j + 1) >> 1) & 1);
-          patience.wait(&sm.o_done[t], j & 1);  // P lies where S goes
-          fence_after();
-          score(t, next);
-          if (t == tiles - 1) mma_commit(&sm.k_empty[next]);
+          for (int i = 1; i < 4; ++i) mma_ss(d, q + i * 2, kk + i * 2, kQK, true, one);
         }
+        mma_commit(&sm.s_full[t], one);
+      };
+      patience.wait(&sm.q_full, 0);
+      patience.wait(&sm.k_full[0], 0);
+      fence_after();
+#pragma unroll 1
+      for (int t = 0; t < tiles; ++t) score(t, k_desc);
+      mma_commit(&sm.k_empty[0], one);
+#pragma unroll 1
+      for (int j = 0; j < chunks; ++j) {
+        const int st = j & 1, next = st ^ 1;
+        const bool more = j + 1 < chunks;
+        patience.wait(&sm.v_full[st], (j >> 1) & 1);
+        if (more) patience.wait(&sm.k_full[next], ((j + 1) >> 1) & 1);
+#pragma unroll 1
+        for (int t = 0; t < tiles; ++t) {
+          patience.wait(&sm.p_full[t], j & 1);
+          fence_after();
+          uint64_t v = v_desc + st * kTile;
+          const uint32_t d = mem + t * 128;
+          uint32_t p = d + kTiles * 128;
+#pragma unroll 1
+          for (int k = 0; k < kKeys / 64; ++k, v += 4 * 128, p += 4 * 8) {
+            mma_ts(d, p, v, kPV, j + k > 0, one);
+#pragma unroll
+            for (int i = 1; i < 4; ++i) mma_ts(d, p + i * 8, v + i * 128, kPV, true, one);
+          }
+          mma_commit(&sm.o_done[t], one);
+          if (more) {
+            patience.wait(&sm.o_done[t], j & 1);  // P lies where S goes
+            fence_after();
+            score(t, k_desc + next * kTile);
+          }
+        }
+        mma_commit(&sm.v_empty[st], one);
+        if (more) mma_commit(&sm.k_empty[next], one);
       }
-    }
     }
   }
 
