@@ -779,31 +779,30 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
 //    registers (a chunk ahead), to half, into shared memory in the 128-byte
 //    swizzled layout.  K as it lies is K-major for S = Q K^T, V is MN-major
 //    for O = P V: no transpose;
-//  * one thread issues the products: S of a tile of 128 rows into tensor
-//    memory, and O += P V with P read from tensor memory;
+//  * one thread for each tile of 128 rows issues its products: S into tensor
+//    memory, and O += P V with P read from there;
 //  * four warps for each tile of rows take S, a thread a row: weights
 //    2^(score - base) in half go back over S as P, their sum stays in the
 //    thread.  The base moves only when a score passes it by kMove, as in the
 //    kernel above: then the weights are taken again and O is scaled in place.
 // Two tiles of rows alternate: while one is in softmax the tensor core works
-// on the other, and K and V are converted once for both.
-// Tensor memory (512 columns): O of both tiles, S of both; P lies over S.
+// on the other, and K and V are converted once for both.  A tile has two
+// buffers for S, so that the next scores are there when a softmax ends.
+// Tensor memory (512 columns): O of both tiles, two S of both; P lies over S.
 
-constexpr int kTiles = 2, kKeys = 128;
+constexpr int kTiles = 2, kKeys = 64, kRing = 4;
 constexpr int kFillWarps = 4;
-constexpr int kManyThreads = (4 * kTiles + kFillWarps + 4) * 32;  // the last four: one issues the products
-// Registers of a thread of each kind; launched with 128, so the sum over all may be 512 * 128.
-constexpr int kRowRegs = 184, kFillRegs = 96, kIssueRegs = 40;
-static_assert(kRowRegs * 128 * kTiles + kFillRegs * 128 + kIssueRegs * 128 <= kManyThreads * 128, "register split");
+constexpr int kManyThreads = (4 * kTiles + kFillWarps + kTiles) * 32;
 
 template <int D>
 struct ManySmem {
-  static constexpr int kBlock = 128 * 128;  // 128 rows of 64 halves, swizzled
-  alignas(1024) uint8_t q[kTiles][D / 64][kBlock];
-  alignas(1024) uint8_t k[2][D / 64][kBlock];
-  alignas(1024) uint8_t v[2][D / 64][kBlock];
-  uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[kTiles], p_full[kTiles], o_done[kTiles];
-  alignas(4) uint8_t bad[4][kFillWarps];  // of a chunk of keys, a warp's two units: whose page is outside the pool
+  static constexpr int kRows = 128 * 128, kCols = kKeys * 128;  // 64 halves of 128 rows, of kKeys keys, swizzled
+  alignas(1024) uint8_t q[kTiles][D / 64][kRows];
+  alignas(1024) uint8_t k[kRing][D / 64][kCols];
+  alignas(1024) uint8_t v[kRing][D / 64][kCols];
+  uint64_t q_full, k_full[kRing], v_full[kRing], k_empty[kRing], v_empty[kRing];
+  uint64_t s_full[kTiles][2], p_full[kTiles][2], o_done[kTiles];
+  alignas(4) uint8_t bad[2 * kRing][kFillWarps];  // of a chunk of keys, a warp's unit: its page is outside the pool
   uint32_t tmem;
 };
 
@@ -838,9 +837,9 @@ struct Patience {
 
 // A shared memory operand in the 128-byte swizzled layout.  K-major: 8 rows of
 // 128 bytes every 1024 bytes.  MN-major: 8 rows along K every 1024 bytes, the
-// next 64 columns a block of 128 rows further.
+// next 64 columns a block of kKeys rows further.
 __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, bool mn_major) {
-  return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)(mn_major ? (128 * 128) >> 4 : 1) << 16 | (uint64_t)(1024 >> 4) << 32 |
+  return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)(mn_major ? (kKeys * 128) >> 4 : 1) << 16 | (uint64_t)(1024 >> 4) << 32 |
          (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 // 128 rows, N columns, half operands, float sums.
@@ -899,15 +898,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-template <int N>
-__device__ __forceinline__ void more_registers() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void fewer_registers() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-
 #define FKV_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
 #define FKV_W8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
 // 16 or 32 columns of the warp's 32 lanes.
@@ -1005,11 +995,14 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
 
   if (threadIdx.x == 0) {
     mbar_init(&sm.q_full, 128 * tiles);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kRing; ++i) {
       mbar_init(&sm.k_full[i], kFillWarps * 32), mbar_init(&sm.v_full[i], kFillWarps * 32);
-      mbar_init(&sm.k_empty[i], 1), mbar_init(&sm.v_empty[i], 1);
+      mbar_init(&sm.k_empty[i], tiles), mbar_init(&sm.v_empty[i], tiles);
     }
-    for (int t = 0; t < kTiles; ++t) mbar_init(&sm.s_full[t], 1), mbar_init(&sm.p_full[t], 128), mbar_init(&sm.o_done[t], 1);
+    for (int t = 0; t < kTiles; ++t) {
+      for (int i = 0; i < 2; ++i) mbar_init(&sm.s_full[t][i], 1), mbar_init(&sm.p_full[t][i], 128);
+      mbar_init(&sm.o_done[t], 1);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 4 * kTiles + kFillWarps) {
@@ -1021,12 +1014,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
   fence_after();
   const uint32_t tmem = sm.tmem;
   auto o_at = [&](int t) { return tmem + t * 128; };
-  auto s_at = [&](int t) { return tmem + (kTiles + t) * 128; };
+  auto s_at = [&](int t, int i) { return tmem + (kTiles + t) * 128 + i * kKeys; };
   Patience patience;
 
   if (warp < 4 * kTiles) {
     // ---- a thread for each row ----
-    more_registers<kRowRegs>();
     const int t = warp >> 2, r = (warp & 3) * 32 + lane, row = row0 + t * 128 + r;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // the warp's 32 lanes of tensor memory
     if (t < tiles) {
@@ -1069,34 +1061,25 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
       const int lowest = __reduce_min_sync(~0u, valid ? end : INT32_MAX);
       float base = kNone, bar = -INFINITY, l[4] = {0, 0, 0, 0};
       for (int j = 0; j < chunks; ++j) {
-        patience.wait(&sm.s_full[t], j & 1);
+        patience.wait(&sm.s_full[t][j & 1], (j >> 1) & 1);
         fence_after();
-        const uint32_t S = s_at(t) + lanes;
-        const uint32_t bad = *(volatile uint32_t *)sm.bad[j & 3];
-        const bool hide = (j + 1) * kKeys > lowest || bad;
-        uint32_t x[4][32];
+        const uint32_t S = s_at(t, j & 1) + lanes;
+        uint32_t x[2][32];
         tmem_load32(x[0], S), tmem_load32(x[1], S + 32);
+        const uint32_t bad = *(volatile uint32_t *)sm.bad[j & (2 * kRing - 1)];
         tmem_wait_load(x[0]), tmem_wait_load(x[1]);
-        tmem_load32(x[2], S + 64), tmem_load32(x[3], S + 96);
+        if ((j + 1) * kKeys > lowest || bad) {  // only what the row sees
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (j * kKeys + 32 * c + i >= end || ((bad >> (8 * (2 * c + i / 16))) & 1)) x[c][i] = 0xFF800000u;
+        }
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        auto half = [&](int c0) {  // what the row sees of 64 columns, and the largest of it
-          if (hide) {
 #pragma unroll
-            for (int c = c0; c < c0 + 2; ++c) {
-              const uint32_t gone = bad >> (8 * c);
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (((gone >> (i / 16)) & 1) || j * kKeys + 32 * c + i >= end) x[c][i] = 0xFF800000u;
-            }
-          }
-#pragma unroll
-          for (int c = c0; c < c0 + 2; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[c][i]));
-        };
-        half(0);
-        tmem_wait_load(x[2]), tmem_wait_load(x[3]);
-        half(2);
+          for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[c][i]));
         const float most_here = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         if (__any_sync(~0u, most_here > bar)) {  // rare after the first chunks
           float f = 1.0f;
@@ -1108,7 +1091,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) l[i] *= f;
-          if (j > 0) {  // the product before is done: this chunk's S came after it
+          if (j > 0) {
             patience.wait(&sm.o_done[t], (j - 1) & 1);
             fence_after();
 #pragma unroll 1
@@ -1125,7 +1108,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
         const uint64_t mul2 = pair(mul, mul), base2 = pair(-base, -base);
         uint64_t l01 = pair(l[0], l[1]), l23 = pair(l[2], l[3]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
           uint32_t p[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -1143,11 +1126,14 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
         l[0] = la.x, l[1] = la.y, l[2] = lb.x, l[3] = lb.y;
         tmem_wait_store();
         fence_before();
-        mbar_arrive(&sm.p_full[t]);
+        mbar_arrive(&sm.p_full[t][j & 1]);
       }
 
       // O / l
       if (chunks) {
+        // the last S came after the product two chunks before it: the one between is waited for first, or a
+        // wait for the last could take the phase before that one for it
+        if (chunks > 1) patience.wait(&sm.o_done[t], (chunks - 2) & 1);
         patience.wait(&sm.o_done[t], (chunks - 1) & 1);
         fence_after();
       }
@@ -1182,9 +1168,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
     }
   } else if (warp < 4 * kTiles + kFillWarps) {
     // ---- K and V into shared memory ----
-    fewer_registers<kFillRegs>();
-    // Warp w brings units 2 w and 2 w + 1 of a chunk, 8 tokens at a time, a quarter of a row a lane: 8 lanes
-    // that store together have 8 rows, so the swizzle spreads them over all banks.
+    // Warp w brings unit w of a chunk, 8 tokens at a time, a quarter of a row a lane: 8 lanes that store together
+    // have 8 rows, so the swizzle spreads them over all banks.
     const int w = warp - 4 * kTiles, tok = lane & 7, quarter = lane >> 3;
     constexpr int kWords = D / 32;  // of a lane's piece, 8 channels each
     const int at_row = tok * (D / 2) + quarter * (D / 8), at_scale = 8 * D + tok * (D / 16) + quarter * (D / 64);
@@ -1192,57 +1177,52 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
 #pragma unroll
     for (int k = 0; k < kWords; ++k) {
       const int c = quarter * kWords + k;
-      at_chunk[k] = (c >> 3) * ManySmem<D>::kBlock + w * 32 * 128 + tok * 128 + ((c & 7) ^ tok) * 16;
+      at_chunk[k] = (c >> 3) * ManySmem<D>::kCols + w * 16 * 128 + tok * 128 + ((c & 7) ^ tok) * 16;
     }
-    auto page_of = [&](int j, int i) {
-      const int u = j * (kKeys / 16) + 2 * w + i, e = (int)(((uint64_t)u * a.upb_magic) >> 40);
+    auto page_of = [&](int j) {
+      const int u = j * (kKeys / 16) + w, e = (int)(((uint64_t)u * a.upb_magic) >> 40);
       return u * 16 < most && e < a.max_blocks ? a.tables[b * a.table_stride + e] : -1;
     };
-    uint32_t x[4][kWords], sc[4];  // pieces of one side of a chunk, on their way
-    const uint8_t *unit[2];        // the chunk's units; any place where there is none, and no scale is taken
-    int page[2];
+    uint32_t x[2][2][kWords], sc[2][2];  // pieces of K and of V of a chunk, on their way
+    const uint8_t *unit;                 // none: nothing is loaded and no scale taken
+    int page;
     uint32_t bad = 0;
-    auto find = [&](int j) {  // the units of chunk j, and the pages of the chunk after it
-      bad = 0;
+    auto find = [&](int j) {  // the unit of chunk j, and the page of the chunk after it
+      const int u = j * (kKeys / 16) + w, e = (int)(((uint64_t)u * a.upb_magic) >> 40);
+      const bool good = page >= 0 && page < a.num_blocks;
+      unit = good ? a.layer + page * a.block_stride + ((int64_t)h * a.upb + u - e * a.upb) * (9 * D) : nullptr;
+      bad = !good && u * 16 < most;
+      page = page_of(j + 1);
+    };
+    auto fetch = [&](int j, int side) {
+      const uint8_t *p = unit + side * a.kv_stride;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int u = j * (kKeys / 16) + 2 * w + i, e = (int)(((uint64_t)u * a.upb_magic) >> 40);
-        const bool good = page[i] >= 0 && page[i] < a.num_blocks;
-        unit[i] = good ? a.layer + page[i] * a.block_stride + ((int64_t)h * a.upb + u - e * a.upb) * (9 * D) : nullptr;
-        bad |= !good && u * 16 < most ? 1u << i : 0;
-        page[i] = page_of(j + 1, i);
-      }
-    };
-    auto fetch = [&](int j, int64_t side) {
+        sc[side][i] = 0;  // what no row sees may be anything: its scale counts as zero
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint8_t *p = unit[i >> 1];
-        sc[i] = 0;  // what no row sees may be anything: its scale counts as zero
-#pragma unroll
-        for (int k = 0; k < kWords; ++k) x[i][k] = 0;
-        if (p) {
-          p += side + (i & 1) * 8 * (D / 2);
+        for (int k = 0; k < kWords; ++k) x[side][i][k] = 0;
+        if (unit) {
           if constexpr (D == 128) {
-            const uint4 y = __ldg(reinterpret_cast<const uint4 *>(p + at_row));
-            x[i][0] = y.x, x[i][1] = y.y, x[i][2] = y.z, x[i][3] = y.w;
+            const uint4 y = __ldg(reinterpret_cast<const uint4 *>(p + at_row + i * 8 * (D / 2)));
+            x[side][i][0] = y.x, x[side][i][1] = y.y, x[side][i][2] = y.z, x[side][i][3] = y.w;
           } else {
-            const uint2 y = __ldg(reinterpret_cast<const uint2 *>(p + at_row));
-            x[i][0] = y.x, x[i][1] = y.y;
+            const uint2 y = __ldg(reinterpret_cast<const uint2 *>(p + at_row + i * 8 * (D / 2)));
+            x[side][i][0] = y.x, x[side][i][1] = y.y;
           }
-          p += at_scale - (i & 1) * 8 * (D / 2 - D / 16);
-          if (j * kKeys + (2 * w + (i >> 1)) * 16 + (i & 1) * 8 + tok < most)
-            sc[i] = D == 128 ? __ldg(reinterpret_cast<const uint16_t *>(p)) : __ldg(p);
+          const uint8_t *q = p + at_scale + i * 8 * (D / 16);
+          if (j * kKeys + w * 16 + i * 8 + tok < most)
+            sc[side][i] = D == 128 ? __ldg(reinterpret_cast<const uint16_t *>(q)) : __ldg(q);
         }
       }
     };
-    auto put = [&](uint32_t dst) {
+    auto put = [&](uint32_t dst, int side) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t s[2] = {__byte_perm(sc[i], 0, 0x0404) >> 1, __byte_perm(sc[i], 0, 0x1414) >> 1};
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t s[2] = {__byte_perm(sc[side][i], 0, 0x0404) >> 1, __byte_perm(sc[side][i], 0, 0x1414) >> 1};
 #pragma unroll
         for (int k = 0; k < kWords; ++k) {
           uint32_t y[4];
-          e2m1x8_to_half2(x[i][k], y);
+          e2m1x8_to_half2(x[side][i][k], y);
 #pragma unroll
           for (int m = 0; m < 4; ++m) y[m] = hmul2(y[m], s[D == 128 ? k >> 1 : 0]);
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + at_chunk[k] + i * 8 * 128), "r"(y[0]), "r"(y[1]),
@@ -1252,79 +1232,68 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
       }
     };
     const uint32_t k_at = smem_addr(sm.k[0]), v_at = smem_addr(sm.v[0]);
-    constexpr uint32_t kStage = D / 64 * ManySmem<D>::kBlock;
-    page[0] = page_of(0, 0), page[1] = page_of(0, 1);
-    if (chunks) find(0), fetch(0, 0);
+    constexpr uint32_t kStage = D / 64 * ManySmem<D>::kCols;
+    page = page_of(0);
+    if (chunks) find(0), fetch(0, 0), fetch(0, 1);
     for (int j = 0; j < chunks; ++j) {
-      const int st = j & 1;
-      if (j >= 2) patience.wait(&sm.k_empty[st], ((j >> 1) + 1) & 1);
-      put(k_at + st * kStage);
-      if (lane == 0) sm.bad[j & 3][w] = (uint8_t)bad;  // read before chunk j + 4 gets here
-      fetch(j, a.kv_stride);
+      const int st = j & (kRing - 1), parity = (j / kRing + 1) & 1;
+      if (j >= kRing) patience.wait(&sm.k_empty[st], parity);
+      put(k_at + st * kStage, 0);
+      if (lane == 0) sm.bad[j & (2 * kRing - 1)][w] = (uint8_t)bad;  // read before chunk j + 2 kRing gets here
       fence_async();
       mbar_arrive(&sm.k_full[st]);
-      if (j >= 2) patience.wait(&sm.v_empty[st], ((j >> 1) + 1) & 1);
-      put(v_at + st * kStage);
-      if (j + 1 < chunks) find(j + 1), fetch(j + 1, 0);
+      const bool more = j + 1 < chunks;
+      if (more) find(j + 1), fetch(j + 1, 0);
+      if (j >= kRing) patience.wait(&sm.v_empty[st], parity);
+      put(v_at + st * kStage, 1);
       fence_async();
       mbar_arrive(&sm.v_full[st]);
+      if (more) fetch(j + 1, 1);
     }
   } else {
-    // ---- the products ----
-    fewer_registers<kIssueRegs>();
-    if (warp == 4 * kTiles + kFillWarps && chunks) {
-      constexpr uint32_t kQK = mma_desc(kKeys, false), kPV = mma_desc(D, true);
-      constexpr uint32_t kTile = D / 64 * ManySmem<D>::kBlock / 16, kBlock16 = ManySmem<D>::kBlock / 16;  // in descriptors
-      const uint32_t one = elect_one();
-      const uint32_t mem = __shfl_sync(~0u, tmem, 0);
-      const uint64_t q_desc = smem_desc(smem_addr(sm.q), false), k_desc = smem_desc(smem_addr(sm.k), false),
-                     v_desc = smem_desc(smem_addr(sm.v), true);
-      // loops and not straight code: this warp shares its instruction cache with three busier ones
-      auto score = [&](int t, uint64_t kk) {
-        uint64_t q = q_desc + t * kTile;
-        const uint32_t d = mem + (kTiles + t) * 128;
+    // ---- the products: a warp for each tile ----
+    // In loops and not straight code: these warps share their instruction caches with three busier ones each.  The
+    // shuffles keep what addresses and trip counts come from in uniform registers, where the instructions want them.
+    constexpr uint32_t kQK = mma_desc(kKeys, false), kPV = mma_desc(D, true);
+    // of descriptors, in 16 bytes: a tile of Q and its blocks, a stage of K or V and its blocks
+    constexpr uint32_t kRows16 = ManySmem<D>::kRows / 16, kCols16 = ManySmem<D>::kCols / 16, kBlocks = D / 64;
+    const int t = __shfl_sync(~0u, warp, 0) - (4 * kTiles + kFillWarps);
+    const int n = __shfl_sync(~0u, t < tiles ? chunks : 0, 0);
+    const uint32_t one = elect_one(), o = __shfl_sync(~0u, tmem, 0) + t * 128, s = o + kTiles * 128;
+    const uint64_t q_desc = smem_desc(smem_addr(sm.q), false) + t * kBlocks * kRows16,
+                   k_desc = smem_desc(smem_addr(sm.k), false), v_desc = smem_desc(smem_addr(sm.v), true);
+    auto score = [&](int j) {  // S of chunk j
+      uint64_t q = q_desc, k = k_desc + (j & (kRing - 1)) * kBlocks * kCols16;
+      const uint32_t d = s + (j & 1) * kKeys;
 #pragma unroll 1
-        for (int k = 0; k < D / 64; ++k, q += kBlock16, kk += kBlock16) {
-          mma_ss(d, q, kk, kQK, k > 0, one);
+      for (int c = 0; c < kBlocks; ++c, q += kRows16, k += kCols16) {
+        mma_ss(d, q, k, kQK, c > 0, one);
 #pragma unroll
-          for (int i = 1; i < 4; ++i) mma_ss(d, q + i * 2, kk + i * 2, kQK, true, one);
-        }
-        mma_commit(&sm.s_full[t], one);
-      };
-      patience.wait(&sm.q_full, 0);
-      patience.wait(&sm.k_full[0], 0);
-      fence_after();
+        for (int i = 1; i < 4; ++i) mma_ss(d, q + i * 2, k + i * 2, kQK, true, one);
+      }
+      mma_commit(&sm.s_full[t][j & 1], one);
+      mma_commit(&sm.k_empty[j & (kRing - 1)], one);
+    };
+    if (n) patience.wait(&sm.q_full, 0);
 #pragma unroll 1
-      for (int t = 0; t < tiles; ++t) score(t, k_desc);
-      mma_commit(&sm.k_empty[0], one);
-#pragma unroll 1
-      for (int j = 0; j < chunks; ++j) {
-        const int st = j & 1, next = st ^ 1;
-        const bool more = j + 1 < chunks;
-        patience.wait(&sm.v_full[st], (j >> 1) & 1);
-        if (more) patience.wait(&sm.k_full[next], ((j + 1) >> 1) & 1);
-#pragma unroll 1
-        for (int t = 0; t < tiles; ++t) {
-          patience.wait(&sm.p_full[t], j & 1);
-          fence_after();
-          uint64_t v = v_desc + st * kTile;
-          const uint32_t d = mem + t * 128;
-          uint32_t p = d + kTiles * 128;
-#pragma unroll 1
-          for (int k = 0; k < kKeys / 64; ++k, v += 4 * 128, p += 4 * 8) {
-            mma_ts(d, p, v, kPV, j + k > 0, one);
+    for (int i = -2; i < n; ++i) {
+      if (i >= 0) {
+        patience.wait(&sm.v_full[i & (kRing - 1)], (i / kRing) & 1);
+        patience.wait(&sm.p_full[t][i & 1], (i >> 1) & 1);
+        fence_after();
+        const uint32_t p = s + (i & 1) * kKeys;
+        const uint64_t v = v_desc + (i & (kRing - 1)) * kBlocks * kCols16;
+        mma_ts(o, p, v, kPV, i > 0, one);
 #pragma unroll
-            for (int i = 1; i < 4; ++i) mma_ts(d, p + i * 8, v + i * 128, kPV, true, one);
-          }
-          mma_commit(&sm.o_done[t], one);
-          if (more) {
-            patience.wait(&sm.o_done[t], j & 1);  // P lies where S goes
-            fence_after();
-            score(t, k_desc + next * kTile);
-          }
-        }
-        mma_commit(&sm.v_empty[st], one);
-        if (more) mma_commit(&sm.k_empty[next], one);
+        for (int k = 1; k < kKeys / 16; ++k) mma_ts(o, p + k * 8, v + k * 128, kPV, true, one);
+        mma_commit(&sm.o_done[t], one);
+        mma_commit(&sm.v_empty[i & (kRing - 1)], one);
+      }
+      if (i + 2 < n) {  // two chunks ahead: its S goes where this chunk's P lies
+        patience.wait(&sm.k_full[(i + 2) & (kRing - 1)], ((i + 2) / kRing) & 1);
+        if (i >= 0) patience.wait(&sm.o_done[t], i & 1);
+        fence_after();
+        score(i + 2);
       }
     }
   }
