@@ -800,8 +800,8 @@ struct ManySmem {
   alignas(1024) uint8_t q[kTiles][D / 64][kRows];
   alignas(1024) uint8_t k[kRing][D / 64][kCols];
   alignas(1024) uint8_t v[kRing][D / 64][kCols];
-  uint64_t q_full, k_full[kRing], v_full[kRing], k_empty[kRing], v_empty[kRing];
-  uint64_t s_full[kTiles][2], p_full[kTiles][2], o_done[kTiles];
+  uint64_t q_full, full[kRing], empty[kRing];  // of a step: K two chunks ahead, and V
+  uint64_t s_full[kTiles][2], p_full[kTiles][2], o_done[kTiles], all_done[kTiles];
   alignas(4) uint8_t bad[2 * kRing][kFillWarps];  // of a chunk of keys, a warp's unit: its page is outside the pool
   uint32_t tmem;
 };
@@ -933,6 +933,14 @@ __device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[32]) {
 }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// A turn of tile t's warp on a quarter of the SM: a barrier of the two warps there.
+__device__ __forceinline__ void turn_wait(int t, int quarter) {
+  asm volatile("barrier.sync %0, 64;" ::"r"(1 + 4 * t + quarter) : "memory");
+}
+__device__ __forceinline__ void turn_give(int t, int quarter) {
+  asm volatile("barrier.arrive %0, 64;" ::"r"(1 + 4 * t + quarter) : "memory");
+}
+
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_constant__ AttnArgs a) {
   constexpr int R = kTiles * 128;
@@ -995,13 +1003,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
 
   if (threadIdx.x == 0) {
     mbar_init(&sm.q_full, 128 * tiles);
-    for (int i = 0; i < kRing; ++i) {
-      mbar_init(&sm.k_full[i], kFillWarps * 32), mbar_init(&sm.v_full[i], kFillWarps * 32);
-      mbar_init(&sm.k_empty[i], tiles), mbar_init(&sm.v_empty[i], tiles);
-    }
+    for (int i = 0; i < kRing; ++i) mbar_init(&sm.full[i], kFillWarps * 32), mbar_init(&sm.empty[i], tiles);
     for (int t = 0; t < kTiles; ++t) {
       for (int i = 0; i < 2; ++i) mbar_init(&sm.s_full[t][i], 1), mbar_init(&sm.p_full[t][i], 128);
-      mbar_init(&sm.o_done[t], 1);
+      mbar_init(&sm.o_done[t], 1), mbar_init(&sm.all_done[t], 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -1060,6 +1065,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
       const int end = valid ? end_of(row) : 0;
       const int lowest = __reduce_min_sync(~0u, valid ? end : INT32_MAX);
       float base = kNone, bar = -INFINITY, l[4] = {0, 0, 0, 0};
+      if (t == 1 && chunks) turn_give(0, warp & 3);
       for (int j = 0; j < chunks; ++j) {
         patience.wait(&sm.s_full[t][j & 1], (j >> 1) & 1);
         fence_after();
@@ -1105,6 +1111,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
             }
           }
         }
+        // Exponentials are what the tiles contend for: the warps of both tiles on a quarter of the SM take turns, so
+        // that one's fall into the other's waits and reads.
+        if (tiles > 1) turn_wait(t, warp & 3);
         const uint64_t mul2 = pair(mul, mul), base2 = pair(-base, -base);
         uint64_t l01 = pair(l[0], l[1]), l23 = pair(l[2], l[3]);
 #pragma unroll
@@ -1122,6 +1131,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
           }
           tmem_store16(S + 16 * c, p);
         }
+        if (tiles > 1 && !(t == 1 && j == chunks - 1)) turn_give(t ^ 1, warp & 3);
         const float2 la = unpair(l01), lb = unpair(l23);
         l[0] = la.x, l[1] = la.y, l[2] = lb.x, l[3] = lb.y;
         tmem_wait_store();
@@ -1131,10 +1141,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
 
       // O / l
       if (chunks) {
-        // the last S came after the product two chunks before it: the one between is waited for first, or a
-        // wait for the last could take the phase before that one for it
-        if (chunks > 1) patience.wait(&sm.o_done[t], (chunks - 2) & 1);
-        patience.wait(&sm.o_done[t], (chunks - 1) & 1);
+        patience.wait(&sm.all_done[t], 0);
         fence_after();
       }
       const int tok_head = h * a.group + row - i0 * a.group;
@@ -1233,22 +1240,29 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
     };
     const uint32_t k_at = smem_addr(sm.k[0]), v_at = smem_addr(sm.v[0]);
     constexpr uint32_t kStage = D / 64 * ManySmem<D>::kCols;
+    // Steps i from -2 on: K of chunk i + 2, then V of chunk i.  Their pieces are loaded a step ahead.
+    const uint8_t *units[3];  // of the chunks i, i + 1, i + 2
     page = page_of(0);
-    if (chunks) find(0), fetch(0, 0), fetch(0, 1);
-    for (int j = 0; j < chunks; ++j) {
-      const int st = j & (kRing - 1), parity = (j / kRing + 1) & 1;
-      if (j >= kRing) patience.wait(&sm.k_empty[st], parity);
-      put(k_at + st * kStage, 0);
-      if (lane == 0) sm.bad[j & (2 * kRing - 1)][w] = (uint8_t)bad;  // read before chunk j + 2 kRing gets here
+    if (chunks) find(0), fetch(0, 0);
+#pragma unroll 1
+    for (int i = chunks ? -2 : 0; i < chunks; ++i) {
+      const int slot = (i + 2) & (kRing - 1);
+      if (i + 2 >= kRing) patience.wait(&sm.empty[slot], ((i + 2) / kRing + 1) & 1);
+      units[0] = units[1], units[1] = units[2], units[2] = unit;
+      if (i + 2 < chunks) {
+        put(k_at + slot * kStage, 0);
+        if (lane == 0) sm.bad[(i + 2) & (2 * kRing - 1)][w] = (uint8_t)bad;  // read before the chunk 2 kRing on gets here
+        if (i + 3 < chunks) find(i + 3), fetch(i + 3, 0);
+      }
+      if (i >= 0) put(v_at + (i & (kRing - 1)) * kStage, 1);
       fence_async();
-      mbar_arrive(&sm.k_full[st]);
-      const bool more = j + 1 < chunks;
-      if (more) find(j + 1), fetch(j + 1, 0);
-      if (j >= kRing) patience.wait(&sm.v_empty[st], parity);
-      put(v_at + st * kStage, 1);
-      fence_async();
-      mbar_arrive(&sm.v_full[st]);
-      if (more) fetch(j + 1, 1);
+      mbar_arrive(&sm.full[slot]);
+      if (i + 1 >= 0 && i + 1 < chunks) {
+        const uint8_t *keep = unit;
+        unit = units[1];
+        fetch(i + 1, 1);
+        unit = keep;
+      }
     }
   } else {
     // ---- the products: a warp for each tile ----
@@ -1258,7 +1272,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
     // of descriptors, in 16 bytes: a tile of Q and its blocks, a stage of K or V and its blocks
     constexpr uint32_t kRows16 = ManySmem<D>::kRows / 16, kCols16 = ManySmem<D>::kCols / 16, kBlocks = D / 64;
     const int t = __shfl_sync(~0u, warp, 0) - (4 * kTiles + kFillWarps);
-    const int n = __shfl_sync(~0u, t < tiles ? chunks : 0, 0);
+    const int n = __shfl_sync(~0u, t < tiles ? chunks : 0, 0);  // none: no step at all
     const uint32_t one = elect_one(), o = __shfl_sync(~0u, tmem, 0) + t * 128, s = o + kTiles * 128;
     const uint64_t q_desc = smem_desc(smem_addr(sm.q), false) + t * kBlocks * kRows16,
                    k_desc = smem_desc(smem_addr(sm.k), false), v_desc = smem_desc(smem_addr(sm.v), true);
@@ -1272,13 +1286,12 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
         for (int i = 1; i < 4; ++i) mma_ss(d, q + i * 2, k + i * 2, kQK, true, one);
       }
       mma_commit(&sm.s_full[t][j & 1], one);
-      mma_commit(&sm.k_empty[j & (kRing - 1)], one);
     };
-    if (n) patience.wait(&sm.q_full, 0);
+    auto filled = [&](int i) { patience.wait(&sm.full[(i + 2) & (kRing - 1)], ((i + 2) / kRing) & 1); };
+    if (n) patience.wait(&sm.q_full, 0), filled(-2);
 #pragma unroll 1
-    for (int i = -2; i < n; ++i) {
+    for (int i = n ? -2 : 0; i < n; ++i) {
       if (i >= 0) {
-        patience.wait(&sm.v_full[i & (kRing - 1)], (i / kRing) & 1);
         patience.wait(&sm.p_full[t][i & 1], (i >> 1) & 1);
         fence_after();
         const uint32_t p = s + (i & 1) * kKeys;
@@ -1287,15 +1300,16 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
 #pragma unroll
         for (int k = 1; k < kKeys / 16; ++k) mma_ts(o, p + k * 8, v + k * 128, kPV, true, one);
         mma_commit(&sm.o_done[t], one);
-        mma_commit(&sm.v_empty[i & (kRing - 1)], one);
       }
       if (i + 2 < n) {  // two chunks ahead: its S goes where this chunk's P lies
-        patience.wait(&sm.k_full[(i + 2) & (kRing - 1)], ((i + 2) / kRing) & 1);
         if (i >= 0) patience.wait(&sm.o_done[t], i & 1);
         fence_after();
         score(i + 2);
       }
+      mma_commit(&sm.empty[(i + 2) & (kRing - 1)], one);
+      if (i + 1 < n) filled(i + 1);
     }
+    if (n) mma_commit(&sm.all_done[t], one);
   }
 
   __syncwarp();
