@@ -786,13 +786,15 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
 //    thread.  The base moves only when a score passes it by kMove, as in the
 //    kernel above: then the weights are taken again and O is scaled in place.
 // Two tiles of rows alternate: while one is in softmax the tensor core works
-// on the other, and K and V are converted once for both.  A tile has two
-// buffers for S, so that the next scores are there when a softmax ends.
-// Tensor memory (512 columns): O of both tiles, two S of both; P lies over S.
+// on the other, and K and V are converted once for both.
+// Tensor memory (512 columns): O of both tiles, S of both; P lies over S.
 
-constexpr int kTiles = 2, kKeys = 64, kRing = 4;
+constexpr int kTiles = 2, kKeys = 128, kRing = 2;
 constexpr int kFillWarps = 4;
-constexpr int kManyThreads = (4 * kTiles + kFillWarps + kTiles) * 32;
+constexpr int kManyThreads = (4 * kTiles + kFillWarps + 4) * 32;  // of the last four, one for each tile issues products
+// Registers of a thread of each kind; launched with 128, so the sum over all may be 512 * 128.
+constexpr int kRowRegs = 184, kFillRegs = 96, kIssueRegs = 40;
+static_assert(kRowRegs * 128 * kTiles + kFillRegs * 128 + kIssueRegs * 128 <= kManyThreads * 128, "register split");
 
 template <int D>
 struct ManySmem {
@@ -800,9 +802,9 @@ struct ManySmem {
   alignas(1024) uint8_t q[kTiles][D / 64][kRows];
   alignas(1024) uint8_t k[kRing][D / 64][kCols];
   alignas(1024) uint8_t v[kRing][D / 64][kCols];
-  uint64_t q_full, full[kRing], empty[kRing];  // of a step: K two chunks ahead, and V
-  uint64_t s_full[kTiles][2], p_full[kTiles][2], o_done[kTiles], all_done[kTiles];
-  alignas(4) uint8_t bad[2 * kRing][kFillWarps];  // of a chunk of keys, a warp's unit: its page is outside the pool
+  uint64_t q_full, full[kRing], empty[kRing];  // of a step: K a chunk ahead, and V
+  uint64_t s_full[kTiles], p_full[kTiles][2], o_done[kTiles], all_done[kTiles];
+  alignas(4) uint8_t bad[2 * kRing][kFillWarps];  // of a chunk of keys, a warp's two units: whose page is outside the pool
   uint32_t tmem;
 };
 
@@ -898,6 +900,15 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 #define FKV_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
 #define FKV_W8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
 // 16 or 32 columns of the warp's 32 lanes.
@@ -1005,7 +1016,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
     mbar_init(&sm.q_full, 128 * tiles);
     for (int i = 0; i < kRing; ++i) mbar_init(&sm.full[i], kFillWarps * 32), mbar_init(&sm.empty[i], tiles);
     for (int t = 0; t < kTiles; ++t) {
-      for (int i = 0; i < 2; ++i) mbar_init(&sm.s_full[t][i], 1), mbar_init(&sm.p_full[t][i], 128);
+      mbar_init(&sm.s_full[t], 1);
+      for (int i = 0; i < 2; ++i) mbar_init(&sm.p_full[t][i], 128);
       mbar_init(&sm.o_done[t], 1), mbar_init(&sm.all_done[t], 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -1019,11 +1031,12 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
   fence_after();
   const uint32_t tmem = sm.tmem;
   auto o_at = [&](int t) { return tmem + t * 128; };
-  auto s_at = [&](int t, int i) { return tmem + (kTiles + t) * 128 + i * kKeys; };
+  auto s_at = [&](int t) { return tmem + (kTiles + t) * 128; };
   Patience patience;
 
   if (warp < 4 * kTiles) {
     // ---- a thread for each row ----
+    more_registers<kRowRegs>();
     const int t = warp >> 2, r = (warp & 3) * 32 + lane, row = row0 + t * 128 + r;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // the warp's 32 lanes of tensor memory
     if (t < tiles) {
@@ -1067,25 +1080,32 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
       float base = kNone, bar = -INFINITY, l[4] = {0, 0, 0, 0};
       if (t == 1 && chunks) turn_give(0, warp & 3);
       for (int j = 0; j < chunks; ++j) {
-        patience.wait(&sm.s_full[t][j & 1], (j >> 1) & 1);
+        patience.wait(&sm.s_full[t], j & 1);
         fence_after();
-        const uint32_t S = s_at(t, j & 1) + lanes;
-        uint32_t x[2][32];
+        const uint32_t S = s_at(t) + lanes;
+        uint32_t x[4][32];
         tmem_load32(x[0], S), tmem_load32(x[1], S + 32);
         const uint32_t bad = *(volatile uint32_t *)sm.bad[j & (2 * kRing - 1)];
         tmem_wait_load(x[0]), tmem_wait_load(x[1]);
-        if ((j + 1) * kKeys > lowest || bad) {  // only what the row sees
+        tmem_load32(x[2], S + 64), tmem_load32(x[3], S + 96);
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        auto half = [&](int c0) {  // the largest of 64 columns
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
+          for (int c = c0; c < c0 + 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[c][i]));
+        };
+        if ((j + 1) * kKeys > lowest || bad) {  // only what the row sees
+          tmem_wait_load(x[2]), tmem_wait_load(x[3]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (j * kKeys + 32 * c + i >= end || ((bad >> (8 * (2 * c + i / 16))) & 1)) x[c][i] = 0xFF800000u;
+              if (j * kKeys + 32 * c + i >= end || ((bad >> (8 * c + i / 16)) & 1)) x[c][i] = 0xFF800000u;
         }
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[c][i]));
+        half(0);
+        tmem_wait_load(x[2]), tmem_wait_load(x[3]);
+        half(2);
         const float most_here = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         if (__any_sync(~0u, most_here > bar)) {  // rare after the first chunks
           float f = 1.0f;
@@ -1117,7 +1137,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
         const uint64_t mul2 = pair(mul, mul), base2 = pair(-base, -base);
         uint64_t l01 = pair(l[0], l[1]), l23 = pair(l[2], l[3]);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < 4; ++c) {
           uint32_t p[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -1130,13 +1150,18 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
             p[i] = pack_half2(u, v);
           }
           tmem_store16(S + 16 * c, p);
+          if (c == 1) {  // the product with the first half of the keys starts here
+            tmem_wait_store();
+            fence_before();
+            mbar_arrive(&sm.p_full[t][0]);
+          }
         }
         if (tiles > 1 && !(t == 1 && j == chunks - 1)) turn_give(t ^ 1, warp & 3);
         const float2 la = unpair(l01), lb = unpair(l23);
         l[0] = la.x, l[1] = la.y, l[2] = lb.x, l[3] = lb.y;
         tmem_wait_store();
         fence_before();
-        mbar_arrive(&sm.p_full[t][j & 1]);
+        mbar_arrive(&sm.p_full[t][1]);
       }
 
       // O / l
@@ -1175,7 +1200,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
     }
   } else if (warp < 4 * kTiles + kFillWarps) {
     // ---- K and V into shared memory ----
-    // Warp w brings unit w of a chunk, 8 tokens at a time, a quarter of a row a lane: 8 lanes that store together
+    fewer_registers<kFillRegs>();
+    // Warp w brings units 2 w and 2 w + 1 of a chunk, 8 tokens at a time, a quarter of a row a lane: 8 lanes that store together
     // have 8 rows, so the swizzle spreads them over all banks.
     const int w = warp - 4 * kTiles, tok = lane & 7, quarter = lane >> 3;
     constexpr int kWords = D / 32;  // of a lane's piece, 8 channels each
@@ -1184,47 +1210,51 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
 #pragma unroll
     for (int k = 0; k < kWords; ++k) {
       const int c = quarter * kWords + k;
-      at_chunk[k] = (c >> 3) * ManySmem<D>::kCols + w * 16 * 128 + tok * 128 + ((c & 7) ^ tok) * 16;
+      at_chunk[k] = (c >> 3) * ManySmem<D>::kCols + w * 32 * 128 + tok * 128 + ((c & 7) ^ tok) * 16;
     }
-    auto page_of = [&](int j) {
-      const int u = j * (kKeys / 16) + w, e = (int)(((uint64_t)u * a.upb_magic) >> 40);
+    auto page_of = [&](int j, int i) {
+      const int u = j * (kKeys / 16) + 2 * w + i, e = (int)(((uint64_t)u * a.upb_magic) >> 40);
       return u * 16 < most && e < a.max_blocks ? a.tables[b * a.table_stride + e] : -1;
     };
-    uint32_t x[2][2][kWords], sc[2][2];  // pieces of K and of V of a chunk, on their way
-    const uint8_t *unit;                 // none: nothing is loaded and no scale taken
-    int page;
+    uint32_t x[2][4][kWords], sc[2][4];  // pieces of K and of V of a chunk, on their way
+    int64_t unit[2], last[2];            // units of a chunk, and of the one before, from the layer on; none: -1
+    int page[2];
     uint32_t bad = 0;
-    auto find = [&](int j) {  // the unit of chunk j, and the page of the chunk after it
-      const int u = j * (kKeys / 16) + w, e = (int)(((uint64_t)u * a.upb_magic) >> 40);
-      const bool good = page >= 0 && page < a.num_blocks;
-      unit = good ? a.layer + page * a.block_stride + ((int64_t)h * a.upb + u - e * a.upb) * (9 * D) : nullptr;
-      bad = !good && u * 16 < most;
-      page = page_of(j + 1);
-    };
-    auto fetch = [&](int j, int side) {
-      const uint8_t *p = unit + side * a.kv_stride;
+    auto find = [&](int j) {  // the units of chunk j, and the pages of the chunk after it
+      bad = 0;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
+        const int u = j * (kKeys / 16) + 2 * w + i, e = (int)(((uint64_t)u * a.upb_magic) >> 40);
+        const bool good = page[i] >= 0 && page[i] < a.num_blocks;
+        unit[i] = good ? page[i] * a.block_stride + ((int64_t)h * a.upb + u - e * a.upb) * (9 * D) : -1;
+        bad |= !good && u * 16 < most ? 1u << i : 0;
+        page[i] = page_of(j + 1, i);
+      }
+    };
+    auto fetch = [&](int j, int side, const int64_t(&from)[2]) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
         sc[side][i] = 0;  // what no row sees may be anything: its scale counts as zero
 #pragma unroll
         for (int k = 0; k < kWords; ++k) x[side][i][k] = 0;
-        if (unit) {
+        if (from[i >> 1] >= 0) {
+          const uint8_t *p = a.layer + from[i >> 1] + side * a.kv_stride;
           if constexpr (D == 128) {
-            const uint4 y = __ldg(reinterpret_cast<const uint4 *>(p + at_row + i * 8 * (D / 2)));
+            const uint4 y = __ldg(reinterpret_cast<const uint4 *>(p + at_row + (i & 1) * 8 * (D / 2)));
             x[side][i][0] = y.x, x[side][i][1] = y.y, x[side][i][2] = y.z, x[side][i][3] = y.w;
           } else {
-            const uint2 y = __ldg(reinterpret_cast<const uint2 *>(p + at_row + i * 8 * (D / 2)));
+            const uint2 y = __ldg(reinterpret_cast<const uint2 *>(p + at_row + (i & 1) * 8 * (D / 2)));
             x[side][i][0] = y.x, x[side][i][1] = y.y;
           }
-          const uint8_t *q = p + at_scale + i * 8 * (D / 16);
-          if (j * kKeys + w * 16 + i * 8 + tok < most)
+          const uint8_t *q = p + at_scale + (i & 1) * 8 * (D / 16);
+          if (j * kKeys + w * 32 + i * 8 + tok < most)
             sc[side][i] = D == 128 ? __ldg(reinterpret_cast<const uint16_t *>(q)) : __ldg(q);
         }
       }
     };
     auto put = [&](uint32_t dst, int side) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < 4; ++i) {
         const uint32_t s[2] = {__byte_perm(sc[side][i], 0, 0x0404) >> 1, __byte_perm(sc[side][i], 0, 0x1414) >> 1};
 #pragma unroll
         for (int k = 0; k < kWords; ++k) {
@@ -1240,32 +1270,27 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
     };
     const uint32_t k_at = smem_addr(sm.k[0]), v_at = smem_addr(sm.v[0]);
     constexpr uint32_t kStage = D / 64 * ManySmem<D>::kCols;
-    // Steps i from -2 on: K of chunk i + 2, then V of chunk i.  Their pieces are loaded a step ahead.
-    const uint8_t *units[3];  // of the chunks i, i + 1, i + 2
-    page = page_of(0);
-    if (chunks) find(0), fetch(0, 0);
+    // Steps i from -1 on: K of chunk i + 1, then V of chunk i.  Their pieces are loaded a step ahead.
+    page[0] = page_of(0, 0), page[1] = page_of(0, 1);
+    if (chunks) find(0), fetch(0, 0, unit);
 #pragma unroll 1
-    for (int i = chunks ? -2 : 0; i < chunks; ++i) {
-      const int slot = (i + 2) & (kRing - 1);
-      if (i + 2 >= kRing) patience.wait(&sm.empty[slot], ((i + 2) / kRing + 1) & 1);
-      units[0] = units[1], units[1] = units[2], units[2] = unit;
-      if (i + 2 < chunks) {
+    for (int i = chunks ? -1 : 0; i < chunks; ++i) {
+      const int slot = (i + 1) & (kRing - 1);
+      if (i + 1 >= kRing) patience.wait(&sm.empty[slot], ((i + 1) / kRing + 1) & 1);
+      last[0] = unit[0], last[1] = unit[1];  // of chunk i + 1, whose V comes next
+      if (i + 1 < chunks) {
         put(k_at + slot * kStage, 0);
-        if (lane == 0) sm.bad[(i + 2) & (2 * kRing - 1)][w] = (uint8_t)bad;  // read before the chunk 2 kRing on gets here
-        if (i + 3 < chunks) find(i + 3), fetch(i + 3, 0);
+        if (lane == 0) sm.bad[(i + 1) & (2 * kRing - 1)][w] = (uint8_t)bad;  // read before the chunk 2 kRing on gets here
+        if (i + 2 < chunks) find(i + 2), fetch(i + 2, 0, unit);
       }
       if (i >= 0) put(v_at + (i & (kRing - 1)) * kStage, 1);
       fence_async();
       mbar_arrive(&sm.full[slot]);
-      if (i + 1 >= 0 && i + 1 < chunks) {
-        const uint8_t *keep = unit;
-        unit = units[1];
-        fetch(i + 1, 1);
-        unit = keep;
-      }
+      if (i + 1 < chunks) fetch(i + 1, 1, last);
     }
   } else {
     // ---- the products: a warp for each tile ----
+    fewer_registers<kIssueRegs>();
     // In loops and not straight code: these warps share their instruction caches with three busier ones each.  The
     // shuffles keep what addresses and trip counts come from in uniform registers, where the instructions want them.
     constexpr uint32_t kQK = mma_desc(kKeys, false), kPV = mma_desc(D, true);
@@ -1278,35 +1303,37 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
                    k_desc = smem_desc(smem_addr(sm.k), false), v_desc = smem_desc(smem_addr(sm.v), true);
     auto score = [&](int j) {  // S of chunk j
       uint64_t q = q_desc, k = k_desc + (j & (kRing - 1)) * kBlocks * kCols16;
-      const uint32_t d = s + (j & 1) * kKeys;
 #pragma unroll 1
       for (int c = 0; c < kBlocks; ++c, q += kRows16, k += kCols16) {
-        mma_ss(d, q, k, kQK, c > 0, one);
+        mma_ss(s, q, k, kQK, c > 0, one);
 #pragma unroll
-        for (int i = 1; i < 4; ++i) mma_ss(d, q + i * 2, k + i * 2, kQK, true, one);
+        for (int i = 1; i < 4; ++i) mma_ss(s, q + i * 2, k + i * 2, kQK, true, one);
       }
-      mma_commit(&sm.s_full[t][j & 1], one);
+      mma_commit(&sm.s_full[t], one);
     };
-    auto filled = [&](int i) { patience.wait(&sm.full[(i + 2) & (kRing - 1)], ((i + 2) / kRing) & 1); };
-    if (n) patience.wait(&sm.q_full, 0), filled(-2);
+    auto filled = [&](int i) { patience.wait(&sm.full[(i + 1) & (kRing - 1)], ((i + 1) / kRing) & 1); };
+    if (n) patience.wait(&sm.q_full, 0), filled(-1);
 #pragma unroll 1
-    for (int i = n ? -2 : 0; i < n; ++i) {
+    for (int i = n ? -1 : 0; i < n; ++i) {
       if (i >= 0) {
-        patience.wait(&sm.p_full[t][i & 1], (i >> 1) & 1);
-        fence_after();
-        const uint32_t p = s + (i & 1) * kKeys;
-        const uint64_t v = v_desc + (i & (kRing - 1)) * kBlocks * kCols16;
-        mma_ts(o, p, v, kPV, i > 0, one);
+        uint32_t p = s;
+        uint64_t v = v_desc + (i & (kRing - 1)) * kBlocks * kCols16;
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half, p += 32, v += kKeys / 2 * 8) {
+          patience.wait(&sm.p_full[t][half], i & 1);
+          fence_after();
+          mma_ts(o, p, v, kPV, i + half > 0, one);
 #pragma unroll
-        for (int k = 1; k < kKeys / 16; ++k) mma_ts(o, p + k * 8, v + k * 128, kPV, true, one);
+          for (int k = 1; k < kKeys / 32; ++k) mma_ts(o, p + k * 8, v + k * 128, kPV, true, one);
+        }
         mma_commit(&sm.o_done[t], one);
       }
-      if (i + 2 < n) {  // two chunks ahead: its S goes where this chunk's P lies
+      if (i + 1 < n) {  // its S goes where this chunk's P lies
         if (i >= 0) patience.wait(&sm.o_done[t], i & 1);
         fence_after();
-        score(i + 2);
+        score(i + 1);
       }
-      mma_commit(&sm.empty[(i + 2) & (kRing - 1)], one);
+      mma_commit(&sm.empty[(i + 1) & (kRing - 1)], one);
       if (i + 1 < n) filled(i + 1);
     }
     if (n) mma_commit(&sm.all_done[t], one);
