@@ -24,7 +24,8 @@ struct AttnArgs {
   int64_t num_blocks, kv_stride, block_stride;
   int tokens_per_block, kv_heads, group;
   int upb;             // units of a block
-  uint64_t upb_magic;  // u / upb = (u * upb_magic) >> 40 for u < 2^28, upb <= 2^12
+  // x / upb = (x * upb_magic) >> 40, x / group likewise, for x < 2^28 and divisors up to 2^12
+  uint64_t upb_magic, group_magic;
   const uint8_t *q;
   int64_t q_token_stride, q_head_stride;  // bytes
   uint8_t *out;
@@ -52,7 +53,7 @@ template <bool BF16, int N>
 __device__ __forceinline__ void store_row(const AttnArgs &a, int64_t first, int h, int row, int nrows, int c,
                                           const float (&v)[N], float m, float l) {
   if (row >= nrows) return;
-  const int i = row / a.group, qh = h * a.group + row - i * a.group;
+  const int i = (int)(((uint64_t)row * a.group_magic) >> 40), qh = h * a.group + row - i * a.group;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   uint32_t w[N / 2];
 #pragma unroll
@@ -131,6 +132,8 @@ struct Item {     // what a warp needs of one sequence
   int blocks;     // blocks of R (token, head) rows
   int units;      // units to pass, at least one where there are rows
 };
+
+__device__ __forceinline__ int token_of(const AttnArgs &a, int row) { return (int)(((uint64_t)row * a.group_magic) >> 40); }
 
 template <int R>
 __device__ __forceinline__ Item item_of(const AttnArgs &a, int b) {
@@ -489,7 +492,7 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) x[i] = 0;
         if (r < nrows) {
-          const int i0 = r / a.group;
+          const int i0 = token_of(a, r);
           const uint8_t *p = a.q + (cur.it.first + i0) * a.q_token_stride +
                              (h * a.group + r - i0 * a.group) * a.q_head_stride + t * (D / 2);
 #pragma unroll
@@ -523,7 +526,7 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
           int e = 0;
           if (rr < nrows) {
             e = cur.it.len;
-            if (a.causal) e = max(min(e, cur.it.len_q - cur.it.rows + rr / a.group + 1), 0);
+            if (a.causal) e = max(min(e, cur.it.len_q - cur.it.rows + token_of(a, rr) + 1), 0);
             lowest = min(lowest, e);
           }
           end[n][j] = e;
@@ -793,7 +796,7 @@ constexpr int kTiles = 2, kKeys = 128, kRing = 2;
 constexpr int kFillWarps = 4;
 constexpr int kManyThreads = (4 * kTiles + kFillWarps + 4) * 32;  // of the last four, one for each tile issues products
 // Registers of a thread of each kind; launched with 128, so the sum over all may be 512 * 128.
-constexpr int kRowRegs = 184, kFillRegs = 96, kIssueRegs = 40;
+constexpr int kRowRegs = 192, kFillRegs = 96, kIssueRegs = 32;
 static_assert(kRowRegs * 128 * kTiles + kFillRegs * 128 + kIssueRegs * 128 <= kManyThreads * 128, "register split");
 
 template <int D>
@@ -803,7 +806,7 @@ struct ManySmem {
   alignas(1024) uint8_t k[kRing][D / 64][kCols];
   alignas(1024) uint8_t v[kRing][D / 64][kCols];
   uint64_t q_full, full[kRing], empty[kRing];  // of a step: K a chunk ahead, and V
-  uint64_t s_full[kTiles], p_full[kTiles][2], o_done[kTiles], all_done[kTiles];
+  uint64_t s_full[kTiles], o_done[kTiles], all_done[kTiles];
   alignas(4) uint8_t bad[2 * kRing][kFillWarps];  // of a chunk of keys, a warp's two units: whose page is outside the pool
   uint32_t tmem;
 };
@@ -911,12 +914,21 @@ __device__ __forceinline__ void fewer_registers() {
 
 #define FKV_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
 #define FKV_W8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
-// 16 or 32 columns of the warp's 32 lanes.
-__device__ __forceinline__ void tmem_load16(uint32_t (&r)[16], uint32_t at) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-               : FKV_R8(r, 0), FKV_R8(r, 8)
-               : "r"(at)
+// What was loaded may be used from here on: the registers go through the wait.
+#define FKV_RW8(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7])
+__device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : FKV_RW8(r, 0), FKV_RW8(r, 8), FKV_RW8(r, 16), FKV_RW8(r, 24)
+               :
                : "memory");
+}
+// 8, 16 or 32 columns of the warp's 32 lanes.
+__device__ __forceinline__ void tmem_load8(uint32_t (&r)[8], uint32_t at) {  // and waits
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : FKV_R8(r, 0) : "r"(at) : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : FKV_RW8(r, 0) : : "memory");
+}
+__device__ __forceinline__ void tmem_store8(uint32_t at, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), FKV_W8(r, 0) : "memory");
 }
 __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&r)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
@@ -931,25 +943,19 @@ __device__ __forceinline__ void tmem_load32(uint32_t (&r)[32], uint32_t at) {
       : "r"(at)
       : "memory");
 }
-// What was loaded may be used from here on: the registers go through the wait.
-#define FKV_RW8(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7])
-__device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" : FKV_RW8(r, 0), FKV_RW8(r, 8) : : "memory");
-}
-__device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : FKV_RW8(r, 0), FKV_RW8(r, 8), FKV_RW8(r, 16), FKV_RW8(r, 24)
-               :
-               : "memory");
-}
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// A turn of tile t's warp on a quarter of the SM: a barrier of the two warps there.
-__device__ __forceinline__ void turn_wait(int t, int quarter) {
-  asm volatile("barrier.sync %0, 64;" ::"r"(1 + 4 * t + quarter) : "memory");
+// Barriers between warps of the CTA by number: turns of a tile's warp on a
+// quarter of the SM (the two warps there), halves of P (a tile's four warps and
+// the one that issues its products).  These and not barriers in shared memory
+// where it can be: an access to one of those waits in the same queue as the
+// exponentials, some hundred cycles when it is full.
+constexpr int kTurn = 1, kPReady = kTurn + 4 * kTiles;
+__device__ __forceinline__ void named_wait(int id, int threads) {
+  asm volatile("barrier.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
-__device__ __forceinline__ void turn_give(int t, int quarter) {
-  asm volatile("barrier.arrive %0, 64;" ::"r"(1 + 4 * t + quarter) : "memory");
+__device__ __forceinline__ void named_arrive(int id, int threads) {
+  asm volatile("barrier.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
 template <int D, bool BF16>
@@ -1006,7 +1012,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
   const int tiles = nrows - row0 > 128 ? 2 : 1;
   auto end_of = [&](int row) {  // the keys that a row sees
     int e = it.len;
-    if (a.causal) e = max(min(e, it.len_q - it.rows + row / a.group + 1), 0);
+    if (a.causal) e = max(min(e, it.len_q - it.rows + token_of(a, row) + 1), 0);
     return e;
   };
   const int most = end_of(min(nrows - 1, row0 + R - 1));
@@ -1017,7 +1023,6 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
     for (int i = 0; i < kRing; ++i) mbar_init(&sm.full[i], kFillWarps * 32), mbar_init(&sm.empty[i], tiles);
     for (int t = 0; t < kTiles; ++t) {
       mbar_init(&sm.s_full[t], 1);
-      for (int i = 0; i < 2; ++i) mbar_init(&sm.p_full[t][i], 128);
       mbar_init(&sm.o_done[t], 1), mbar_init(&sm.all_done[t], 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -1041,36 +1046,40 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // the warp's 32 lanes of tensor memory
     if (t < tiles) {
       const bool valid = row < nrows;
-      const int i0 = valid ? row / a.group : 0;
+      // The warp's 32 rows come in together, kAtOnce at a time with kLanes lanes for each, so that whole rows are read.
+      constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;
+      const int part = lane % kLanes, among = lane / kLanes;
+      const uint32_t at_q = smem_addr(&sm.q[t][part / 8][0]) + ((warp & 3) * 32 + among) * 128;
+      auto place = [&](int i) { return at_q + i * 128 + ((part % 8) ^ ((i + among) & 7)) * 16; };  // of row i + among
+#pragma unroll 4
+      for (int i = 0; i < 32; i += kAtOnce) {
+        const int rr = min(row0 + t * 128 + (warp & 3) * 32 + i + among, nrows - 1), tok = token_of(a, rr);
+        copy16(place(i), a.q + (it.first + tok) * a.q_token_stride + (h * a.group + rr - tok * a.group) * a.q_head_stride + part * 16);
+      }
+      copies_commit();
+      copies_wait<0>();
       float mul = 0;
-      {
-        const uint8_t *p = a.q + (it.first + i0) * a.q_token_stride + (h * a.group + row - i0 * a.group) * a.q_head_stride;
+#pragma unroll 2
+      for (int i = 0; i < 32; i += kAtOnce) {  // a lane converts the piece that it brought
+        uint32_t w[4];
+        load_shared(w, place(i));
         float amax = 0;
-        uint4 x[D / 8];
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) x[i] = valid ? reinterpret_cast<const uint4 *>(p)[i] : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 f = pair_to_float2<BF16>(w[j]);
-            amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
-          }
+        for (int k = 0; k < 4; ++k) {
+          const float2 f = pair_to_float2<BF16>(w[k]);
+          amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
         }
+#pragma unroll
+        for (int k = 1; k < kLanes; k <<= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, k));
         const float f = row_factor(amax), fs = a.scale < 0.0f ? -f : f;
-        mul = fmaxf(fabsf(a.scale) * 1.4426950408889634f * (1.0f / f), 1e-37f);
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-          uint32_t y[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 z = pair_to_float2<BF16>(w[j]);
-            y[j] = pack_half2(z.x * fs, z.y * fs);
-          }
-          *reinterpret_cast<uint4 *>(&sm.q[t][i / 8][r * 128 + ((i % 8) ^ (r & 7)) * 16]) = make_uint4(y[0], y[1], y[2], y[3]);
+        for (int k = 0; k < 4; ++k) {
+          const float2 z = pair_to_float2<BF16>(w[k]);
+          w[k] = pack_half2(z.x * fs, z.y * fs);
         }
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place(i)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+        const float theirs = __shfl_sync(~0u, f, lane % kAtOnce * kLanes);
+        if (lane / kAtOnce == i / kAtOnce) mul = fmaxf(fabsf(a.scale) * 1.4426950408889634f * (1.0f / theirs), 1e-37f);
       }
       fence_async();
       mbar_arrive(&sm.q_full);
@@ -1078,7 +1087,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
       const int end = valid ? end_of(row) : 0;
       const int lowest = __reduce_min_sync(~0u, valid ? end : INT32_MAX);
       float base = kNone, bar = -INFINITY, l[4] = {0, 0, 0, 0};
-      if (t == 1 && chunks) turn_give(0, warp & 3);
+      if (t == 1 && chunks) named_arrive(kTurn + (warp & 3), 64);
       for (int j = 0; j < chunks; ++j) {
         patience.wait(&sm.s_full[t], j & 1);
         fence_after();
@@ -1088,32 +1097,50 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
         const uint32_t bad = *(volatile uint32_t *)sm.bad[j & (2 * kRing - 1)];
         tmem_wait_load(x[0]), tmem_wait_load(x[1]);
         tmem_load32(x[2], S + 64), tmem_load32(x[3], S + 96);
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        auto half = [&](int c0) {  // the largest of 64 columns
-#pragma unroll
-          for (int c = c0; c < c0 + 2; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[c][i]));
-        };
+        tmem_wait_load(x[2]), tmem_wait_load(x[3]);
         if ((j + 1) * kKeys > lowest || bad) {  // only what the row sees
-          tmem_wait_load(x[2]), tmem_wait_load(x[3]);
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (j * kKeys + 32 * c + i >= end || ((bad >> (8 * c + i / 16)) & 1)) x[c][i] = 0xFF800000u;
         }
-        half(0);
-        tmem_wait_load(x[2]), tmem_wait_load(x[3]);
-        half(2);
-        const float most_here = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-        if (__any_sync(~0u, most_here > bar)) {  // rare after the first chunks
+        // Exponentials are what the tiles contend for: the warps of both tiles on a quarter of the SM take turns, so
+        // that one's fall into the other's waits and reads.
+        if (tiles > 1) named_wait(kTurn + 4 * t + (warp & 3), 64);
+        uint64_t mul2 = pair(mul, mul), base2 = pair(-base, -base), part01, part23;
+        auto weights = [&](int c, uint32_t(&p)[16]) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 y = unpair(fma2(pair(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])), mul2, base2));
+            const float u = exp2_fast(y.x), v = exp2_fast(y.y);
+            if (i & 1)
+              part23 = add2(part23, pair(u, v));
+            else
+              part01 = add2(part01, pair(u, v));
+            p[i] = pack_half2(u, v);
+          }
+        };
+        uint32_t p[2][16];
+        // The first half of the weights is taken with the base as it is while the row's largest score is found.
+#pragma unroll 1
+        for (bool again = false;; again = true) {
+          part01 = part23 = 0;
+          weights(0, p[0]), weights(1, p[1]);
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[c][i]));
+          const float most_here = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+          if (again || !__any_sync(~0u, most_here > bar)) break;  // rare after the first chunks
           float f = 1.0f;
           if (most_here > bar) {  // other rows stay: a row does not depend on its neighbours
             const float to = most_here * mul - kLift;
             f = exp2_fast(base - to);
             base = to;
             bar = __fdividef(to + kMove, mul);
+            base2 = pair(-base, -base);
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) l[i] *= f;
@@ -1121,47 +1148,27 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
             patience.wait(&sm.o_done[t], (j - 1) & 1);
             fence_after();
 #pragma unroll 1
-            for (int c = 0; c < D / 16; ++c) {
-              uint32_t y[16];
-              tmem_load16(y, o_at(t) + lanes + 16 * c);
-              tmem_wait_load(y);
+            for (int c = 0; c < D / 8; ++c) {
+              uint32_t y[8];
+              tmem_load8(y, o_at(t) + lanes + 8 * c);
 #pragma unroll
-              for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
-              tmem_store16(o_at(t) + lanes + 16 * c, y);
+              for (int i = 0; i < 8; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
+              tmem_store8(o_at(t) + lanes + 8 * c, y);
             }
           }
         }
-        // Exponentials are what the tiles contend for: the warps of both tiles on a quarter of the SM take turns, so
-        // that one's fall into the other's waits and reads.
-        if (tiles > 1) turn_wait(t, warp & 3);
-        const uint64_t mul2 = pair(mul, mul), base2 = pair(-base, -base);
-        uint64_t l01 = pair(l[0], l[1]), l23 = pair(l[2], l[3]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t p[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 y = unpair(fma2(pair(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])), mul2, base2));
-            const float u = exp2_fast(y.x), v = exp2_fast(y.y);
-            if (i & 1)
-              l23 = add2(l23, pair(u, v));
-            else
-              l01 = add2(l01, pair(u, v));
-            p[i] = pack_half2(u, v);
-          }
-          tmem_store16(S + 16 * c, p);
-          if (c == 1) {  // the product with the first half of the keys starts here
-            tmem_wait_store();
-            fence_before();
-            mbar_arrive(&sm.p_full[t][0]);
-          }
-        }
-        if (tiles > 1 && !(t == 1 && j == chunks - 1)) turn_give(t ^ 1, warp & 3);
-        const float2 la = unpair(l01), lb = unpair(l23);
-        l[0] = la.x, l[1] = la.y, l[2] = lb.x, l[3] = lb.y;
+        tmem_store16(S, p[0]), tmem_store16(S + 16, p[1]);
         tmem_wait_store();
         fence_before();
-        mbar_arrive(&sm.p_full[t][1]);
+        named_arrive(kPReady + 2 * t, 160);  // the product with the first half of the keys starts here
+        weights(2, p[0]), weights(3, p[1]);
+        tmem_store16(S + 32, p[0]), tmem_store16(S + 48, p[1]);
+        if (tiles > 1 && !(t == 1 && j == chunks - 1)) named_arrive(kTurn + 4 * (t ^ 1) + (warp & 3), 64);
+        const float2 la = unpair(part01), lb = unpair(part23);
+        l[0] += la.x, l[1] += la.y, l[2] += lb.x, l[3] += lb.y;
+        tmem_wait_store();
+        fence_before();
+        named_arrive(kPReady + 2 * t + 1, 160);
       }
 
       // O / l
@@ -1169,22 +1176,23 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
         patience.wait(&sm.all_done[t], 0);
         fence_after();
       }
-      const int tok_head = h * a.group + row - i0 * a.group;
       const float sum = (l[0] + l[1]) + (l[2] + l[3]), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      uint8_t *dst = a.out + (it.first + i0) * a.o_token_stride + tok_head * a.o_head_stride;
+      // through the rows' places in shared memory, whose queries are done with, so that whole rows are written
+      const uint32_t at_row = smem_addr(&sm.q[t][0][0]) + r * 128;
 #pragma unroll 1
-      for (int c = 0; c < D / 16; ++c) {
-        uint32_t x[16];
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t x[32];
         if (chunks) {
-          tmem_load16(x, o_at(t) + lanes + 16 * c);
+          tmem_load32(x, o_at(t) + lanes + 32 * c);
           tmem_wait_load(x);
         }
-        if (valid) {
-          uint32_t y[8];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float u = sum == 0.0f ? 0.0f : __uint_as_float(x[2 * k]) * inv;
-            const float v = sum == 0.0f ? 0.0f : __uint_as_float(x[2 * k + 1]) * inv;
+        for (int i = 0; i < 4; ++i) {
+          uint32_t y[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float u = sum == 0.0f ? 0.0f : __uint_as_float(x[8 * i + 2 * k]) * inv;
+            const float v = sum == 0.0f ? 0.0f : __uint_as_float(x[8 * i + 2 * k + 1]) * inv;
             if (BF16) {
               const __nv_bfloat162 z = __floats2bfloat162_rn(u, v);
               y[k] = *reinterpret_cast<const uint32_t *>(&z);
@@ -1192,11 +1200,27 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
               y[k] = pack_half2(u, v);
             }
           }
-          reinterpret_cast<uint4 *>(dst)[2 * c] = make_uint4(y[0], y[1], y[2], y[3]);
-          reinterpret_cast<uint4 *>(dst)[2 * c + 1] = make_uint4(y[4], y[5], y[6], y[7]);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at_row + c / 2 * ManySmem<D>::kRows +
+                                                                        ((c % 2 * 4 + i) ^ (r & 7)) * 16),
+                       "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3])
+                       : "memory");
         }
       }
-      if (a.lse && valid) a.lse[(it.first + i0) * (a.kv_heads * a.group) + tok_head] = natural_lse(base, sum);
+      __syncwarp();
+#pragma unroll 4
+      for (int i = 0; i < 32; i += kAtOnce) {
+        const int rr = row0 + t * 128 + (warp & 3) * 32 + i + among, tok = token_of(a, rr);
+        uint32_t w[4];
+        load_shared(w, place(i));
+        if (rr < nrows)
+          *reinterpret_cast<uint4 *>(a.out + (it.first + tok) * a.o_token_stride +
+                                     (h * a.group + rr - tok * a.group) * a.o_head_stride + part * 16) =
+              make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      if (a.lse && valid) {
+        const int tok = token_of(a, row);
+        a.lse[(it.first + tok) * (a.kv_heads * a.group) + h * a.group + row - tok * a.group] = natural_lse(base, sum);
+      }
     }
   } else if (warp < 4 * kTiles + kFillWarps) {
     // ---- K and V into shared memory ----
@@ -1320,7 +1344,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
         uint64_t v = v_desc + (i & (kRing - 1)) * kBlocks * kCols16;
 #pragma unroll 1
         for (int half = 0; half < 2; ++half, p += 32, v += kKeys / 2 * 8) {
-          patience.wait(&sm.p_full[t][half], i & 1);
+          named_wait(kPReady + 2 * t + half, 160);
           fence_after();
           mma_ts(o, p, v, kPV, i + half > 0, one);
 #pragma unroll
@@ -1441,10 +1465,11 @@ int fkv_fp4_attention(const void *layer, int64_t num_blocks, int tokens_per_bloc
     return fail(FKV_ERR_UNSUPPORTED, std::string(w) + "queries must be bfloat16 or half");
   if (num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads)
     return bad("the query heads must be a multiple of the key heads");
+  if (num_q_heads / num_kv_heads > 4096) return bad("at most 4096 query heads to a key head");
   if (num_blocks < 0 || num_q_tokens < 0 || num_seqs < 0 || max_blocks < 0) return bad("counts must be non-negative");
   if (!std::isfinite(softmax_scale)) return bad("softmax_scale must be finite");
   if (num_q_tokens == 0 || num_seqs == 0) return FKV_OK;
-  if (num_q_tokens * num_q_heads >= INT32_MAX) return bad("2^31 (token, head) rows or more in one call");
+  if (num_q_tokens * num_q_heads >= 1 << 28) return bad("2^28 (token, head) rows or more in one call");
   if (!q || !out || !seq_lens || (max_blocks > 0 && !block_tables) || (num_blocks > 0 && !layer)) return bad("null pointer");
   if (!cu_seqlens_q && num_q_tokens % num_seqs) return bad("without cu_seqlens_q every sequence has the same number of new tokens");
   if ((uintptr_t)layer % 16 || kv_stride_in_bytes % 16 || block_stride_in_bytes % 16 || (uintptr_t)q % 16 ||
@@ -1456,6 +1481,7 @@ int fkv_fp4_attention(const void *layer, int64_t num_blocks, int tokens_per_bloc
   a.block_stride = block_stride_in_bytes, a.tokens_per_block = tokens_per_block, a.kv_heads = num_kv_heads;
   a.group = num_q_heads / num_kv_heads;
   a.upb = tokens_per_block / 16, a.upb_magic = ((uint64_t)1 << 40) / a.upb + 1;
+  a.group_magic = ((uint64_t)1 << 40) / a.group + 1;
   a.q = (const uint8_t *)q, a.q_token_stride = q_token_stride_in_bytes, a.q_head_stride = q_head_stride_in_bytes;
   a.out = (uint8_t *)out, a.o_token_stride = out_token_stride_in_bytes, a.o_head_stride = out_head_stride_in_bytes;
   a.lse = lse, a.num_q = num_q_tokens, a.tables = block_tables, a.table_stride = block_table_stride;
