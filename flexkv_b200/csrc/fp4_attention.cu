@@ -24,8 +24,7 @@ struct AttnArgs {
   int64_t num_blocks, kv_stride, block_stride;
   int tokens_per_block, kv_heads, group;
   int upb;             // units of a block
-  // x / upb = (x * upb_magic) >> 40, x / group likewise, for x < 2^28 and divisors up to 2^12
-  uint64_t upb_magic, group_magic;
+  uint64_t upb_magic;  // u / upb = (u * upb_magic) >> 40 for u < 2^28, upb <= 2^12
   const uint8_t *q;
   int64_t q_token_stride, q_head_stride;  // bytes
   uint8_t *out;
@@ -53,7 +52,7 @@ template <bool BF16, int N>
 __device__ __forceinline__ void store_row(const AttnArgs &a, int64_t first, int h, int row, int nrows, int c,
                                           const float (&v)[N], float m, float l) {
   if (row >= nrows) return;
-  const int i = (int)(((uint64_t)row * a.group_magic) >> 40), qh = h * a.group + row - i * a.group;
+  const int i = row / a.group, qh = h * a.group + row - i * a.group;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   uint32_t w[N / 2];
 #pragma unroll
@@ -132,8 +131,6 @@ struct Item {     // what a warp needs of one sequence
   int blocks;     // blocks of R (token, head) rows
   int units;      // units to pass, at least one where there are rows
 };
-
-__device__ __forceinline__ int token_of(const AttnArgs &a, int row) { return (int)(((uint64_t)row * a.group_magic) >> 40); }
 
 template <int R>
 __device__ __forceinline__ Item item_of(const AttnArgs &a, int b) {
@@ -492,7 +489,7 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) x[i] = 0;
         if (r < nrows) {
-          const int i0 = token_of(a, r);
+          const int i0 = r / a.group;
           const uint8_t *p = a.q + (cur.it.first + i0) * a.q_token_stride +
                              (h * a.group + r - i0 * a.group) * a.q_head_stride + t * (D / 2);
 #pragma unroll
@@ -526,7 +523,7 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
           int e = 0;
           if (rr < nrows) {
             e = cur.it.len;
-            if (a.causal) e = max(min(e, cur.it.len_q - cur.it.rows + token_of(a, rr) + 1), 0);
+            if (a.causal) e = max(min(e, cur.it.len_q - cur.it.rows + rr / a.group + 1), 0);
             lowest = min(lowest, e);
           }
           end[n][j] = e;
@@ -789,15 +786,13 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
 //    thread.  The base moves only when a score passes it by kMove, as in the
 //    kernel above: then the weights are taken again and O is scaled in place.
 // Two tiles of rows alternate: while one is in softmax the tensor core works
-// on the other, and K and V are converted once for both.
-// Tensor memory (512 columns): O of both tiles, S of both; P lies over S.
+// on the other, and K and V are converted once for both.  A tile has two
+// buffers for S, so that the next scores are there when a softmax ends.
+// Tensor memory (512 columns): O of both tiles, two S of both; P lies over S.
 
-constexpr int kTiles = 2, kKeys = 128, kRing = 2;
+constexpr int kTiles = 2, kKeys = 64, kRing = 4;
 constexpr int kFillWarps = 4;
-constexpr int kManyThreads = (4 * kTiles + kFillWarps + 4) * 32;  // of the last four, one for each tile issues products
-// Registers of a thread of each kind; launched with 128, so the sum over all may be 512 * 128.
-constexpr int kRowRegs = 192, kFillRegs = 96, kIssueRegs = 32;
-static_assert(kRowRegs * 128 * kTiles + kFillRegs * 128 + kIssueRegs * 128 <= kManyThreads * 128, "register split");
+constexpr int kManyThreads = (4 * kTiles + kFillWarps + kTiles) * 32;
 
 template <int D>
 struct ManySmem {
@@ -805,9 +800,9 @@ struct ManySmem {
   alignas(1024) uint8_t q[kTiles][D / 64][kRows];
   alignas(1024) uint8_t k[kRing][D / 64][kCols];
   alignas(1024) uint8_t v[kRing][D / 64][kCols];
-  uint64_t q_full, full[kRing], empty[kRing];  // of a step: K a chunk ahead, and V
-  uint64_t s_full[kTiles], o_done[kTiles], all_done[kTiles];
-  alignas(4) uint8_t bad[2 * kRing][kFillWarps];  // of a chunk of keys, a warp's two units: whose page is outside the pool
+  uint64_t q_full, full[kRing], empty[kRing];  // of a step: K two chunks ahead, and V
+  uint64_t s_full[kTiles][2], p_full[kTiles][2], o_done[kTiles], all_done[kTiles];
+  alignas(4) uint8_t bad[2 * kRing][kFillWarps];  // of a chunk of keys, a warp's unit: its page is outside the pool
   uint32_t tmem;
 };
 
@@ -903,32 +898,14 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-template <int N>
-__device__ __forceinline__ void more_registers() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void fewer_registers() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-
 #define FKV_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
 #define FKV_W8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
-// What was loaded may be used from here on: the registers go through the wait.
-#define FKV_RW8(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7])
-__device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : FKV_RW8(r, 0), FKV_RW8(r, 8), FKV_RW8(r, 16), FKV_RW8(r, 24)
-               :
+// 16 or 32 columns of the warp's 32 lanes.
+__device__ __forceinline__ void tmem_load16(uint32_t (&r)[16], uint32_t at) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : FKV_R8(r, 0), FKV_R8(r, 8)
+               : "r"(at)
                : "memory");
-}
-// 8, 16 or 32 columns of the warp's 32 lanes.
-__device__ __forceinline__ void tmem_load8(uint32_t (&r)[8], uint32_t at) {  // and waits
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : FKV_R8(r, 0) : "r"(at) : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" : FKV_RW8(r, 0) : : "memory");
-}
-__device__ __forceinline__ void tmem_store8(uint32_t at, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), FKV_W8(r, 0) : "memory");
 }
 __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&r)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
@@ -943,20 +920,18 @@ __device__ __forceinline__ void tmem_load32(uint32_t (&r)[32], uint32_t at) {
       : "r"(at)
       : "memory");
 }
+// What was loaded may be used from here on: the registers go through the wait.
+#define FKV_RW8(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7])
+__device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : FKV_RW8(r, 0), FKV_RW8(r, 8) : : "memory");
+}
+__device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : FKV_RW8(r, 0), FKV_RW8(r, 8), FKV_RW8(r, 16), FKV_RW8(r, 24)
+               :
+               : "memory");
+}
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-// Barriers between warps of the CTA by number: turns of a tile's warp on a
-// quarter of the SM (the two warps there), halves of P (a tile's four warps and
-// the one that issues its products).  These and not barriers in shared memory
-// where it can be: an access to one of those waits in the same queue as the
-// exponentials, some hundred cycles when it is full.
-constexpr int kTurn = 1, kPReady = kTurn + 4 * kTiles;
-__device__ __forceinline__ void named_wait(int id, int threads) {
-  asm volatile("barrier.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-__device__ __forceinline__ void named_arrive(int id, int threads) {
-  asm volatile("barrier.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_constant__ AttnArgs a) {
@@ -1012,7 +987,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
   const int tiles = nrows - row0 > 128 ? 2 : 1;
   auto end_of = [&](int row) {  // the keys that a row sees
     int e = it.len;
-    if (a.causal) e = max(min(e, it.len_q - it.rows + token_of(a, row) + 1), 0);
+    if (a.causal) e = max(min(e, it.len_q - it.rows + row / a.group + 1), 0);
     return e;
   };
   const int most = end_of(min(nrows - 1, row0 + R - 1));
@@ -1022,7 +997,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
     mbar_init(&sm.q_full, 128 * tiles);
     for (int i = 0; i < kRing; ++i) mbar_init(&sm.full[i], kFillWarps * 32), mbar_init(&sm.empty[i], tiles);
     for (int t = 0; t < kTiles; ++t) {
-      mbar_init(&sm.s_full[t], 1);
+      for (int i = 0; i < 2; ++i) mbar_init(&sm.s_full[t][i], 1), mbar_init(&sm.p_full[t][i], 128);
       mbar_init(&sm.o_done[t], 1), mbar_init(&sm.all_done[t], 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -1036,50 +1011,45 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
   fence_after();
   const uint32_t tmem = sm.tmem;
   auto o_at = [&](int t) { return tmem + t * 128; };
-  auto s_at = [&](int t) { return tmem + (kTiles + t) * 128; };
+  auto s_at = [&](int t, int i) { return tmem + (kTiles + t) * 128 + i * kKeys; };
   Patience patience;
 
   if (warp < 4 * kTiles) {
     // ---- a thread for each row ----
-    more_registers<kRowRegs>();
     const int t = warp >> 2, r = (warp & 3) * 32 + lane, row = row0 + t * 128 + r;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // the warp's 32 lanes of tensor memory
     if (t < tiles) {
       const bool valid = row < nrows;
-      // The warp's 32 rows come in together, kAtOnce at a time with kLanes lanes for each, so that whole rows are read.
-      constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;
-      const int part = lane % kLanes, among = lane / kLanes;
-      const uint32_t at_q = smem_addr(&sm.q[t][part / 8][0]) + ((warp & 3) * 32 + among) * 128;
-      auto place = [&](int i) { return at_q + i * 128 + ((part % 8) ^ ((i + among) & 7)) * 16; };  // of row i + among
-#pragma unroll 4
-      for (int i = 0; i < 32; i += kAtOnce) {
-        const int rr = min(row0 + t * 128 + (warp & 3) * 32 + i + among, nrows - 1), tok = token_of(a, rr);
-        copy16(place(i), a.q + (it.first + tok) * a.q_token_stride + (h * a.group + rr - tok * a.group) * a.q_head_stride + part * 16);
-      }
-      copies_commit();
-      copies_wait<0>();
+      const int i0 = valid ? row / a.group : 0;
       float mul = 0;
-#pragma unroll 2
-      for (int i = 0; i < 32; i += kAtOnce) {  // a lane converts the piece that it brought
-        uint32_t w[4];
-        load_shared(w, place(i));
+      {
+        const uint8_t *p = a.q + (it.first + i0) * a.q_token_stride + (h * a.group + row - i0 * a.group) * a.q_head_stride;
         float amax = 0;
+        uint4 x[D / 8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 f = pair_to_float2<BF16>(w[k]);
-          amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+        for (int i = 0; i < D / 8; ++i) x[i] = valid ? reinterpret_cast<const uint4 *>(p)[i] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = pair_to_float2<BF16>(w[j]);
+            amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
         }
-#pragma unroll
-        for (int k = 1; k < kLanes; k <<= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, k));
         const float f = row_factor(amax), fs = a.scale < 0.0f ? -f : f;
+        mul = fmaxf(fabsf(a.scale) * 1.4426950408889634f * (1.0f / f), 1e-37f);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 z = pair_to_float2<BF16>(w[k]);
-          w[k] = pack_half2(z.x * fs, z.y * fs);
+        for (int i = 0; i < D / 8; ++i) {
+          const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+          uint32_t y[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 z = pair_to_float2<BF16>(w[j]);
+            y[j] = pack_half2(z.x * fs, z.y * fs);
+          }
+          *reinterpret_cast<uint4 *>(&sm.q[t][i / 8][r * 128 + ((i % 8) ^ (r & 7)) * 16]) = make_uint4(y[0], y[1], y[2], y[3]);
         }
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place(i)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-        const float theirs = __shfl_sync(~0u, f, lane % kAtOnce * kLanes);
-        if (lane / kAtOnce == i / kAtOnce) mul = fmaxf(fabsf(a.scale) * 1.4426950408889634f * (1.0f / theirs), 1e-37f);
       }
       fence_async();
       mbar_arrive(&sm.q_full);
@@ -1087,60 +1057,34 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
       const int end = valid ? end_of(row) : 0;
       const int lowest = __reduce_min_sync(~0u, valid ? end : INT32_MAX);
       float base = kNone, bar = -INFINITY, l[4] = {0, 0, 0, 0};
-      if (t == 1 && chunks) named_arrive(kTurn + (warp & 3), 64);
       for (int j = 0; j < chunks; ++j) {
-        patience.wait(&sm.s_full[t], j & 1);
+        patience.wait(&sm.s_full[t][j & 1], (j >> 1) & 1);
         fence_after();
-        const uint32_t S = s_at(t) + lanes;
-        uint32_t x[4][32];
+        const uint32_t S = s_at(t, j & 1) + lanes;
+        uint32_t x[2][32];
         tmem_load32(x[0], S), tmem_load32(x[1], S + 32);
         const uint32_t bad = *(volatile uint32_t *)sm.bad[j & (2 * kRing - 1)];
         tmem_wait_load(x[0]), tmem_wait_load(x[1]);
-        tmem_load32(x[2], S + 64), tmem_load32(x[3], S + 96);
-        tmem_wait_load(x[2]), tmem_wait_load(x[3]);
         if ((j + 1) * kKeys > lowest || bad) {  // only what the row sees
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (j * kKeys + 32 * c + i >= end || ((bad >> (8 * c + i / 16)) & 1)) x[c][i] = 0xFF800000u;
+              if (j * kKeys + 32 * c + i >= end || ((bad >> (8 * (2 * c + i / 16))) & 1)) x[c][i] = 0xFF800000u;
         }
-        // Exponentials are what the tiles contend for: the warps of both tiles on a quarter of the SM take turns, so
-        // that one's fall into the other's waits and reads.
-        if (tiles > 1) named_wait(kTurn + 4 * t + (warp & 3), 64);
-        uint64_t mul2 = pair(mul, mul), base2 = pair(-base, -base), part01, part23;
-        auto weights = [&](int c, uint32_t(&p)[16]) {
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 y = unpair(fma2(pair(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])), mul2, base2));
-            const float u = exp2_fast(y.x), v = exp2_fast(y.y);
-            if (i & 1)
-              part23 = add2(part23, pair(u, v));
-            else
-              part01 = add2(part01, pair(u, v));
-            p[i] = pack_half2(u, v);
-          }
-        };
-        uint32_t p[2][16];
-        // The first half of the weights is taken with the base as it is while the row's largest score is found.
-#pragma unroll 1
-        for (bool again = false;; again = true) {
-          part01 = part23 = 0;
-          weights(0, p[0]), weights(1, p[1]);
-          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[c][i]));
-          const float most_here = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-          if (again || !__any_sync(~0u, most_here > bar)) break;  // rare after the first chunks
+          for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[c][i]));
+        const float most_here = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        if (__any_sync(~0u, most_here > bar)) {  // rare after the first chunks
           float f = 1.0f;
           if (most_here > bar) {  // other rows stay: a row does not depend on its neighbours
             const float to = most_here * mul - kLift;
             f = exp2_fast(base - to);
             base = to;
             bar = __fdividef(to + kMove, mul);
-            base2 = pair(-base, -base);
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) l[i] *= f;
@@ -1148,27 +1092,38 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
             patience.wait(&sm.o_done[t], (j - 1) & 1);
             fence_after();
 #pragma unroll 1
-            for (int c = 0; c < D / 8; ++c) {
-              uint32_t y[8];
-              tmem_load8(y, o_at(t) + lanes + 8 * c);
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t y[16];
+              tmem_load16(y, o_at(t) + lanes + 16 * c);
+              tmem_wait_load(y);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
-              tmem_store8(o_at(t) + lanes + 8 * c, y);
+              for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
+              tmem_store16(o_at(t) + lanes + 16 * c, y);
             }
           }
         }
-        tmem_store16(S, p[0]), tmem_store16(S + 16, p[1]);
+        const uint64_t mul2 = pair(mul, mul), base2 = pair(-base, -base);
+        uint64_t l01 = pair(l[0], l[1]), l23 = pair(l[2], l[3]);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t p[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 y = unpair(fma2(pair(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])), mul2, base2));
+            const float u = exp2_fast(y.x), v = exp2_fast(y.y);
+            if (i & 1)
+              l23 = add2(l23, pair(u, v));
+            else
+              l01 = add2(l01, pair(u, v));
+            p[i] = pack_half2(u, v);
+          }
+          tmem_store16(S + 16 * c, p);
+        }
+        const float2 la = unpair(l01), lb = unpair(l23);
+        l[0] = la.x, l[1] = la.y, l[2] = lb.x, l[3] = lb.y;
         tmem_wait_store();
         fence_before();
-        named_arrive(kPReady + 2 * t, 160);  // the product with the first half of the keys starts here
-        weights(2, p[0]), weights(3, p[1]);
-        tmem_store16(S + 32, p[0]), tmem_store16(S + 48, p[1]);
-        if (tiles > 1 && !(t == 1 && j == chunks - 1)) named_arrive(kTurn + 4 * (t ^ 1) + (warp & 3), 64);
-        const float2 la = unpair(part01), lb = unpair(part23);
-        l[0] += la.x, l[1] += la.y, l[2] += lb.x, l[3] += lb.y;
-        tmem_wait_store();
-        fence_before();
-        named_arrive(kPReady + 2 * t + 1, 160);
+        mbar_arrive(&sm.p_full[t][j & 1]);
       }
 
       // O / l
@@ -1176,23 +1131,22 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
         patience.wait(&sm.all_done[t], 0);
         fence_after();
       }
+      const int tok_head = h * a.group + row - i0 * a.group;
       const float sum = (l[0] + l[1]) + (l[2] + l[3]), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      // through the rows' places in shared memory, whose queries are done with, so that whole rows are written
-      const uint32_t at_row = smem_addr(&sm.q[t][0][0]) + r * 128;
+      uint8_t *dst = a.out + (it.first + i0) * a.o_token_stride + tok_head * a.o_head_stride;
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t x[32];
+      for (int c = 0; c < D / 16; ++c) {
+        uint32_t x[16];
         if (chunks) {
-          tmem_load32(x, o_at(t) + lanes + 32 * c);
+          tmem_load16(x, o_at(t) + lanes + 16 * c);
           tmem_wait_load(x);
         }
+        if (valid) {
+          uint32_t y[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t y[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float u = sum == 0.0f ? 0.0f : __uint_as_float(x[8 * i + 2 * k]) * inv;
-            const float v = sum == 0.0f ? 0.0f : __uint_as_float(x[8 * i + 2 * k + 1]) * inv;
+          for (int k = 0; k < 8; ++k) {
+            const float u = sum == 0.0f ? 0.0f : __uint_as_float(x[2 * k]) * inv;
+            const float v = sum == 0.0f ? 0.0f : __uint_as_float(x[2 * k + 1]) * inv;
             if (BF16) {
               const __nv_bfloat162 z = __floats2bfloat162_rn(u, v);
               y[k] = *reinterpret_cast<const uint32_t *>(&z);
@@ -1200,32 +1154,15 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
               y[k] = pack_half2(u, v);
             }
           }
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at_row + c / 2 * ManySmem<D>::kRows +
-                                                                        ((c % 2 * 4 + i) ^ (r & 7)) * 16),
-                       "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3])
-                       : "memory");
+          reinterpret_cast<uint4 *>(dst)[2 * c] = make_uint4(y[0], y[1], y[2], y[3]);
+          reinterpret_cast<uint4 *>(dst)[2 * c + 1] = make_uint4(y[4], y[5], y[6], y[7]);
         }
       }
-      __syncwarp();
-#pragma unroll 4
-      for (int i = 0; i < 32; i += kAtOnce) {
-        const int rr = row0 + t * 128 + (warp & 3) * 32 + i + among, tok = token_of(a, rr);
-        uint32_t w[4];
-        load_shared(w, place(i));
-        if (rr < nrows)
-          *reinterpret_cast<uint4 *>(a.out + (it.first + tok) * a.o_token_stride +
-                                     (h * a.group + rr - tok * a.group) * a.o_head_stride + part * 16) =
-              make_uint4(w[0], w[1], w[2], w[3]);
-      }
-      if (a.lse && valid) {
-        const int tok = token_of(a, row);
-        a.lse[(it.first + tok) * (a.kv_heads * a.group) + h * a.group + row - tok * a.group] = natural_lse(base, sum);
-      }
+      if (a.lse && valid) a.lse[(it.first + i0) * (a.kv_heads * a.group) + tok_head] = natural_lse(base, sum);
     }
   } else if (warp < 4 * kTiles + kFillWarps) {
     // ---- K and V into shared memory ----
-    fewer_registers<kFillRegs>();
-    // Warp w brings units 2 w and 2 w + 1 of a chunk, 8 tokens at a time, a quarter of a row a lane: 8 lanes that store together
+    // Warp w brings unit w of a chunk, 8 tokens at a time, a quarter of a row a lane: 8 lanes that store together
     // have 8 rows, so the swizzle spreads them over all banks.
     const int w = warp - 4 * kTiles, tok = lane & 7, quarter = lane >> 3;
     constexpr int kWords = D / 32;  // of a lane's piece, 8 channels each
@@ -1234,51 +1171,47 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
 #pragma unroll
     for (int k = 0; k < kWords; ++k) {
       const int c = quarter * kWords + k;
-      at_chunk[k] = (c >> 3) * ManySmem<D>::kCols + w * 32 * 128 + tok * 128 + ((c & 7) ^ tok) * 16;
+      at_chunk[k] = (c >> 3) * ManySmem<D>::kCols + w * 16 * 128 + tok * 128 + ((c & 7) ^ tok) * 16;
     }
-    auto page_of = [&](int j, int i) {
-      const int u = j * (kKeys / 16) + 2 * w + i, e = (int)(((uint64_t)u * a.upb_magic) >> 40);
+    auto page_of = [&](int j) {
+      const int u = j * (kKeys / 16) + w, e = (int)(((uint64_t)u * a.upb_magic) >> 40);
       return u * 16 < most && e < a.max_blocks ? a.tables[b * a.table_stride + e] : -1;
     };
-    uint32_t x[2][4][kWords], sc[2][4];  // pieces of K and of V of a chunk, on their way
-    int64_t unit[2], last[2];            // units of a chunk, and of the one before, from the layer on; none: -1
-    int page[2];
+    uint32_t x[2][2][kWords], sc[2][2];  // pieces of K and of V of a chunk, on their way
+    const uint8_t *unit;                 // none: nothing is loaded and no scale taken
+    int page;
     uint32_t bad = 0;
-    auto find = [&](int j) {  // the units of chunk j, and the pages of the chunk after it
-      bad = 0;
+    auto find = [&](int j) {  // the unit of chunk j, and the page of the chunk after it
+      const int u = j * (kKeys / 16) + w, e = (int)(((uint64_t)u * a.upb_magic) >> 40);
+      const bool good = page >= 0 && page < a.num_blocks;
+      unit = good ? a.layer + page * a.block_stride + ((int64_t)h * a.upb + u - e * a.upb) * (9 * D) : nullptr;
+      bad = !good && u * 16 < most;
+      page = page_of(j + 1);
+    };
+    auto fetch = [&](int j, int side) {
+      const uint8_t *p = unit + side * a.kv_stride;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int u = j * (kKeys / 16) + 2 * w + i, e = (int)(((uint64_t)u * a.upb_magic) >> 40);
-        const bool good = page[i] >= 0 && page[i] < a.num_blocks;
-        unit[i] = good ? page[i] * a.block_stride + ((int64_t)h * a.upb + u - e * a.upb) * (9 * D) : -1;
-        bad |= !good && u * 16 < most ? 1u << i : 0;
-        page[i] = page_of(j + 1, i);
-      }
-    };
-    auto fetch = [&](int j, int side, const int64_t(&from)[2]) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
         sc[side][i] = 0;  // what no row sees may be anything: its scale counts as zero
 #pragma unroll
         for (int k = 0; k < kWords; ++k) x[side][i][k] = 0;
-        if (from[i >> 1] >= 0) {
-          const uint8_t *p = a.layer + from[i >> 1] + side * a.kv_stride;
+        if (unit) {
           if constexpr (D == 128) {
-            const uint4 y = __ldg(reinterpret_cast<const uint4 *>(p + at_row + (i & 1) * 8 * (D / 2)));
+            const uint4 y = __ldg(reinterpret_cast<const uint4 *>(p + at_row + i * 8 * (D / 2)));
             x[side][i][0] = y.x, x[side][i][1] = y.y, x[side][i][2] = y.z, x[side][i][3] = y.w;
           } else {
-            const uint2 y = __ldg(reinterpret_cast<const uint2 *>(p + at_row + (i & 1) * 8 * (D / 2)));
+            const uint2 y = __ldg(reinterpret_cast<const uint2 *>(p + at_row + i * 8 * (D / 2)));
             x[side][i][0] = y.x, x[side][i][1] = y.y;
           }
-          const uint8_t *q = p + at_scale + (i & 1) * 8 * (D / 16);
-          if (j * kKeys + w * 32 + i * 8 + tok < most)
+          const uint8_t *q = p + at_scale + i * 8 * (D / 16);
+          if (j * kKeys + w * 16 + i * 8 + tok < most)
             sc[side][i] = D == 128 ? __ldg(reinterpret_cast<const uint16_t *>(q)) : __ldg(q);
         }
       }
     };
     auto put = [&](uint32_t dst, int side) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 2; ++i) {
         const uint32_t s[2] = {__byte_perm(sc[side][i], 0, 0x0404) >> 1, __byte_perm(sc[side][i], 0, 0x1414) >> 1};
 #pragma unroll
         for (int k = 0; k < kWords; ++k) {
@@ -1294,27 +1227,32 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
     };
     const uint32_t k_at = smem_addr(sm.k[0]), v_at = smem_addr(sm.v[0]);
     constexpr uint32_t kStage = D / 64 * ManySmem<D>::kCols;
-    // Steps i from -1 on: K of chunk i + 1, then V of chunk i.  Their pieces are loaded a step ahead.
-    page[0] = page_of(0, 0), page[1] = page_of(0, 1);
-    if (chunks) find(0), fetch(0, 0, unit);
+    // Steps i from -2 on: K of chunk i + 2, then V of chunk i.  Their pieces are loaded a step ahead.
+    const uint8_t *units[3];  // of the chunks i, i + 1, i + 2
+    page = page_of(0);
+    if (chunks) find(0), fetch(0, 0);
 #pragma unroll 1
-    for (int i = chunks ? -1 : 0; i < chunks; ++i) {
-      const int slot = (i + 1) & (kRing - 1);
-      if (i + 1 >= kRing) patience.wait(&sm.empty[slot], ((i + 1) / kRing + 1) & 1);
-      last[0] = unit[0], last[1] = unit[1];  // of chunk i + 1, whose V comes next
-      if (i + 1 < chunks) {
+    for (int i = chunks ? -2 : 0; i < chunks; ++i) {
+      const int slot = (i + 2) & (kRing - 1);
+      if (i + 2 >= kRing) patience.wait(&sm.empty[slot], ((i + 2) / kRing + 1) & 1);
+      units[0] = units[1], units[1] = units[2], units[2] = unit;
+      if (i + 2 < chunks) {
         put(k_at + slot * kStage, 0);
-        if (lane == 0) sm.bad[(i + 1) & (2 * kRing - 1)][w] = (uint8_t)bad;  // read before the chunk 2 kRing on gets here
-        if (i + 2 < chunks) find(i + 2), fetch(i + 2, 0, unit);
+        if (lane == 0) sm.bad[(i + 2) & (2 * kRing - 1)][w] = (uint8_t)bad;  // read before the chunk 2 kRing on gets here
+        if (i + 3 < chunks) find(i + 3), fetch(i + 3, 0);
       }
       if (i >= 0) put(v_at + (i & (kRing - 1)) * kStage, 1);
       fence_async();
       mbar_arrive(&sm.full[slot]);
-      if (i + 1 < chunks) fetch(i + 1, 1, last);
+      if (i + 1 >= 0 && i + 1 < chunks) {
+        const uint8_t *keep = unit;
+        unit = units[1];
+        fetch(i + 1, 1);
+        unit = keep;
+      }
     }
   } else {
     // ---- the products: a warp for each tile ----
-    fewer_registers<kIssueRegs>();
     // In loops and not straight code: these warps share their instruction caches with three busier ones each.  The
     // shuffles keep what addresses and trip counts come from in uniform registers, where the instructions want them.
     constexpr uint32_t kQK = mma_desc(kKeys, false), kPV = mma_desc(D, true);
@@ -1327,37 +1265,35 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
                    k_desc = smem_desc(smem_addr(sm.k), false), v_desc = smem_desc(smem_addr(sm.v), true);
     auto score = [&](int j) {  // S of chunk j
       uint64_t q = q_desc, k = k_desc + (j & (kRing - 1)) * kBlocks * kCols16;
+      const uint32_t d = s + (j & 1) * kKeys;
 #pragma unroll 1
       for (int c = 0; c < kBlocks; ++c, q += kRows16, k += kCols16) {
-        mma_ss(s, q, k, kQK, c > 0, one);
+        mma_ss(d, q, k, kQK, c > 0, one);
 #pragma unroll
-        for (int i = 1; i < 4; ++i) mma_ss(s, q + i * 2, k + i * 2, kQK, true, one);
+        for (int i = 1; i < 4; ++i) mma_ss(d, q + i * 2, k + i * 2, kQK, true, one);
       }
-      mma_commit(&sm.s_full[t], one);
+      mma_commit(&sm.s_full[t][j & 1], one);
     };
-    auto filled = [&](int i) { patience.wait(&sm.full[(i + 1) & (kRing - 1)], ((i + 1) / kRing) & 1); };
-    if (n) patience.wait(&sm.q_full, 0), filled(-1);
+    auto filled = [&](int i) { patience.wait(&sm.full[(i + 2) & (kRing - 1)], ((i + 2) / kRing) & 1); };
+    if (n) patience.wait(&sm.q_full, 0), filled(-2);
 #pragma unroll 1
-    for (int i = n ? -1 : 0; i < n; ++i) {
+    for (int i = n ? -2 : 0; i < n; ++i) {
       if (i >= 0) {
-        uint32_t p = s;
-        uint64_t v = v_desc + (i & (kRing - 1)) * kBlocks * kCols16;
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half, p += 32, v += kKeys / 2 * 8) {
-          named_wait(kPReady + 2 * t + half, 160);
-          fence_after();
-          mma_ts(o, p, v, kPV, i + half > 0, one);
+        patience.wait(&sm.p_full[t][i & 1], (i >> 1) & 1);
+        fence_after();
+        const uint32_t p = s + (i & 1) * kKeys;
+        const uint64_t v = v_desc + (i & (kRing - 1)) * kBlocks * kCols16;
+        mma_ts(o, p, v, kPV, i > 0, one);
 #pragma unroll
-          for (int k = 1; k < kKeys / 32; ++k) mma_ts(o, p + k * 8, v + k * 128, kPV, true, one);
-        }
+        for (int k = 1; k < kKeys / 16; ++k) mma_ts(o, p + k * 8, v + k * 128, kPV, true, one);
         mma_commit(&sm.o_done[t], one);
       }
-      if (i + 1 < n) {  // its S goes where this chunk's P lies
+      if (i + 2 < n) {  // two chunks ahead: its S goes where this chunk's P lies
         if (i >= 0) patience.wait(&sm.o_done[t], i & 1);
         fence_after();
-        score(i + 1);
+        score(i + 2);
       }
-      mma_commit(&sm.empty[(i + 1) & (kRing - 1)], one);
+      mma_commit(&sm.empty[(i + 2) & (kRing - 1)], one);
       if (i + 1 < n) filled(i + 1);
     }
     if (n) mma_commit(&sm.all_done[t], one);
@@ -1465,11 +1401,10 @@ int fkv_fp4_attention(const void *layer, int64_t num_blocks, int tokens_per_bloc
     return fail(FKV_ERR_UNSUPPORTED, std::string(w) + "queries must be bfloat16 or half");
   if (num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads)
     return bad("the query heads must be a multiple of the key heads");
-  if (num_q_heads / num_kv_heads > 4096) return bad("at most 4096 query heads to a key head");
   if (num_blocks < 0 || num_q_tokens < 0 || num_seqs < 0 || max_blocks < 0) return bad("counts must be non-negative");
   if (!std::isfinite(softmax_scale)) return bad("softmax_scale must be finite");
   if (num_q_tokens == 0 || num_seqs == 0) return FKV_OK;
-  if (num_q_tokens * num_q_heads >= 1 << 28) return bad("2^28 (token, head) rows or more in one call");
+  if (num_q_tokens * num_q_heads >= INT32_MAX) return bad("2^31 (token, head) rows or more in one call");
   if (!q || !out || !seq_lens || (max_blocks > 0 && !block_tables) || (num_blocks > 0 && !layer)) return bad("null pointer");
   if (!cu_seqlens_q && num_q_tokens % num_seqs) return bad("without cu_seqlens_q every sequence has the same number of new tokens");
   if ((uintptr_t)layer % 16 || kv_stride_in_bytes % 16 || block_stride_in_bytes % 16 || (uintptr_t)q % 16 ||
@@ -1481,7 +1416,6 @@ int fkv_fp4_attention(const void *layer, int64_t num_blocks, int tokens_per_bloc
   a.block_stride = block_stride_in_bytes, a.tokens_per_block = tokens_per_block, a.kv_heads = num_kv_heads;
   a.group = num_q_heads / num_kv_heads;
   a.upb = tokens_per_block / 16, a.upb_magic = ((uint64_t)1 << 40) / a.upb + 1;
-  a.group_magic = ((uint64_t)1 << 40) / a.group + 1;
   a.q = (const uint8_t *)q, a.q_token_stride = q_token_stride_in_bytes, a.q_head_stride = q_head_stride_in_bytes;
   a.out = (uint8_t *)out, a.o_token_stride = out_token_stride_in_bytes, a.o_head_stride = out_head_stride_in_bytes;
   a.lse = lse, a.num_q = num_q_tokens, a.tables = block_tables, a.table_stride = block_table_stride;
