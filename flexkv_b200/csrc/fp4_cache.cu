@@ -31,9 +31,13 @@ struct RowsArgs {
   int num_heads;
   int kv_dim;
   int tokens_per_block;
+  int upb;                // units (16 tokens) of a block
+  int groups;             // groups (16 channels) of a head
+  uint64_t upb_magic, groups_magic;  // x / upb = (x * upb_magic) >> 40 for x < 2^28 and a divisor up to 2^12
+  bool far;               // more units than that in the 4-bit layer, or in a block
   int64_t num_rows;       // tokens of the call (blocks * tokens_per_block for the block form)
   int64_t num_slots;      // slots of the 4-bit layer
-  int64_t num_row_slots;  // slots of the 16-bit side (block form)
+  int64_t num_blocks, num_row_blocks;  // of the 4-bit and of the 16-bit side (block form)
   int64_t fp4_kv_stride, fp4_block_stride;
   int64_t token_stride[2], head_stride[2];        // bytes, 16-bit side
   int64_t row_block_stride;                        // bytes, block form
@@ -67,78 +71,114 @@ __device__ __forceinline__ void store_group(uint8_t *p, const uint32_t (&r)[8]) 
   }
 }
 
-// One thread per group of 16 channels.  A CTA takes R consecutive rows of the
-// list (R = 16, or 1 for a call with fewer rows than 16) of one layer and
-// side, for every head; threads run over groups first, then rows, then heads,
-// so 32 lanes store 256 payload bytes and 32 scale bytes of one unit next to
-// each other.  NG: groups of a head, 0 = at run time.
+// One thread per group of 16 channels, kUnroll of them under way at a time.  A
+// CTA takes R consecutive rows of the list (R = 16, or 1 for a call with fewer
+// rows than 16) of one layer and side, for every head: neighbouring threads have
+// neighbouring groups, then rows, so that 32 lanes store 256 payload bytes and
+// 32 scale bytes of one unit next to each other.  NG: groups of a head where
+// they and the rows divide the CTA's threads evenly: a thread then keeps its
+// row and group through all heads and looks its slot up once.  0: at run time,
+// a place for each group.
 template <bool WRITE, bool BF16, bool BLOCKS, bool WIDE, int NG, int R>
-__global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constant__ RowsArgs a, int groups) {
-  const int ng = NG ? NG : groups;
-  const int layer = blockIdx.y / a.kv_dim, side = blockIdx.y % a.kv_dim;
+__global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constant__ RowsArgs a) {
+  const int ng = NG ? NG : a.groups, D = 16 * ng;
+  const int layer = a.kv_dim == 1 ? blockIdx.y : blockIdx.y >> 1, side = a.kv_dim == 1 ? 0 : blockIdx.y & 1;
   const int64_t row0 = (int64_t)blockIdx.x * R;
-  const int work = a.num_heads * R * ng;
   uint8_t *const fp4 = a.fp4[layer] + side * a.fp4_kv_stride;
   uint8_t *const rows = a.rows[side][layer];
-  const int D = 16 * ng, tpb = a.tokens_per_block;
-  for (int w0 = threadIdx.x; w0 < work; w0 += kThreads * kUnroll) {
-    uint32_t x[kUnroll][8];
-    uint8_t *pay[kUnroll], *sc[kUnroll], *row[kUnroll];
+  const int64_t token_stride = a.token_stride[side], head_stride = a.head_stride[side];
+  const int64_t unit_step = (int64_t)a.upb * (9 * D);  // from a head's unit to the next head's
+
+  // Unit of the first head and 16-bit row of row t of the CTA: null where there is none.
+  auto find = [&](int t, uint8_t *&unit, uint8_t *&row, int &off) {
+    const int64_t i = row0 + t;
+    unit = row = nullptr;
+    if (i >= a.num_rows) return;
+    if (BLOCKS) {
+      // a block's rows are multiples of 16, R = 16: row 0 says which block
+      const int64_t u = row0 >> 4;
+      const int64_t blk = a.far ? u / a.upb : (int64_t)(((uint64_t)u * a.upb_magic) >> 40);
+      const int in = (int)(u - blk * a.upb);
+      const int64_t fb = a.fp4_ids[blk], rb = a.row_ids[blk];
+      if (fb < 0 || fb >= a.num_blocks || rb < 0 || rb >= a.num_row_blocks) return;
+      off = t;
+      unit = fp4 + fb * a.fp4_block_stride + (int64_t)in * (9 * D);
+      row = rows + rb * a.row_block_stride + (in * 16 + t) * token_stride;
+    } else {
+      row = rows + i * token_stride;
+      const int64_t slot = a.fp4_ids[i];
+      if (slot < 0 || slot >= a.num_slots) return;
+      const int64_t u = slot >> 4;
+      const int64_t blk = a.far ? u / a.upb : (int64_t)(((uint64_t)u * a.upb_magic) >> 40);
+      off = (int)(slot & 15);
+      unit = fp4 + blk * a.fp4_block_stride + (u - blk * a.upb) * (9 * D);
+    }
+  };
+  auto load = [&](uint32_t(&x)[8], const uint8_t *unit, const uint8_t *row, int off, int g) {
+    if (WRITE) {
+      if (unit) load_group<WIDE>(row + g * 32, x);
+    } else if (unit) {
+      const uint2 p = *reinterpret_cast<const uint2 *>(unit + off * (D / 2) + g * 8);
+      x[0] = p.x, x[1] = p.y, x[2] = unit[8 * D + off * ng + g];
+    } else {
+      x[0] = x[1] = x[2] = 0;  // a row without a slot reads as zeros
+    }
+  };
+  auto finish = [&](uint32_t(&x)[8], uint8_t *unit, uint8_t *row, int off, int g) {
+    if (WRITE) {
+      if (!unit) return;
+      uint2 p;
+      const uint32_t code = quantise_group<BF16>(x, p);
+      *reinterpret_cast<uint2 *>(unit + off * (D / 2) + g * 8) = p;
+      unit[8 * D + off * ng + g] = (uint8_t)code;
+    } else if (row) {
+      uint32_t y[8];
+      dequantise_group<BF16>(make_uint2(x[0], x[1]), x[2], y);
+      store_group<WIDE>(row + g * 32, y);
+    }
+  };
+
+  if (NG) {
+    constexpr int kPlaces = NG ? R * NG : 1, kStep = kThreads / kPlaces;  // heads at a time
+    const int t = threadIdx.x % kPlaces / (NG ? NG : 1), g = threadIdx.x % (NG ? NG : 1);
+    uint8_t *unit, *row;
+    int off = 0;
+    find(t, unit, row, off);
+    if (!row || (WRITE && !unit)) return;
+    for (int h0 = threadIdx.x / kPlaces; h0 < a.num_heads; h0 += kStep * kUnroll) {
+      uint32_t x[kUnroll][8];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int w = w0 + u * kThreads;
-      pay[u] = nullptr, row[u] = nullptr;
-      if (w < work) {
-        const int g = w % ng, t = (w / ng) % R, h = w / (ng * R);
-        const int64_t i = row0 + t;
-        if (i < a.num_rows) {
-          int64_t slot;
-          if (BLOCKS) {
-            const int64_t b = i / tpb, off = i % tpb;
-            const int64_t fb = a.fp4_ids[b], rb = a.row_ids[b];
-            slot = fb < 0 ? -1 : fb * tpb + off;
-            if (rb < 0 || rb >= a.num_row_slots) slot = -1;
-            row[u] = rows + rb * a.row_block_stride + off * a.token_stride[side] + h * a.head_stride[side] + g * 32;
-          } else {
-            slot = a.fp4_ids[i];
-            row[u] = rows + i * a.token_stride[side] + h * a.head_stride[side] + g * 32;
-          }
-          if (slot >= 0 && slot < a.num_slots) {
-            const int64_t b = slot / tpb;
-            const int off = (int)(slot - b * tpb);
-            uint8_t *unit = fp4 + b * a.fp4_block_stride + ((int64_t)h * (tpb / 16) + off / 16) * (9 * D);
-            pay[u] = unit + (off % 16) * (D / 2) + g * 8;
-            sc[u] = unit + 8 * D + (off % 16) * ng + g;
-          }
-          if (pay[u]) {
-            if (WRITE) {
-              load_group<WIDE>(row[u], x[u]);
-            } else {
-              const uint2 p = *reinterpret_cast<const uint2 *>(pay[u]);
-              x[u][0] = p.x, x[u][1] = p.y, x[u][2] = *sc[u];
-            }
-          } else if (!WRITE && !BLOCKS) {
-            x[u][0] = x[u][1] = x[u][2] = 0;  // a row without a slot reads as zeros
-          } else {
-            row[u] = nullptr;
-          }
-        }
+      for (int k = 0; k < kUnroll; ++k) {
+        const int h = h0 + k * kStep;
+        if (h < a.num_heads) load(x[k], unit ? unit + h * unit_step : nullptr, row + h * head_stride, off, g);
+      }
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k) {
+        const int h = h0 + k * kStep;
+        if (h < a.num_heads) finish(x[k], unit ? unit + h * unit_step : nullptr, row + h * head_stride, off, g);
       }
     }
+  } else {
+    const int work = a.num_heads * R * ng;
+    for (int w0 = threadIdx.x; w0 < work; w0 += kThreads * kUnroll) {
+      uint32_t x[kUnroll][8];
+      uint8_t *unit[kUnroll], *row[kUnroll];
+      int off[kUnroll], g[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      if (!row[u]) continue;
-      if (WRITE) {
-        if (!pay[u]) continue;
-        uint2 p;
-        const uint32_t code = quantise_group<BF16>(x[u], p);
-        *reinterpret_cast<uint2 *>(pay[u]) = p;
-        *sc[u] = (uint8_t)code;
-      } else {
-        uint32_t y[8];
-        dequantise_group<BF16>(make_uint2(x[u][0], x[u][1]), x[u][2], y);
-        store_group<WIDE>(row[u], y);
+      for (int k = 0; k < kUnroll; ++k) {
+        const int w = w0 + k * kThreads;
+        unit[k] = row[k] = nullptr, off[k] = 0;
+        if (w >= work) continue;
+        const int q = (int)(((uint64_t)w * a.groups_magic) >> 40), h = q / R;  // w / ng
+        g[k] = w - q * ng;
+        find(q % R, unit[k], row[k], off[k]);
+        if (row[k]) row[k] += h * head_stride;
+        if (unit[k]) unit[k] += h * unit_step;
+        if (row[k]) load(x[k], unit[k], row[k], off[k], g[k]);
       }
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k)
+        if (row[k]) finish(x[k], unit[k], row[k], off[k], g[k]);
     }
   }
 }
@@ -146,17 +186,18 @@ __global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constan
 template <bool WRITE, bool BF16, bool BLOCKS, bool WIDE, int R>
 void launch_ng(const RowsArgs &a, dim3 grid, int ng, cudaStream_t s) {
   switch (ng) {
-    case 4: fp4_rows_kernel<WRITE, BF16, BLOCKS, WIDE, 4, R><<<grid, kThreads, 0, s>>>(a, ng); break;
-    case 8: fp4_rows_kernel<WRITE, BF16, BLOCKS, WIDE, 8, R><<<grid, kThreads, 0, s>>>(a, ng); break;
-    default: fp4_rows_kernel<WRITE, BF16, BLOCKS, WIDE, 0, R><<<grid, kThreads, 0, s>>>(a, ng); break;
+    case 4: fp4_rows_kernel<WRITE, BF16, BLOCKS, WIDE, 4, R><<<grid, kThreads, 0, s>>>(a); break;
+    case 8: fp4_rows_kernel<WRITE, BF16, BLOCKS, WIDE, 8, R><<<grid, kThreads, 0, s>>>(a); break;
+    case 16: fp4_rows_kernel<WRITE, BF16, BLOCKS, WIDE, 16, R><<<grid, kThreads, 0, s>>>(a); break;
+    default: fp4_rows_kernel<WRITE, BF16, BLOCKS, WIDE, 0, R><<<grid, kThreads, 0, s>>>(a); break;
   }
 }
 template <bool WRITE, bool BF16, bool BLOCKS, bool WIDE>
 void launch_r(const RowsArgs &a, int rows_at_once, dim3 grid, int ng, cudaStream_t s) {
-  if (rows_at_once == 16)
+  if (BLOCKS || rows_at_once == 16)
     launch_ng<WRITE, BF16, BLOCKS, WIDE, 16>(a, grid, ng, s);
   else
-    launch_ng<WRITE, BF16, BLOCKS, WIDE, 1>(a, grid, ng, s);
+    launch_ng<WRITE, BF16, BLOCKS, WIDE, BLOCKS ? 16 : 1>(a, grid, ng, s);
 }
 template <bool WRITE, bool BLOCKS>
 void launch_rows(const RowsArgs &a, bool bf16, bool wide, int r, dim3 grid, int ng, cudaStream_t s) {
@@ -186,6 +227,9 @@ bool aligned(const void *p, int64_t to) { return (uintptr_t)p % to == 0; }
 template <bool WRITE, bool BLOCKS>
 int run_rows(RowsArgs &a, int num_layers, int head_size, int dtype, bool wide, cudaStream_t s) {
   const int ng = head_size / 16, r = a.num_rows < 16 ? 1 : 16;
+  a.upb = a.tokens_per_block / 16, a.groups = ng;
+  a.upb_magic = ((uint64_t)1 << 40) / a.upb + 1, a.groups_magic = ((uint64_t)1 << 40) / ng + 1;
+  a.far = a.num_slots >> 32 || a.num_rows >> 32 || a.upb > 4096;
   // grid.x counts row groups: 2^31 - 1 of them is the launch limit
   const int64_t gx = (a.num_rows + r - 1) / r;
   if (gx > INT32_MAX) return fail(FKV_ERR_INVALID_ARG, "more than 2^31 groups of rows in one call");
@@ -254,7 +298,7 @@ int blocks_call(const char *who, int num_layers, void *const *fp4_layers, void *
   }
   RowsArgs a{};
   a.num_heads = heads, a.kv_dim = kv_dim, a.tokens_per_block = tpb;
-  a.num_rows = num * tpb, a.num_slots = fp4_num_blocks * tpb, a.num_row_slots = kv_num_blocks;
+  a.num_rows = num * tpb, a.num_slots = fp4_num_blocks * tpb, a.num_blocks = fp4_num_blocks, a.num_row_blocks = kv_num_blocks;
   a.fp4_kv_stride = fp4_kv_stride, a.fp4_block_stride = fp4_block_stride;
   a.row_block_stride = kv_block_stride;
   for (int i = 0; i < 2; ++i) a.head_stride[i] = 2 * head_size, a.token_stride[i] = (int64_t)2 * head_size * heads;

@@ -23,6 +23,14 @@ __device__ __forceinline__ uint32_t scale_code(float v) {
   return c < 226 ? c : 226;
 }
 
+// amax / 6 for scale_code, exact where it decides: amax has at most 11
+// significant bits, so the quotient either is a border of the scales (5 bits)
+// or is 2^-11 of it away, and the product with 1/6, off by 2^-23, rounded to 15
+// bits is on the same side, or the border itself.
+__device__ __forceinline__ float sixth(float amax) {
+  return __uint_as_float((__float_as_uint(amax * (1.0f / 6.0f)) + 0x100u) & ~0x1FFu);
+}
+
 // The half a scale code stands for, in both halves of a register.
 __device__ __forceinline__ uint32_t scale_half2(uint32_t code) { return code * 0x00800080u; }
 
@@ -72,7 +80,7 @@ __device__ __forceinline__ float2 pair_to_float2(uint32_t x) {
 // x / s is formed as x * (1 / s) and passed through half precision, which
 // makes the rounding to e2m1 exact: x has at most 11 significant bits and s
 // 4, so x / s either is a tie between two e2m1 values or is at least 1/1920
-// of it away.  The product is within 2^-23 of the quotient, so a tie becomes
+// of it away.  The product is within 2^-22 of the quotient, so a tie becomes
 // the tie itself in half (all seven ties are halves), and nothing else does
 // (half a step of half precision is less than the distance: 1/2048 of the
 // power of two below).
@@ -101,13 +109,14 @@ __device__ __forceinline__ uint32_t quantise_group(uint32_t (&x)[8], uint2 &payl
       amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
     }
   }
-  const uint32_t code = scale_code(__fdiv_rn(amax, 6.0f));
+  const uint32_t code = scale_code(sixth(amax));
   if (code == 0) {  // amax / 6 rounds to nothing
     payload = make_uint2(0, 0);
     return 0;
   }
   const __half2 s2 = *reinterpret_cast<const __half2 *>(&(const uint32_t &)scale_half2(code));
-  const float inv = __frcp_rn(__low2float(s2));
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(__low2float(s2)));
   uint32_t out[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
