@@ -170,11 +170,18 @@ __device__ __forceinline__ Cut find_cut(const AttnArgs &a) {
     const Item it = item_of<R>(a, b);
     return (int64_t)it.units * (it.blocks * a.kv_heads);
   };
+  auto scan = [&](int64_t x) {  // sum over the lanes up to this one
+#pragma unroll 1
+    for (int i = 1; i < 32; i <<= 1) {
+      const int64_t o = __shfl_up_sync(~0u, x, i);
+      if (lane >= i) x += o;
+    }
+    return x;
+  };
   Cut cut;
-  int64_t total = 0;
-  for (int b = lane; b < a.num_seqs; b += 32) total += work_of(b);
-#pragma unroll
-  for (int i = 1; i < 32; i <<= 1) total += __shfl_xor_sync(~0u, total, i);
+  int64_t mine = lane < a.num_seqs ? work_of(lane) : 0, total = mine;
+  for (int b = lane + 32; b < a.num_seqs; b += 32) total += work_of(b);
+  total = __shfl_sync(~0u, scan(total), 31);
   const int64_t want = (total + kWarps - 1) / kWarps;  // a unit for each warp, at least
   const uint32_t n = want < gridDim.x ? (uint32_t)want : gridDim.x;
   if (blockIdx.x >= n) {
@@ -188,13 +195,8 @@ __device__ __forceinline__ Cut find_cut(const AttnArgs &a) {
   // the sequence of `begin`, 32 at a time
   int64_t before = 0;
   for (int b0 = 0;; b0 += 32) {
-    const int64_t mine = b0 + lane < a.num_seqs ? work_of(b0 + lane) : 0;
-    int64_t upto = mine;
-#pragma unroll 1
-    for (int i = 1; i < 32; i <<= 1) {
-      const int64_t o = __shfl_up_sync(~0u, upto, i);
-      if (lane >= i) upto += o;
-    }
+    if (b0) mine = b0 + lane < a.num_seqs ? work_of(b0 + lane) : 0;
+    const int64_t upto = scan(mine);
     const uint32_t past = __ballot_sync(~0u, before + upto > cut.begin);
     if (past) {  // `begin` lies before the total, so this comes
       const int l = __ffs(past) - 1;
@@ -462,6 +464,27 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
       copies_commit();
     };
     next_page = page_of(in.at + lane);
+    // queries of the segment, as they lie: n = g, channels D / 4 * t on
+    uint32_t qx[NT][D / 8];
+    auto load_queries = [&] {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int r = cur.rb * R + n * 8 + g;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) qx[n][i] = 0;
+        if (r < cur.it.rows * a.group) {
+          const int i0 = r / a.group;
+          const uint8_t *p = a.q + (cur.it.first + i0) * a.q_token_stride +
+                             (cur.h * a.group + r - i0 * a.group) * a.q_head_stride + t * (D / 2);
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+            qx[n][4 * i] = v.x, qx[n][4 * i + 1] = v.y, qx[n][4 * i + 2] = v.z, qx[n][4 * i + 3] = v.w;
+          }
+        }
+      }
+    };
+    load_queries();
     take_batch();
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) issue(s);
@@ -477,27 +500,14 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
     for (;;) {  // segments
       const int h = cur.h;
       const int row0 = cur.rb * R, nrows = cur.it.rows * a.group;  // of the sequence's (token, head) rows
-      // queries, n = g, channels D / 4 * t on; multiplier and end of the rows 2 t, 2 t + 1
+      // queries in half; multiplier and end of the rows 2 t, 2 t + 1
       uint32_t qf[NT][KS][2];
       float mul[NT][2], bar[NT][2];  // bar: the sum q k past which the row's base moves
       int end[NT][2], lowest = INT32_MAX, highest = 0;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const int r = row0 + n * 8 + g;
-        uint32_t x[D / 8];
+        const uint32_t(&x)[D / 8] = qx[n];
         float amax = 0;
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) x[i] = 0;
-        if (r < nrows) {
-          const int i0 = r / a.group;
-          const uint8_t *p = a.q + (cur.it.first + i0) * a.q_token_stride +
-                             (h * a.group + r - i0 * a.group) * a.q_head_stride + t * (D / 2);
-#pragma unroll
-          for (int i = 0; i < D / 32; ++i) {
-            const uint4 v = reinterpret_cast<const uint4 *>(p)[i];
-            x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
-          }
-        }
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
           const float2 f = pair_to_float2<BF16>(x[i]);
@@ -693,6 +703,7 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
         sm.meta[warp][starts] = {1, starts, ends, h, row0, nrows, cur.it.first, unit0, unit0 + cur.it.units - 1};
       }
       if (!cur.next_segment(a)) break;
+      load_queries();
     }
   }
 
@@ -722,16 +733,23 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
     const PartMeta pm = sm.open[i];
     if (!pm.there) continue;
     const int c0 = cut.cta_of(pm.begin), n = cut.cta_of(pm.last) - c0 + 1;
-    if (threadIdx.x == 0) {
-      const bool last = arrive(arrived + c0, call) == n;
-      if (last) arrived[c0] = 0;  // for a replay of this launch
-      __threadfence();
-      sm.is_last = last;
-    }
-    __syncthreads();
-    if (sm.is_last) {
-      // a warp gathers every kWarps-th CTA's slot, 8 rows at a time, into its part
-      const int groups = min(n, kWarps);
+    auto slot_of = [&](int k) { return slots + (int64_t)(2 * (c0 + k) + (k == 0)) * slot_floats<D>(R); };
+    // Whether this CTA is the last of `count` at a word; the word is left at 0 for a replay of this launch.
+    auto last_of = [&](unsigned long long *word, int count) {
+      if (threadIdx.x == 0) {
+        const bool last = arrive(word, call) == count;
+        if (last) *word = 0;
+        __threadfence();
+        sm.is_last = last;
+      }
+      __syncthreads();
+      const bool last = sm.is_last;
+      __syncthreads();
+      return last;
+    };
+    // Joins the slots k0, k0 + step, ...: a warp gathers every kWarps-th, 8 rows at a time, into its part.
+    auto join_slots = [&](int k0, int step, int count, float *to) {
+      const int groups = min(count, kWarps);
       if (warp < groups) {
         Part<D, NT> &mine = sm.part[warp];
         for (int n8 = 0; n8 < NT; ++n8) {
@@ -740,19 +758,24 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
           float acc[8 / kRows][4], M[8 / kRows], L[8 / kRows];
 #pragma unroll
           for (int r = 0; r < 8 / kRows; ++r) M[r] = kNone, L[r] = 0, acc[r][0] = acc[r][1] = acc[r][2] = acc[r][3] = 0;
-#pragma unroll 2
-          for (int k = warp; k < n; k += kWarps) {
-            const float *slot = slots + (int64_t)(2 * (c0 + k) + (k == 0)) * slot_floats<D>(R);
+#pragma unroll 1
+          for (int k = warp; k < count; k += kWarps) {
+            const float *slot = slot_of(k0 + k * step);
+            float2 ml[8 / kRows];
+            float4 v[8 / kRows];
 #pragma unroll
             for (int r = 0; r < 8 / kRows; ++r) {
               const int rr = n8 * 8 + r * kRows + lane / kLanes;
-              const float2 ml = __ldcg(reinterpret_cast<const float2 *>(slot + R * D + 2 * rr));
-              const float4 v = __ldcg(reinterpret_cast<const float4 *>(slot + rr * D + c));
-              const float to = fmaxf(M[r], ml.x), f = exp2_fast(M[r] - to), y = exp2_fast(ml.x - to);
-              M[r] = to;
-              L[r] = L[r] * f + ml.y * y;
-              acc[r][0] = acc[r][0] * f + v.x * y, acc[r][1] = acc[r][1] * f + v.y * y;
-              acc[r][2] = acc[r][2] * f + v.z * y, acc[r][3] = acc[r][3] * f + v.w * y;
+              ml[r] = __ldcg(reinterpret_cast<const float2 *>(slot + R * D + 2 * rr));
+              v[r] = __ldcg(reinterpret_cast<const float4 *>(slot + rr * D + c));
+            }
+#pragma unroll
+            for (int r = 0; r < 8 / kRows; ++r) {
+              const float m = fmaxf(M[r], ml[r].x), f = exp2_fast(M[r] - m), y = exp2_fast(ml[r].x - m);
+              M[r] = m;
+              L[r] = L[r] * f + ml[r].y * y;
+              acc[r][0] = acc[r][0] * f + v[r].x * y, acc[r][1] = acc[r][1] * f + v[r].y * y;
+              acc[r][2] = acc[r][2] * f + v[r].z * y, acc[r][3] = acc[r][3] * f + v[r].w * y;
             }
           }
 #pragma unroll
@@ -764,9 +787,20 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
         }
       }
       __syncthreads();
-      join_parts<D, NT, BF16>(a, sm, 0, false, groups, pm, nullptr);
+      join_parts<D, NT, BF16>(a, sm, 0, false, groups, pm, to);
+      __threadfence();
+      __syncthreads();
+    };
+    // More than a slot a warp: the CTAs join them in groups first, so that no CTA has to read them all.
+    int step = 1, count = n;
+    if (n > kWarps) {
+      const int k0 = (blockIdx.x - c0) / kWarps * kWarps, size = min(kWarps, n - k0);
+      // by slot: a CTA can end one of these and start another
+      if (!last_of(arrived + gridDim.x + 2 * (c0 + k0) + (k0 == 0), size)) continue;
+      join_slots(k0, 1, size, slot_of(k0));
+      step = kWarps, count = (n + kWarps - 1) / kWarps;
     }
-    __syncthreads();
+    if (last_of(arrived + c0, count)) join_slots(0, step, count, nullptr);
   }
 }
 
@@ -1321,7 +1355,7 @@ unsigned long long next_call() {
 
 template <int D, int NT>
 int64_t decode_workspace(int ctas) {
-  return (int64_t)ctas * 2 * slot_floats<D>(8 * NT) * 4 + (int64_t)ctas * 8;
+  return (int64_t)ctas * 2 * slot_floats<D>(8 * NT) * 4 + (int64_t)ctas * 3 * 8;
 }
 int64_t decode_workspace(int D, int nt, int ctas) {
   return D == 128 ? (nt == 1 ? decode_workspace<128, 1>(ctas) : nt == 2 ? decode_workspace<128, 2>(ctas) : decode_workspace<128, 4>(ctas))
