@@ -112,8 +112,8 @@ __device__ __forceinline__ void store_row(const AttnArgs &a, int64_t first, int 
 template <int NT>
 struct DecodeShape {
   static constexpr int kWarps = NT == 1 ? 12 : NT == 2 ? 8 : 4;
-  static constexpr int kUps = 2;
-  static constexpr int kStages = NT == 4 ? 4 : 3;
+  static constexpr int kUps = NT == 4 ? 1 : 2;
+  static constexpr int kStages = NT == 4 ? 8 : 3;
 };
 
 constexpr float kNone = -1e30f;  // a row's base before any key
@@ -259,6 +259,11 @@ struct Walk {
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void copy16(uint32_t dst, const uint8_t *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy16_if(uint32_t dst, const uint8_t *src, bool on) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %2, 0;\n @p cp.async.cg.shared.global [%0], [%1], 16;\n}" ::"r"(dst), "l"(src),
+               "r"((int)on)
+               : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -443,10 +448,11 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
               copy16(dst + i * 512, src + i * 512);
               copy16(dst + kUnit + i * 512, srcv + i * 512);
             }
-            if (lane < kUnit % 512 / 16) {
-              copy16(dst + kUnit / 512 * 512, src + kUnit / 512 * 512);
-              copy16(dst + kUnit + kUnit / 512 * 512, srcv + kUnit / 512 * 512);
-            }
+            // what is left of both sides goes together, V's by the lanes after K's
+            constexpr int kFull = kUnit / 512 * 512, kRest = (kUnit - kFull) / 16;
+            static_assert(2 * kRest <= 32, "the rests of both sides are one copy");
+            const bool isv = lane >= kRest;
+            copy16_if(dst + kFull + (isv ? kUnit - kRest * 16 : 0), (isv ? srcv - kRest * 16 : src) + kFull, lane < 2 * kRest);
           }
         }
         valid = (valid & ~(((1u << kUps) - 1) << (kUps * stage))) | (mask << (kUps * stage));
@@ -557,65 +563,87 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
         l[n][0] = l[n][1] = 0;
       }
 
-      auto unit = [&](uint32_t slot, int base, bool there) {
-        float s[NT][4];
-        uint32_t w[2][KW], sc[2][(D + 127) / 128 * 2];
+      for (; cur.has_chunk(); cur.next_chunk()) {
+        const uint32_t ok = (valid >> (kUps * stage)) & ((1u << kUps) - 1);
+        copies_wait<kStages - 2>();
+        __syncwarp();  // the chunk is there, and every lane is done with the one before, whose slot is the next to fill
+        const uint32_t slot = ring + stage * kSlot;
+        issue(stage == 0 ? kStages - 1 : stage - 1);
+        // The units of the chunk together: their chains of products overlap.  One that is not there (past the
+        // segment, or its page outside the pool) is all hidden, whatever its place holds.
+        float s[kUps][NT][4];
+        uint32_t vw[kUps][4][VB / 4], vc[kUps][4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          load_shared(w[i], slot + at_k + 8 * i * (D / 2));
-          const uint32_t c = load_scales<D / 64>(slot + at_ks + 8 * i * (D / 16));
-          sc[i][0] = __byte_perm(c, 0, 0x0404) >> 1;
-          if constexpr (D == 128) sc[i][1] = __byte_perm(c, 0, 0x1414) >> 1;
-        }
-        // V^T: lane g takes channels D / 8 * g on, of the tokens of rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-        uint32_t vw[4][VB / 4], vc[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          load_shared(vw[i], slot + at_v[i & 1] + 8 * (i >> 1) * (D / 2));
-          vc[i] = load_scales<1>(slot + at_vs[i & 1] + 8 * (i >> 1) * (D / 16));
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[n][i] = 0;
-#pragma unroll
-        for (int j = 0; j < KW; ++j) {
-          uint32_t x[2][4];
+        for (int u = 0; u < kUps; ++u) {
+          const uint32_t at = slot + u * 2 * kUnit;
+          uint32_t w[2][KW], sc[2][(D + 127) / 128 * 2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            e2m1x8_to_half2(w[i][j], x[i]);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) x[i][k] = hmul2(x[i][k], sc[i][D == 128 ? j / 2 : 0]);
+            load_shared(w[i], at + at_k + 8 * i * (D / 2));
+            const uint32_t c = load_scales<D / 64>(at + at_ks + 8 * i * (D / 16));
+            sc[i][0] = __byte_perm(c, 0, 0x0404) >> 1;
+            if constexpr (D == 128) sc[i][1] = __byte_perm(c, 0, 0x1414) >> 1;
           }
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const uint32_t f[4] = {x[0][2 * k], x[1][2 * k], x[0][2 * k + 1], x[1][2 * k + 1]};
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma(s[n], f, qf[n][2 * j + k][0], qf[n][2 * j + k][1]);
-          }
-        }
-        if (!there || base + 16 > lowest) {  // hidden scores to -inf
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (!there || base + tok + 8 * (i >> 1) >= end[n][i & 1]) s[n][i] = -INFINITY;
-          // what no row sees may be anything: its scale counts as zero
+            for (int i = 0; i < 4; ++i) s[u][n][i] = 0;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (!there || base + tk[i & 1] + 8 * (i >> 1) >= highest) vc[i] = 0;
+          for (int j = 0; j < KW; ++j) {
+            uint32_t x[2][4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              e2m1x8_to_half2(w[i][j], x[i]);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) x[i][k] = hmul2(x[i][k], sc[i][D == 128 ? j / 2 : 0]);
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const uint32_t f[4] = {x[0][2 * k], x[1][2 * k], x[0][2 * k + 1], x[1][2 * k + 1]};
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma(s[u][n], f, qf[n][2 * j + k][0], qf[n][2 * j + k][1]);
+            }
+          }
+          // V^T: lane g takes channels D / 8 * g on, of the tokens of rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            load_shared(vw[u][i], at + at_v[i & 1] + 8 * (i >> 1) * (D / 2));
+            vc[u][i] = load_scales<1>(at + at_vs[i & 1] + 8 * (i >> 1) * (D / 16));
+          }
         }
+        const int base = cur.at * 16;
+        if (ok != (1u << kUps) - 1 || base + kUps * 16 > lowest) {  // hidden scores to -inf
+#pragma unroll
+          for (int u = 0; u < kUps; ++u) {
+            const bool there = (ok >> u) & 1;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (!there || base + 16 * u + tok + 8 * (i >> 1) >= end[n][i & 1]) s[u][n][i] = -INFINITY;
+            // what no row sees may be anything: its scale counts as zero
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (!there || base + 16 * u + tk[i & 1] + 8 * (i >> 1) >= highest) vc[u][i] = 0;
+          }
+        }
+        float top[NT][2];
         bool grow = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) grow |= fmaxf(s[n][i], s[n][i + 2]) > bar[n][i];
+          for (int i = 0; i < 2; ++i) {
+            top[n][i] = fmaxf(s[0][n][i], s[0][n][i + 2]);
+#pragma unroll
+            for (int u = 1; u < kUps; ++u) top[n][i] = fmaxf(top[n][i], fmaxf(s[u][n][i], s[u][n][i + 2]));
+            grow |= top[n][i] > bar[n][i];
+          }
         if (__any_sync(~0u, grow)) {  // rare after the first units
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              float x = fmaxf(s[n][j], s[n][j + 2]);
+              float x = top[n][j];
 #pragma unroll
               for (int i = 4; i < 32; i <<= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, i));
               if (x > bar[n][j]) {  // others stay: a row does not depend on its neighbours
@@ -628,46 +656,38 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
               }
             }
         }
-        uint32_t p[NT][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int u = 0; u < kUps; ++u) {
+          uint32_t p[NT][2];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float x = exp2_fast(fmaf(s[n][2 * i], mul[n][0], -m[n][0]));
-            const float y = exp2_fast(fmaf(s[n][2 * i + 1], mul[n][1], -m[n][1]));
-            l[n][0] += x, l[n][1] += y;
-            p[n][i] = transpose8(pack_half2(x, y));
-          }
-        const uint32_t vs[2] = {(vc[0] << 7) | (vc[1] << 23), (vc[2] << 7) | (vc[3] << 23)};
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int j = 0; j < VB / 4; ++j) {
-          uint32_t x[2][2][4];  // token pair, channel parity, channel pair
+            for (int i = 0; i < 2; ++i) {
+              const float x = exp2_fast(fmaf(s[u][n][2 * i], mul[n][0], -m[n][0]));
+              const float y = exp2_fast(fmaf(s[u][n][2 * i + 1], mul[n][1], -m[n][1]));
+              l[n][0] += x, l[n][1] += y;
+              p[n][i] = transpose8(pack_half2(x, y));
+            }
+          const uint32_t vs[2] = {(vc[u][0] << 7) | (vc[u][1] << 23), (vc[u][2] << 7) | (vc[u][3] << 23)};
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t w0 = vw[2 * i][j], w1 = vw[2 * i + 1][j];
-            e2m1x8_to_half2((w0 & 0x0F0F0F0Fu) | ((w1 << 4) & 0xF0F0F0F0u), x[i][0]);
-            e2m1x8_to_half2(((w0 >> 4) & 0x0F0F0F0Fu) | (w1 & 0xF0F0F0F0u), x[i][1]);
+          for (int j = 0; j < VB / 4; ++j) {
+            uint32_t x[2][2][4];  // token pair, channel parity, channel pair
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[i][0][k] = hmul2(x[i][0][k], vs[i]), x[i][1][k] = hmul2(x[i][1][k], vs[i]);
-          }
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t w0 = vw[u][2 * i][j], w1 = vw[u][2 * i + 1][j];
+              e2m1x8_to_half2((w0 & 0x0F0F0F0Fu) | ((w1 << 4) & 0xF0F0F0F0u), x[i][0]);
+              e2m1x8_to_half2(((w0 >> 4) & 0x0F0F0F0Fu) | (w1 & 0xF0F0F0F0u), x[i][1]);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t f[4] = {x[0][0][k], x[0][1][k], x[1][0][k], x[1][1][k]};
+              for (int k = 0; k < 4; ++k) x[i][0][k] = hmul2(x[i][0][k], vs[i]), x[i][1][k] = hmul2(x[i][1][k], vs[i]);
+            }
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma(o[n][4 * j + k], f, p[n][0], p[n][1]);
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t f[4] = {x[0][0][k], x[0][1][k], x[1][0][k], x[1][1][k]};
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma(o[n][4 * j + k], f, p[n][0], p[n][1]);
+            }
           }
         }
-      };
-
-      for (; cur.has_chunk(); cur.next_chunk()) {
-        const uint32_t ok = valid >> (kUps * stage);
-        const int units = cur.chunk_units();
-        copies_wait<kStages - 2>();
-        __syncwarp();  // the chunk is there, and every lane is done with the one before, whose slot is the next to fill
-        issue(stage == 0 ? kStages - 1 : stage - 1);
-#pragma unroll 1
-        for (int u = 0; u < units; ++u)
-          unit(ring + stage * kSlot + u * 2 * kUnit, (cur.at + u) * 16, (ok >> u) & 1);
         if (++stage == kStages) stage = 0;
       }
 
