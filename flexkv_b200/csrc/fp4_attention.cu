@@ -111,9 +111,8 @@ __device__ __forceinline__ void store_row(const AttnArgs &a, int64_t first, int 
 // Warps of a CTA, units of a chunk and chunks of a warp's ring, for NT row tiles.
 template <int NT>
 struct DecodeShape {
-  static constexpr int kWarps = NT == 1 ? 12 : NT == 2 ? 8 : 4;
-  static constexpr int kUps = NT == 4 ? 1 : 2;
-  static constexpr int kStages = NT == 4 ? 8 : 3;
+  static constexpr int kWarps = NT == 1 ? 12 : 8;
+  static constexpr int kUps = 2, kStages = 3;
 };
 
 constexpr float kNone = -1e30f;  // a row's base before any key
@@ -987,56 +986,68 @@ __device__ __forceinline__ void tmem_wait_load(uint32_t (&r)[32]) {
 }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-template <int D, bool BF16>
-__global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_constant__ AttnArgs a) {
-  constexpr int R = kTiles * 128;
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  auto &sm = *reinterpret_cast<ManySmem<D> *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = blockIdx.x % a.kv_heads, at = blockIdx.x / a.kv_heads;  // a block's heads run together
-
-  // The sequence and its block of rows.  The last blocks of a sequence have most keys, so they come first; with up
-  // to 32 sequences the last of each come before the second last of any.
-  int b = -1, rb = 0;
-  Item it;
+// Block `at` of R rows, of at most `blocks`: its sequence and its place there.
+// The last blocks of a sequence have most keys, so they come first; with up to
+// 32 sequences the last of each come before the second last of any.
+template <int R>
+__device__ __forceinline__ bool find_block(const AttnArgs &a, int at, int blocks, int &b, int &rb) {
+  const int lane = threadIdx.x & 31;
   if (a.num_seqs <= 32) {
-    const int want = at, blocks = lane < a.num_seqs ? item_of<R>(a, lane).blocks : 0;
-    int lo = 0, hi = __reduce_max_sync(~0u, blocks);  // the depth d with sum min(blocks, d) <= want < that of d + 1
-    if (want >= __reduce_add_sync(~0u, blocks)) return;  // the grid is an upper bound
+    const int mine = lane < a.num_seqs ? item_of<R>(a, lane).blocks : 0;
+    int lo = 0, hi = __reduce_max_sync(~0u, mine);  // the depth d with sum min(mine, d) <= at < that of d + 1
+    if (at >= (int)__reduce_add_sync(~0u, mine)) return false;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if ((int)__reduce_add_sync(~0u, min(blocks, mid)) <= want)
+      if ((int)__reduce_add_sync(~0u, min(mine, mid)) <= at)
         lo = mid;
       else
         hi = mid;
     }
-    const int nth = want - (int)__reduce_add_sync(~0u, min(blocks, lo));
-    const uint32_t have = __ballot_sync(~0u, blocks > lo);
-    b = (int)__fns(have, 0, nth + 1);
-    rb = __shfl_sync(~0u, blocks, b) - 1 - lo;
-  } else {
-    const int want = gridDim.x / a.kv_heads - 1 - at;
-    int before = 0;
-    for (int b0 = 0; b0 < a.num_seqs; b0 += 32) {
-      const int mine = b0 + lane < a.num_seqs ? item_of<R>(a, b0 + lane).blocks : 0;
-      int upto = mine;
-#pragma unroll 1
-      for (int i = 1; i < 32; i <<= 1) {
-        const int o = __shfl_up_sync(~0u, upto, i);
-        if (lane >= i) upto += o;
-      }
-      const uint32_t past = __ballot_sync(~0u, before + upto > want);
-      if (past) {
-        const int l = __ffs(past) - 1;
-        b = b0 + l;
-        rb = want - before - __shfl_sync(~0u, upto - mine, l);
-        break;
-      }
-      before += __shfl_sync(~0u, upto, 31);
-    }
-    if (b < 0) return;
+    const int nth = at - (int)__reduce_add_sync(~0u, min(mine, lo));
+    b = (int)__fns(__ballot_sync(~0u, mine > lo), 0, nth + 1);
+    rb = __shfl_sync(~0u, mine, b) - 1 - lo;
+    return true;
   }
-  it = item_of<R>(a, b);
+  const int want = blocks - 1 - at;
+  int before = 0;
+  for (int b0 = 0; b0 < a.num_seqs; b0 += 32) {
+    const int mine = b0 + lane < a.num_seqs ? item_of<R>(a, b0 + lane).blocks : 0;
+    int upto = mine;
+#pragma unroll 1
+    for (int i = 1; i < 32; i <<= 1) {
+      const int o = __shfl_up_sync(~0u, upto, i);
+      if (lane >= i) upto += o;
+    }
+    const uint32_t past = __ballot_sync(~0u, before + upto > want);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      b = b0 + l;
+      rb = want - before - __shfl_sync(~0u, upto - mine, l);
+      return true;
+    }
+    before += __shfl_sync(~0u, upto, 31);
+  }
+  return false;
+}
+
+// A row's share of the workspace where the keys are split: its sums, then base
+// and sum of weights.
+template <int D>
+__host__ __device__ constexpr int split_floats() { return kTiles * 128 * (D + 2); }
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kManyThreads, 1)
+fp4_many_kernel(const __grid_constant__ AttnArgs a, int blocks, int splits, float *__restrict__ parts) {
+  constexpr int R = kTiles * 128;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  auto &sm = *reinterpret_cast<ManySmem<D> *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // a block's heads, and the parts of its keys, run together
+  const int h = blockIdx.x % a.kv_heads, of = blockIdx.x / a.kv_heads, at = of / splits, split = of - at * splits;
+
+  int b, rb;
+  if (!find_block<R>(a, at, blocks, b, rb)) return;  // the grid is an upper bound
+  const Item it = item_of<R>(a, b);
   const int row0 = rb * R, nrows = it.rows * a.group;
   const int tiles = nrows - row0 > 128 ? 2 : 1;
   auto end_of = [&](int row) {  // the keys that a row sees
@@ -1045,7 +1056,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
     return e;
   };
   const int most = end_of(min(nrows - 1, row0 + R - 1));
-  const int chunks = (most + kKeys - 1) / kKeys;
+  const int all = (most + kKeys - 1) / kKeys;
+  const int chunk0 = (int)((int64_t)all * split / splits), chunks = (int)((int64_t)all * (split + 1) / splits) - chunk0;
 
   if (threadIdx.x == 0) {
     mbar_init(&sm.q_full, 128 * tiles);
@@ -1119,12 +1131,13 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
         tmem_load32(x[0], S), tmem_load32(x[1], S + 32);
         const uint32_t bad = *(volatile uint32_t *)sm.bad[j & (2 * kRing - 1)];
         tmem_wait_load(x[0]), tmem_wait_load(x[1]);
-        if ((j + 1) * kKeys > lowest || bad) {  // only what the row sees
+        const int key0 = (chunk0 + j) * kKeys;
+        if (key0 + kKeys > lowest || bad) {  // only what the row sees
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (j * kKeys + 32 * c + i >= end || ((bad >> (8 * (2 * c + i / 16))) & 1)) x[c][i] = 0xFF800000u;
+              if (key0 + 32 * c + i >= end || ((bad >> (8 * (2 * c + i / 16))) & 1)) x[c][i] = 0xFF800000u;
         }
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -1186,7 +1199,22 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
         fence_after();
       }
       const int tok_head = h * a.group + row - i0 * a.group;
-      const float sum = (l[0] + l[1]) + (l[2] + l[3]), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const float sum = (l[0] + l[1]) + (l[2] + l[3]);
+      if (splits > 1) {  // for the kernel below to join
+        float *part = parts + (int64_t)blockIdx.x * split_floats<D>(), *o = part + (t * 128 + r) * D;
+        if (chunks) {
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t x[16];
+            tmem_load16(x, o_at(t) + lanes + 16 * c);
+            tmem_wait_load(x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) reinterpret_cast<uint4 *>(o)[4 * c + i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+          }
+        }
+        reinterpret_cast<float2 *>(part + kTiles * 128 * D)[t * 128 + r] = make_float2(base, sum);
+      } else {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
       uint8_t *dst = a.out + (it.first + i0) * a.o_token_stride + tok_head * a.o_head_stride;
 #pragma unroll 1
       for (int c = 0; c < D / 16; ++c) {
@@ -1213,6 +1241,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
         }
       }
       if (a.lse && valid) a.lse[(it.first + i0) * (a.kv_heads * a.group) + tok_head] = natural_lse(base, sum);
+      }
     }
   } else if (warp < 4 * kTiles + kFillWarps) {
     // ---- K and V into shared memory ----
@@ -1228,7 +1257,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
       at_chunk[k] = (c >> 3) * ManySmem<D>::kCols + w * 16 * 128 + tok * 128 + ((c & 7) ^ tok) * 16;
     }
     auto page_of = [&](int j) {
-      const int u = j * (kKeys / 16) + w, e = (int)(((uint64_t)u * a.upb_magic) >> 40);
+      const int u = (chunk0 + j) * (kKeys / 16) + w, e = (int)(((uint64_t)u * a.upb_magic) >> 40);
       return u * 16 < most && e < a.max_blocks ? a.tables[b * a.table_stride + e] : -1;
     };
     uint32_t x[2][2][kWords], sc[2][2];  // pieces of K and of V of a chunk, on their way
@@ -1236,7 +1265,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
     int page;
     uint32_t bad = 0;
     auto find = [&](int j) {  // the unit of chunk j, and the page of the chunk after it
-      const int u = j * (kKeys / 16) + w, e = (int)(((uint64_t)u * a.upb_magic) >> 40);
+      const int u = (chunk0 + j) * (kKeys / 16) + w, e = (int)(((uint64_t)u * a.upb_magic) >> 40);
       const bool good = page >= 0 && page < a.num_blocks;
       unit = good ? a.layer + page * a.block_stride + ((int64_t)h * a.upb + u - e * a.upb) * (9 * D) : nullptr;
       bad = !good && u * 16 < most;
@@ -1258,7 +1287,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
             x[side][i][0] = y.x, x[side][i][1] = y.y;
           }
           const uint8_t *q = p + at_scale + i * 8 * (D / 16);
-          if (j * kKeys + w * 16 + i * 8 + tok < most)
+          if ((chunk0 + j) * kKeys + w * 16 + i * 8 + tok < most)
             sc[side][i] = D == 128 ? __ldg(reinterpret_cast<const uint16_t *>(q)) : __ldg(q);
         }
       }
@@ -1361,6 +1390,47 @@ __global__ void __launch_bounds__(kManyThreads, 1) fp4_many_kernel(const __grid_
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
+// Joins the parts of the keys that the kernel above has split: a warp for each
+// row, in the parts' order.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) fp4_merge_kernel(const __grid_constant__ AttnArgs a, int blocks, int splits,
+                                                        const float *__restrict__ parts) {
+  constexpr int R = kTiles * 128, kVec = D / 32;  // floats of a lane
+  const int h = blockIdx.x % a.kv_heads, at = blockIdx.x / a.kv_heads, lane = threadIdx.x & 31;
+  const int r = blockIdx.y * 8 + (threadIdx.x >> 5);
+  int b, rb;
+  if (!find_block<R>(a, at, blocks, b, rb)) return;
+  const Item it = item_of<R>(a, b);
+  const int row = rb * R + r, nrows = it.rows * a.group;
+  if (row >= nrows) return;
+  float M = kNone, L = 0, acc[kVec] = {};
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const float *part = parts + ((int64_t)(at * splits + s) * a.kv_heads + h) * split_floats<D>();
+    const float2 ml = reinterpret_cast<const float2 *>(part + R * D)[r];
+    float v[kVec] = {};
+    if (ml.y != 0.0f) {  // a part without keys has no sums
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) v[i] = part[r * D + lane * kVec + i];
+    }
+    const float to = fmaxf(M, ml.x), f = exp2_fast(M - to), y = exp2_fast(ml.x - to);
+    M = to, L = L * f + ml.y * y;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) acc[i] = acc[i] * f + v[i] * y;
+  }
+  const int i0 = row / a.group, qh = h * a.group + row - i0 * a.group;
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  uint8_t *dst = a.out + (it.first + i0) * a.o_token_stride + qh * a.o_head_stride + lane * kVec * 2;
+#pragma unroll
+  for (int i = 0; i < kVec; i += 2) {
+    if (BF16)
+      reinterpret_cast<__nv_bfloat162 *>(dst)[i / 2] = __floats2bfloat162_rn(acc[i] * inv, acc[i + 1] * inv);
+    else
+      reinterpret_cast<uint32_t *>(dst)[i / 2] = pack_half2(acc[i] * inv, acc[i + 1] * inv);
+  }
+  if (a.lse && lane == 0) a.lse[(it.first + i0) * (a.kv_heads * a.group) + qh] = natural_lse(M, L);
+}
+
 // A number of 48 bits for each launch, from a start that differs between processes.
 unsigned long long next_call() {
   static std::atomic<unsigned long long> last{[] {
@@ -1378,8 +1448,8 @@ int64_t decode_workspace(int ctas) {
   return (int64_t)ctas * 2 * slot_floats<D>(8 * NT) * 4 + (int64_t)ctas * 3 * 8;
 }
 int64_t decode_workspace(int D, int nt, int ctas) {
-  return D == 128 ? (nt == 1 ? decode_workspace<128, 1>(ctas) : nt == 2 ? decode_workspace<128, 2>(ctas) : decode_workspace<128, 4>(ctas))
-                  : (nt == 1 ? decode_workspace<64, 1>(ctas) : nt == 2 ? decode_workspace<64, 2>(ctas) : decode_workspace<64, 4>(ctas));
+  if (D == 128) return nt == 1 ? decode_workspace<128, 1>(ctas) : decode_workspace<128, 2>(ctas);
+  return nt == 1 ? decode_workspace<64, 1>(ctas) : decode_workspace<64, 2>(ctas);
 }
 
 template <int D, int NT, bool BF16>
@@ -1396,31 +1466,52 @@ int launch_decode(const AttnArgs &a, int ctas, void *workspace, cudaStream_t s) 
 }
 template <int D, bool BF16>
 int launch_decode(const AttnArgs &a, int nt, int ctas, void *workspace, cudaStream_t s) {
-  switch (nt) {
-    case 1: return launch_decode<D, 1, BF16>(a, ctas, workspace, s);
-    case 2: return launch_decode<D, 2, BF16>(a, ctas, workspace, s);
-    default: return launch_decode<D, 4, BF16>(a, ctas, workspace, s);
-  }
+  return nt == 1 ? launch_decode<D, 1, BF16>(a, ctas, workspace, s) : launch_decode<D, 2, BF16>(a, ctas, workspace, s);
+}
+
+// Launch of the many-rows kernel: a bound of the blocks of rows (the sequences'
+// lengths are on the device), and how many CTAs share a block's keys.
+struct ManyPlan {
+  int64_t blocks;
+  int splits;
+};
+ManyPlan many_plan(int64_t num_q, int group, int kv_heads, int num_seqs, int max_q_len, int sms) {
+  constexpr int R = kTiles * 128;
+  ManyPlan p{num_q * group / R + num_seqs, 1};
+  // as many CTAs as there are SMs where the blocks, by the lengths as told, are fewer; wrong ones cost time only
+  const int64_t told = std::min(p.blocks, (int64_t)num_seqs * (((int64_t)max_q_len * group + R - 1) / R)) * kv_heads;
+  if (told > 0)
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({sms / told, 4 * sms / (p.blocks * kv_heads), 64}));
+  return p;
+}
+int64_t many_workspace(int D, const ManyPlan &p, int kv_heads) {
+  return p.splits == 1 ? 0 : p.blocks * p.splits * kv_heads * 4 * (D == 128 ? split_floats<128>() : split_floats<64>());
 }
 
 template <int D, bool BF16>
-int launch_many(const AttnArgs &a, cudaStream_t s) {
+int launch_many(const AttnArgs &a, const ManyPlan &p, void *workspace, cudaStream_t s) {
   const int smem = sizeof(ManySmem<D>) + 1024;
   auto kernel = fp4_many_kernel<D, BF16>;
   FKV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  // a bound of the blocks of rows: the sequences' lengths are on the device
-  const int64_t blocks = a.num_q * a.group / (kTiles * 128) + a.num_seqs;
-  if (blocks * a.kv_heads > INT32_MAX) return fail(FKV_ERR_INVALID_ARG, "fkv_fp4_attention: 2^31 blocks of rows or more");
-  kernel<<<(unsigned)(blocks * a.kv_heads), kManyThreads, smem, s>>>(a);
+  if (p.blocks * a.kv_heads * p.splits > INT32_MAX)
+    return fail(FKV_ERR_INVALID_ARG, "fkv_fp4_attention: 2^31 blocks of rows or more");
+  kernel<<<(unsigned)(p.blocks * a.kv_heads * p.splits), kManyThreads, smem, s>>>(a, (int)p.blocks, p.splits, (float *)workspace);
   FKV_CUDA(cudaGetLastError());
   note_launch();
+  if (p.splits > 1) {
+    fp4_merge_kernel<D, BF16><<<dim3((unsigned)(p.blocks * a.kv_heads), kTiles * 128 / 8), 256, 0, s>>>(
+        a, (int)p.blocks, p.splits, (const float *)workspace);
+    FKV_CUDA(cudaGetLastError());
+    note_launch();
+  }
   return FKV_OK;
 }
 
-constexpr int kFewRows = 64;  // rows of a key head up to which the few-rows kernel runs
-
-// Tiles of 8 rows that go through the cache together.
-int row_tiles(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
+// Rows of a key head up to which the few-rows kernel runs, 16 at a time.  16
+// sequences of 4000 tokens, 8 key heads of 128: 32 rows 62 us there and 82 us in
+// the many-rows kernel (64 sequences: 176 and 315 us), 64 rows 100 and 82 us.
+constexpr int kFewRows = 32;
+int row_tiles(int64_t rows) { return rows <= 8 ? 1 : 2; }
 
 }  // namespace
 }  // namespace fkv
@@ -1433,7 +1524,9 @@ int64_t fkv_fp4_attention_workspace(int64_t num_q_tokens, int num_q_heads, int n
                                     int max_q_len) {
   ThreadDeviceCtx *ctx;
   if (num_kv_heads <= 0 || get_ctx(-1, &ctx) != FKV_OK) return 0;
-  if ((int64_t)max_q_len * (num_q_heads / num_kv_heads) > kFewRows) return 0;
+  const int group = num_q_heads / num_kv_heads;
+  if ((int64_t)max_q_len * group > kFewRows)
+    return many_workspace(head_size, many_plan(num_q_tokens, group, num_kv_heads, num_seqs, max_q_len, ctx->num_sms), num_kv_heads);
   return decode_workspace(head_size, row_tiles((int64_t)max_q_len * (num_q_heads / num_kv_heads)), ctx->num_sms);
 }
 
@@ -1483,8 +1576,12 @@ int fkv_fp4_attention(const void *layer, int64_t num_blocks, int tokens_per_bloc
   cudaStream_t s = (cudaStream_t)stream;
   const bool bf16 = dtype == FKV_DTYPE_BF16;
   if ((int64_t)max_q_len * a.group > kFewRows) {
-    if (head_size == 128) return bf16 ? launch_many<128, true>(a, s) : launch_many<128, false>(a, s);
-    return bf16 ? launch_many<64, true>(a, s) : launch_many<64, false>(a, s);
+    const ManyPlan p = many_plan(num_q_tokens, a.group, num_kv_heads, num_seqs, max_q_len, ctx->num_sms);
+    const int64_t need = many_workspace(head_size, p, num_kv_heads);
+    if (need && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need))
+      return bad("the workspace is too small or not aligned");
+    if (head_size == 128) return bf16 ? launch_many<128, true>(a, p, workspace, s) : launch_many<128, false>(a, p, workspace, s);
+    return bf16 ? launch_many<64, true>(a, p, workspace, s) : launch_many<64, false>(a, p, workspace, s);
   }
   const int nt = row_tiles((int64_t)max_q_len * a.group);
   if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < decode_workspace(head_size, nt, ctx->num_sms))
