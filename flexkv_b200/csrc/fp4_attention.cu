@@ -874,12 +874,13 @@ __device__ __forceinline__ bool mbar_try(uint64_t *m, int parity) {
       : "memory");
   return ok;
 }
-// A wait has a limit (a try lasts up to a millisecond by itself).  One that
-// runs out is counted and the kernel goes on as if it had come, each later wait
-// with a single try: it ends, and its output is not to be used.
+// A wait has a limit (a try lasts about a microsecond, the whole of them about
+// a second).  One that runs out is counted (fkv_fp4_wait_timeouts) and the
+// kernel goes on as if it had come, each later wait with a single try: it ends,
+// and its output is not to be used.
 __device__ unsigned long long g_wait_timeouts;
 struct Patience {
-  int tries = 2000;
+  int tries = 1 << 20;
   __device__ __forceinline__ void wait(uint64_t *m, int parity) {
     for (int i = 0; i < tries; ++i)
       if (mbar_try(m, parity)) return;
@@ -1520,6 +1521,15 @@ using namespace fkv;
 
 extern "C" {
 
+int fkv_fp4_wait_timeouts(int64_t *count) {
+  clear_error();
+  if (!count) return fail(FKV_ERR_INVALID_ARG, "fkv_fp4_wait_timeouts: null pointer");
+  unsigned long long n = 0;
+  FKV_CUDA(cudaMemcpyFromSymbol(&n, g_wait_timeouts, sizeof(n)));
+  *count = (int64_t)n;
+  return FKV_OK;
+}
+
 int64_t fkv_fp4_attention_workspace(int64_t num_q_tokens, int num_q_heads, int num_kv_heads, int head_size, int num_seqs,
                                     int max_q_len) {
   ThreadDeviceCtx *ctx;
@@ -1551,7 +1561,8 @@ int fkv_fp4_attention(const void *layer, int64_t num_blocks, int tokens_per_bloc
   if (num_blocks < 0 || num_q_tokens < 0 || num_seqs < 0 || max_blocks < 0) return bad("counts must be non-negative");
   if (!std::isfinite(softmax_scale)) return bad("softmax_scale must be finite");
   if (num_q_tokens == 0 || num_seqs == 0) return FKV_OK;
-  if (num_q_tokens * num_q_heads >= INT32_MAX) return bad("2^31 (token, head) rows or more in one call");
+  if (num_q_tokens > INT32_MAX || num_q_tokens * num_q_heads >= INT32_MAX - 65536)
+    return bad("2^31 (token, head) rows or more in one call");
   if (!q || !out || !seq_lens || (max_blocks > 0 && !block_tables) || (num_blocks > 0 && !layer)) return bad("null pointer");
   if (!cu_seqlens_q && num_q_tokens % num_seqs) return bad("without cu_seqlens_q every sequence has the same number of new tokens");
   if ((uintptr_t)layer % 16 || kv_stride_in_bytes % 16 || block_stride_in_bytes % 16 || (uintptr_t)q % 16 ||
@@ -1569,7 +1580,7 @@ int fkv_fp4_attention(const void *layer, int64_t num_blocks, int tokens_per_bloc
   a.max_blocks = max_blocks, a.seq_lens = seq_lens, a.cu = cu_seqlens_q, a.num_seqs = num_seqs;
   a.scale = softmax_scale, a.causal = causal;
   a.rows_each = (int)(num_q_tokens / num_seqs);
-  a.table_tokens = (int)std::min<int64_t>((int64_t)max_blocks * tokens_per_block, INT32_MAX - 15);
+  a.table_tokens = (int)std::min<int64_t>((int64_t)max_blocks * tokens_per_block, INT32_MAX - 255);  // positions are ints
   ThreadDeviceCtx *ctx;
   const int rc = get_ctx(-1, &ctx);
   if (rc != FKV_OK) return rc;

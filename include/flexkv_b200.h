@@ -658,8 +658,8 @@ int fkv_fp4_unpack_blocks(int num_layers, void *const *fp4_layer_ptrs, void *con
  * block block_tables[b * block_table_stride + j / tokens_per_block], of
  * max_blocks entries.  Its row i sees the keys up to position seq_lens[b] -
  * rows + i (causal != 0) or all of them.  A row that sees nothing gives zeros.
- * Tokens past the table, or in a block outside the pool, count as hidden.
- * Rows of no sequence are left as they were.  max_q_len: the most rows of a
+ * Tokens past the table (or past 2^31 - 256), or in a block outside the pool,
+ * count as hidden.  cu_seqlens_q must not decrease.  Rows of no sequence are left as they were.  max_q_len: the most rows of a
  * sequence, which only chooses the kernel.  lse (optional): float [num_q_tokens,
  * num_q_heads], the natural logarithm of the sum of exponentials, -inf for a
  * row that sees nothing.  workspace: device memory of at least
@@ -676,6 +676,12 @@ int fkv_fp4_attention(const void *layer, int64_t num_blocks, int tokens_per_bloc
                       int max_blocks, const int32_t *seq_lens, const int32_t *cu_seqlens_q,
                       int num_seqs, int max_q_len, float softmax_scale, int causal, void *workspace,
                       int64_t workspace_bytes, void *stream);
+
+/* Waits between the warps of an attention kernel that ran out of their limit
+ * (about a second) on the current device so far: 0 unless something is wrong;
+ * the output of a call that counts any is not to be used.  Waits for the
+ * device. */
+int fkv_fp4_wait_timeouts(int64_t *count);
 
 #ifdef __cplusplus
 }

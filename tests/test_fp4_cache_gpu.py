@@ -565,3 +565,68 @@ def test_order_does_not_change_results(new):
     st = decode_state(9, lens=(5000, 177, 2000), new=new)
     a = [fp4_cache.fp4_attention(*st, new) for _ in range(5)]
     assert all(torch.equal(a[0], x) for x in a)
+
+
+def test_no_wait_ran_out():
+    """After all of the above: every wait between the warps of the kernels was met."""
+    import ctypes
+    from flexkv_b200 import _lib
+    n = ctypes.c_int64(-1)
+    assert _lib.load().fkv_fp4_wait_timeouts(ctypes.byref(n)) == 0 and n.value == 0
+    assert _lib.load().fkv_fp4_wait_timeouts(None) == _lib.FKV_ERR_INVALID_ARG
+
+
+@pytest.mark.parametrize("tokens,heads,group", [(40, 2, 4), (100, 1, 8), (300, 1, 2)])
+def test_few_blocks_of_rows_over_many_keys(tokens, heads, group):
+    """The keys of a few rows' blocks split over CTAs and joined, with parts that see nothing."""
+    check_attention(heads, group, 128, 16, "bf16", [3000, 20, 0], [tokens, 20, 0])
+    check_attention(heads, group, 64, 32, "fp16", [1500, tokens], [tokens, tokens], causal=False)
+
+
+def test_more_sequences_than_lanes():
+    """Blocks of rows are found among more sequences than a warp has lanes."""
+    r = np.random.RandomState(3)
+    new = r.randint(0, 30, 45)
+    lens = new + r.randint(0, 40, 45)
+    check_attention(1, 5, 64, 16, "bf16", lens.tolist(), new.tolist())
+
+
+def test_a_head_over_every_cta():
+    """One key head's keys over all CTAs, joined in two steps; with rows of two tiles too."""
+    check_attention(1, 8, 128, 16, "bf16", [30000], [1], uniform=True)
+    check_attention(1, 8, 64, 64, "fp16", [20011, 500], [2, 2])
+
+
+def test_in_place():
+    """out may be q itself."""
+    for new in (1, 4, 100):
+        layer, q, tables, lens, cu = decode_state(3, lens=(1500, 170), new=new)
+        want = fp4_cache.fp4_attention(layer, q, tables, lens, cu, new)
+        got = q.clone()
+        fp4_cache.fp4_attention(layer, got, tables, lens, cu, new, out=got)
+        assert torch.equal(got, want)
+
+
+def test_repeated_sources_and_tables():
+    """The same page in two sequences' tables (a shared prefix), the same slot read twice."""
+    layer = torch.from_numpy(written(2, 8, 2, 16, 64, 1)).cuda()
+    tables = torch.tensor([[3, 5, 1], [3, 5, 7], [3, 5, 1]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([40, 40, 40], dtype=torch.int32, device="cuda")
+    q = torch.randn(1, 4, 64, device="cuda").bfloat16().repeat(3, 1, 1)
+    o = fp4_cache.fp4_attention(layer, q, tables, lens)
+    want, _, weight, size = M.attention(layer.cpu().numpy(), f64(q), tables.cpu().numpy(), lens.cpu().numpy(),
+                                        np.arange(4), 64 ** -0.5, True, 16)
+    assert (np.abs(f64(o) - want) <= M.attention_bounds(weight, size, want, 64, "bf16")).all()
+    slots = torch.tensor([5, 5, 100, 5], device="cuda")
+    k, v = fp4_cache.fp4_read(layer, slots)
+    assert torch.equal(k[0], k[1]) and torch.equal(v[0], v[3])
+
+
+@pytest.mark.skipif("torch.cuda.device_count() < 2")
+def test_another_device():
+    """Tensors of a device that is not the current one."""
+    torch.cuda.set_device(0)
+    layer = torch.from_numpy(written(2, 8, 2, 16, 64, 1)).to("cuda:1")
+    slots = torch.arange(40, device="cuda:1")
+    k, _ = fp4_cache.fp4_read(layer, slots)
+    assert torch.cuda.current_device() == 0 and np.array_equal(f64(k), M.held(layer.cpu().numpy())[0][:40])
