@@ -27,7 +27,9 @@ constexpr int kMaxLayers = 128;  // layers of one launch: their pointers travel 
 constexpr int kThreads = 256;
 constexpr int kUnroll = 4;
 
-struct RowsArgs {
+// LAYERS: what the call's pointers need; they are copied with every launch.
+template <int LAYERS>
+struct RowsArgsOf {
   int num_heads;
   int kv_dim;
   int tokens_per_block;
@@ -43,9 +45,11 @@ struct RowsArgs {
   int64_t row_block_stride;                        // bytes, block form
   const int64_t *fp4_ids;                          // slots (token form) or blocks
   const int64_t *row_ids;                          // blocks of the 16-bit side (block form)
-  uint8_t *fp4[kMaxLayers];
-  uint8_t *rows[2][kMaxLayers];
+  uint8_t *fp4[LAYERS];
+  uint8_t *rows[2][LAYERS];
 };
+template <bool BLOCKS>
+using RowsArgs = RowsArgsOf<BLOCKS ? kMaxLayers : 1>;
 
 // 32 bytes in one access where the address allows it, else two of 16.
 template <bool WIDE>
@@ -80,7 +84,7 @@ __device__ __forceinline__ void store_group(uint8_t *p, const uint32_t (&r)[8]) 
 // row and group through all heads and looks its slot up once.  0: at run time,
 // a place for each group.
 template <bool WRITE, bool BF16, bool BLOCKS, bool WIDE, int NG, int R>
-__global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constant__ RowsArgs a) {
+__global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constant__ RowsArgs<BLOCKS> a) {
   const int ng = NG ? NG : a.groups, D = 16 * ng;
   const int layer = a.kv_dim == 1 ? blockIdx.y : blockIdx.y >> 1, side = a.kv_dim == 1 ? 0 : blockIdx.y & 1;
   const int64_t row0 = (int64_t)blockIdx.x * R;
@@ -184,7 +188,7 @@ __global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constan
 }
 
 template <bool WRITE, bool BF16, bool BLOCKS, bool WIDE, int R>
-void launch_ng(const RowsArgs &a, dim3 grid, int ng, cudaStream_t s) {
+void launch_ng(const RowsArgs<BLOCKS> &a, dim3 grid, int ng, cudaStream_t s) {
   switch (ng) {
     case 4: fp4_rows_kernel<WRITE, BF16, BLOCKS, WIDE, 4, R><<<grid, kThreads, 0, s>>>(a); break;
     case 8: fp4_rows_kernel<WRITE, BF16, BLOCKS, WIDE, 8, R><<<grid, kThreads, 0, s>>>(a); break;
@@ -193,14 +197,14 @@ void launch_ng(const RowsArgs &a, dim3 grid, int ng, cudaStream_t s) {
   }
 }
 template <bool WRITE, bool BF16, bool BLOCKS, bool WIDE>
-void launch_r(const RowsArgs &a, int rows_at_once, dim3 grid, int ng, cudaStream_t s) {
+void launch_r(const RowsArgs<BLOCKS> &a, int rows_at_once, dim3 grid, int ng, cudaStream_t s) {
   if (BLOCKS || rows_at_once == 16)
     launch_ng<WRITE, BF16, BLOCKS, WIDE, 16>(a, grid, ng, s);
   else
     launch_ng<WRITE, BF16, BLOCKS, WIDE, BLOCKS ? 16 : 1>(a, grid, ng, s);
 }
 template <bool WRITE, bool BLOCKS>
-void launch_rows(const RowsArgs &a, bool bf16, bool wide, int r, dim3 grid, int ng, cudaStream_t s) {
+void launch_rows(const RowsArgs<BLOCKS> &a, bool bf16, bool wide, int r, dim3 grid, int ng, cudaStream_t s) {
   if (bf16)
     wide ? launch_r<WRITE, true, BLOCKS, true>(a, r, grid, ng, s) : launch_r<WRITE, true, BLOCKS, false>(a, r, grid, ng, s);
   else
@@ -225,7 +229,7 @@ bool aligned(int64_t v, int64_t to) { return v % to == 0; }
 bool aligned(const void *p, int64_t to) { return (uintptr_t)p % to == 0; }
 
 template <bool WRITE, bool BLOCKS>
-int run_rows(RowsArgs &a, int num_layers, int head_size, int dtype, bool wide, cudaStream_t s) {
+int run_rows(RowsArgs<BLOCKS> &a, int num_layers, int head_size, int dtype, bool wide, cudaStream_t s) {
   const int ng = head_size / 16, r = a.num_rows < 16 ? 1 : 16;
   a.upb = a.tokens_per_block / 16, a.groups = ng;
   a.upb_magic = ((uint64_t)1 << 40) / a.upb + 1, a.groups_magic = ((uint64_t)1 << 40) / ng + 1;
@@ -255,7 +259,7 @@ int tokens_call(const char *who, void *layer, int kv_dim, int64_t num_blocks, in
   if (kv_dim == 1 && v) return fail(FKV_ERR_INVALID_ARG, w + ": a latent layer (kv_dim 1) has no values");
   if (!aligned(layer, 16) || !aligned(kv_stride, 16) || !aligned(block_stride, 16))
     return fail(FKV_ERR_MISALIGNED, w + ": the layer and its strides must be multiples of 16 bytes");
-  RowsArgs a{};
+  RowsArgs<false> a{};
   a.num_heads = heads, a.kv_dim = kv_dim, a.tokens_per_block = tpb;
   a.num_rows = num_tokens, a.num_slots = num_blocks * tpb;
   a.fp4_kv_stride = kv_stride, a.fp4_block_stride = block_stride;
@@ -296,7 +300,7 @@ int blocks_call(const char *who, int num_layers, void *const *fp4_layers, void *
       return fail(FKV_ERR_MISALIGNED, w + ": layers must start on 16-byte boundaries");
     wide = wide && aligned(kv_layers[l], 32);
   }
-  RowsArgs a{};
+  RowsArgs<true> a{};
   a.num_heads = heads, a.kv_dim = kv_dim, a.tokens_per_block = tpb;
   a.num_rows = num * tpb, a.num_slots = fp4_num_blocks * tpb, a.num_blocks = fp4_num_blocks, a.num_row_blocks = kv_num_blocks;
   a.fp4_kv_stride = fp4_kv_stride, a.fp4_block_stride = fp4_block_stride;
