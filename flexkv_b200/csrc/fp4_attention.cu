@@ -24,7 +24,7 @@ struct AttnArgs {
   int64_t num_blocks, kv_stride, block_stride;
   int tokens_per_block, kv_heads, group;
   int upb;             // units of a block
-  uint64_t upb_magic;  // u / upb = (u * upb_magic) >> 40 for u < 2^28, upb <= 2^12
+  Divisor by_upb;      // positions are below 2^31, so a unit's number is below 2^27
   const uint8_t *q;
   int64_t q_token_stride, q_head_stride;  // bytes
   uint8_t *out;
@@ -107,12 +107,26 @@ __device__ __forceinline__ void store_row(const AttnArgs &a, int64_t first, int 
 // writes out; the rest is joined once at the end within the CTA, and pieces of
 // one (sequence, head) in several CTAs by the CTA that comes last, both in a
 // fixed order.
+//
+// Measured (B200, bfloat16, heads of 128): 48 sequences of 6000 to 16384 tokens,
+// 8 key heads, 32 query heads: 133 us for 630 MB, 4.7 TB/s, 73 % of a copy's
+// rate; what bounds it there is the issue of about 290 instructions a unit (64
+// conversions, 64 multiplications, 16 products; the read alone takes 106 us).
+// Why 12 warps, two units a stage and three stages: one unit and six stages take
+// 144 us, 16 warps with one unit and four stages 138, 8 warps with four units
+// 136, 16 warps with two stages of two 131.5 but 15.3 us instead of 13.2 for one
+// sequence of 1000 tokens (at that time).  Small calls are bound by the chain
+// launch, lengths, pages, keys, joins: that sequence 11 us, one of 131071 tokens
+// 17.4 us.
 
 // Warps of a CTA, units of a chunk and chunks of a warp's ring, for NT row tiles.
-template <int NT>
+// Heads of 64 leave registers for more: 64 sequences of 4000 tokens, 8 key heads,
+// take 50 us with 16 warps and 52 with 12 (NT 1), 63 us with 4 units a chunk and
+// 69 with 2 (NT 2).
+template <int D, int NT>
 struct DecodeShape {
-  static constexpr int kWarps = NT == 1 ? 12 : 8;
-  static constexpr int kUps = 2, kStages = 3;
+  static constexpr int kWarps = NT == 2 ? 8 : D == 64 ? 16 : 12;
+  static constexpr int kUps = NT == 2 && D == 64 ? 4 : 2, kStages = 3;
 };
 
 constexpr float kNone = -1e30f;  // a row's base before any key
@@ -346,7 +360,7 @@ struct PartMeta {
 
 template <int D, int NT>
 struct DecodeSmem {
-  static constexpr int kWarps = DecodeShape<NT>::kWarps, kUps = DecodeShape<NT>::kUps, kStages = DecodeShape<NT>::kStages;
+  static constexpr int kWarps = DecodeShape<D, NT>::kWarps, kUps = DecodeShape<D, NT>::kUps, kStages = DecodeShape<D, NT>::kStages;
   alignas(128) uint8_t ring[kWarps][kStages][kUps][2][9 * D];  // at the end: the part that starts in the warp
   Part<D, NT> part[kWarps];                                     // the part that goes on from the warp before
   PartMeta meta[kWarps][2];
@@ -364,7 +378,7 @@ __host__ __device__ constexpr int slot_floats(int rows) { return rows * (D + 2);
 template <int D, int NT, bool BF16>
 __device__ __forceinline__ void join_parts(const AttnArgs &a, const DecodeSmem<D, NT> &sm, int w0, bool ring, int count,
                                            const PartMeta &pm, float *slot) {
-  constexpr int R = 8 * NT, kWarps = DecodeShape<NT>::kWarps;
+  constexpr int R = 8 * NT, kWarps = DecodeShape<D, NT>::kWarps;
   auto part = [&](int k) -> const Part<D, NT> & {
     return k == 0 && ring ? *reinterpret_cast<const Part<D, NT> *>(sm.ring[w0]) : sm.part[w0 + k];
   };
@@ -399,11 +413,11 @@ __device__ __forceinline__ int arrive(unsigned long long *word, unsigned long lo
 }
 
 template <int D, int NT, bool BF16>
-__global__ void __launch_bounds__(DecodeShape<NT>::kWarps * 32, 1)
+__global__ void __launch_bounds__(DecodeShape<D, NT>::kWarps * 32, 1)
 fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots, unsigned long long *__restrict__ arrived,
                   unsigned long long call) {
   constexpr int R = 8 * NT, KS = D / 16, KW = D / 32, VB = D / 16;  // k-steps; words of a lane's K row; bytes of its V row
-  constexpr int kWarps = DecodeShape<NT>::kWarps, kUps = DecodeShape<NT>::kUps, kStages = DecodeShape<NT>::kStages;
+  constexpr int kWarps = DecodeShape<D, NT>::kWarps, kUps = DecodeShape<D, NT>::kUps, kStages = DecodeShape<D, NT>::kStages;
   constexpr int kUnit = 9 * D, kSlot = kUps * 2 * kUnit, kBatch = 32 / kUps;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   auto &sm = *reinterpret_cast<DecodeSmem<D, NT> *>(smem_raw);
@@ -428,11 +442,11 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
     int64_t where = -1;
     int next_page = -1, turn = 0;
     auto page_of = [&](int u) {
-      const int e = (int)(((uint64_t)u * a.upb_magic) >> 40);  // u / units of a block
+      const int e = divide(u, a.by_upb);  // u / units of a block
       return u < in.u1 && e < a.max_blocks ? a.tables[in.b * a.table_stride + e] : -1;
     };
     auto take_batch = [&] {
-      const int u = in.at + lane, e = (int)(((uint64_t)u * a.upb_magic) >> 40);
+      const int u = in.at + lane, e = divide(u, a.by_upb);
       where = next_page < 0 || next_page >= a.num_blocks
                   ? -1
                   : next_page * a.block_stride + ((int64_t)in.h * a.upb + u - e * a.upb) * kUnit;
@@ -836,7 +850,7 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
 //
 // With hundreds of rows for each key the products bound the kernel, so they go
 // to tcgen05.  A CTA takes kTiles * 128 (token, head) rows of one sequence and
-// key head through the keys, kKeys = 128 at a time, as separate warps:
+// key head through the keys, kKeys at a time, as separate warps:
 //  * four warps bring K and V in: 4-bit bytes from global memory into
 //    registers (a chunk ahead), to half, into shared memory in the 128-byte
 //    swizzled layout.  K as it lies is K-major for S = Q K^T, V is MN-major
@@ -846,11 +860,24 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
 //  * four warps for each tile of rows take S, a thread a row: weights
 //    2^(score - base) in half go back over S as P, their sum stays in the
 //    thread.  The base moves only when a score passes it by kMove, as in the
-//    kernel above: then the weights are taken again and O is scaled in place.
+//    kernel above: then O is scaled in place.
 // Two tiles of rows alternate: while one is in softmax the tensor core works
 // on the other, and K and V are converted once for both.  A tile has two
 // buffers for S, so that the next scores are there when a softmax ends.
 // Tensor memory (512 columns): O of both tiles, two S of both; P lies over S.
+// Where the blocks of rows are fewer than the SMs, several CTAs share a block's
+// keys, and a second kernel joins what they have.
+//
+// Measured (B200, bfloat16, heads of 128, 4 query heads to a key head): three
+// chunks of about 3900 tokens behind 1500 cached ones, 655 GFLOP: 710 us, 920
+// TFLOP/s, 55 % of a library product's rate alone and 66 % of its sustained one.
+// A chunk of 64 keys for both tiles takes about 2000 cycles of an SM: the tensor
+// core is busy for 1300 of them (a product of S with 64 columns takes 48 cycles,
+// its operands being 6 KiB of shared memory, one with P 64), the exponentials for
+// 1024.  What is lost lies between them: each tile's chain softmax, P V, S.
+// Tried and slower: chunks of 128 keys with one S (740 us), tiles that take turns
+// at the exponentials (730), part of the exponentials as polynomials (from 810),
+// the maximum found while the last weights are taken (780).
 
 constexpr int kTiles = 2, kKeys = 64, kRing = 4;
 constexpr int kFillWarps = 4;
@@ -877,19 +904,19 @@ __device__ __forceinline__ void mbar_arrive(uint64_t *m) {
 __device__ __forceinline__ bool mbar_try(uint64_t *m, int parity) {
   int ok;
   asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2, %3;\n selp.b32 %0, 1, 0, p;\n}"
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n selp.b32 %0, 1, 0, p;\n}"
       : "=r"(ok)
-      : "r"(smem_addr(m)), "r"(parity), "r"(1000000)
+      : "r"(smem_addr(m)), "r"(parity)
       : "memory");
   return ok;
 }
-// A wait has a limit (a try lasts about a microsecond, the whole of them about
-// a second).  One that runs out is counted (fkv_fp4_wait_timeouts) and the
-// kernel goes on as if it had come, each later wait with a single try: it ends,
-// and its output is not to be used.
+// A wait has a limit (a try that fails lasts 4 us, the whole of them a second).
+// One that runs out is counted (fkv_fp4_wait_timeouts) and the kernel goes on as
+// if it had come, each later wait with a single try: it ends, and its output is
+// not to be used.
 __device__ unsigned long long g_wait_timeouts;
 struct Patience {
-  int tries = 1 << 20;
+  int tries = 1 << 18;
   __device__ __forceinline__ void wait(uint64_t *m, int parity) {
     for (int i = 0; i < tries; ++i)
       if (mbar_try(m, parity)) return;
@@ -1019,7 +1046,7 @@ __device__ __forceinline__ bool find_block(const AttnArgs &a, int at, int blocks
     return true;
   }
   const int want = blocks - 1 - at;
-  int before = 0;
+  int64_t before = 0;
   for (int b0 = 0; b0 < a.num_seqs; b0 += 32) {
     const int mine = b0 + lane < a.num_seqs ? item_of<R>(a, b0 + lane).blocks : 0;
     int upto = mine;
@@ -1032,7 +1059,7 @@ __device__ __forceinline__ bool find_block(const AttnArgs &a, int at, int blocks
     if (past) {
       const int l = __ffs(past) - 1;
       b = b0 + l;
-      rb = want - before - __shfl_sync(~0u, upto - mine, l);
+      rb = (int)(want - before) - __shfl_sync(~0u, upto - mine, l);
       return true;
     }
     before += __shfl_sync(~0u, upto, 31);
@@ -1224,33 +1251,33 @@ fp4_many_kernel(const __grid_constant__ AttnArgs a, int blocks, int splits, floa
         }
         reinterpret_cast<float2 *>(part + kTiles * 128 * D)[t * 128 + r] = make_float2(base, sum);
       } else {
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      uint8_t *dst = a.out + (it.first + i0) * a.o_token_stride + tok_head * a.o_head_stride;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        uint8_t *dst = a.out + (it.first + i0) * a.o_token_stride + tok_head * a.o_head_stride;
 #pragma unroll 1
-      for (int c = 0; c < D / 16; ++c) {
-        uint32_t x[16];
-        if (chunks) {
-          tmem_load16(x, o_at(t) + lanes + 16 * c);
-          tmem_wait_load(x);
-        }
-        if (valid) {
-          uint32_t y[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float u = sum == 0.0f ? 0.0f : __uint_as_float(x[2 * k]) * inv;
-            const float v = sum == 0.0f ? 0.0f : __uint_as_float(x[2 * k + 1]) * inv;
-            if (BF16) {
-              const __nv_bfloat162 z = __floats2bfloat162_rn(u, v);
-              y[k] = *reinterpret_cast<const uint32_t *>(&z);
-            } else {
-              y[k] = pack_half2(u, v);
-            }
+        for (int c = 0; c < D / 16; ++c) {
+          uint32_t x[16];
+          if (chunks) {
+            tmem_load16(x, o_at(t) + lanes + 16 * c);
+            tmem_wait_load(x);
           }
-          reinterpret_cast<uint4 *>(dst)[2 * c] = make_uint4(y[0], y[1], y[2], y[3]);
-          reinterpret_cast<uint4 *>(dst)[2 * c + 1] = make_uint4(y[4], y[5], y[6], y[7]);
+          if (valid) {
+            uint32_t y[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float u = sum == 0.0f ? 0.0f : __uint_as_float(x[2 * k]) * inv;
+              const float v = sum == 0.0f ? 0.0f : __uint_as_float(x[2 * k + 1]) * inv;
+              if (BF16) {
+                const __nv_bfloat162 z = __floats2bfloat162_rn(u, v);
+                y[k] = *reinterpret_cast<const uint32_t *>(&z);
+              } else {
+                y[k] = pack_half2(u, v);
+              }
+            }
+            reinterpret_cast<uint4 *>(dst)[2 * c] = make_uint4(y[0], y[1], y[2], y[3]);
+            reinterpret_cast<uint4 *>(dst)[2 * c + 1] = make_uint4(y[4], y[5], y[6], y[7]);
+          }
         }
-      }
-      if (a.lse && valid) a.lse[(it.first + i0) * (a.kv_heads * a.group) + tok_head] = natural_lse(base, sum);
+        if (a.lse && valid) a.lse[(it.first + i0) * (a.kv_heads * a.group) + tok_head] = natural_lse(base, sum);
       }
     }
   } else if (warp < 4 * kTiles + kFillWarps) {
@@ -1267,7 +1294,7 @@ fp4_many_kernel(const __grid_constant__ AttnArgs a, int blocks, int splits, floa
       at_chunk[k] = (c >> 3) * ManySmem<D>::kCols + w * 16 * 128 + tok * 128 + ((c & 7) ^ tok) * 16;
     }
     auto page_of = [&](int j) {
-      const int u = (chunk0 + j) * (kKeys / 16) + w, e = (int)(((uint64_t)u * a.upb_magic) >> 40);
+      const int u = (chunk0 + j) * (kKeys / 16) + w, e = divide(u, a.by_upb);
       return u * 16 < most && e < a.max_blocks ? a.tables[b * a.table_stride + e] : -1;
     };
     uint32_t x[2][2][kWords], sc[2][2];  // pieces of K and of V of a chunk, on their way
@@ -1275,7 +1302,7 @@ fp4_many_kernel(const __grid_constant__ AttnArgs a, int blocks, int splits, floa
     int page;
     uint32_t bad = 0;
     auto find = [&](int j) {  // the unit of chunk j, and the page of the chunk after it
-      const int u = (chunk0 + j) * (kKeys / 16) + w, e = (int)(((uint64_t)u * a.upb_magic) >> 40);
+      const int u = (chunk0 + j) * (kKeys / 16) + w, e = divide(u, a.by_upb);
       const bool good = page >= 0 && page < a.num_blocks;
       unit = good ? a.layer + page * a.block_stride + ((int64_t)h * a.upb + u - e * a.upb) * (9 * D) : nullptr;
       bad = !good && u * 16 < most;
@@ -1469,7 +1496,7 @@ int launch_decode(const AttnArgs &a, int ctas, void *workspace, cudaStream_t s) 
   FKV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   float *slots = (float *)workspace;
   auto *arrived = (unsigned long long *)(slots + (int64_t)ctas * 2 * slot_floats<D>(8 * NT));
-  kernel<<<ctas, DecodeShape<NT>::kWarps * 32, smem, s>>>(a, slots, arrived, next_call());
+  kernel<<<ctas, DecodeShape<D, NT>::kWarps * 32, smem, s>>>(a, slots, arrived, next_call());
   FKV_CUDA(cudaGetLastError());
   note_launch();
   return FKV_OK;
@@ -1582,7 +1609,7 @@ int fkv_fp4_attention(const void *layer, int64_t num_blocks, int tokens_per_bloc
   a.layer = (const uint8_t *)layer, a.num_blocks = num_blocks, a.kv_stride = kv_stride_in_bytes;
   a.block_stride = block_stride_in_bytes, a.tokens_per_block = tokens_per_block, a.kv_heads = num_kv_heads;
   a.group = num_q_heads / num_kv_heads;
-  a.upb = tokens_per_block / 16, a.upb_magic = ((uint64_t)1 << 40) / a.upb + 1;
+  a.upb = tokens_per_block / 16, a.by_upb = divisor_of(a.upb);
   a.q = (const uint8_t *)q, a.q_token_stride = q_token_stride_in_bytes, a.q_head_stride = q_head_stride_in_bytes;
   a.out = (uint8_t *)out, a.o_token_stride = out_token_stride_in_bytes, a.o_head_stride = out_head_stride_in_bytes;
   a.lse = lse, a.num_q = num_q_tokens, a.tables = block_tables, a.table_stride = block_table_stride;

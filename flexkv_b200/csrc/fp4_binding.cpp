@@ -2,7 +2,8 @@
 // the C ABI (include/flexkv_b200.h).  A CPython module on torch's C++ tensors
 // and not ctypes, because these run once per layer and token: reading the
 // tensors' shapes in Python and converting up to 29 arguments took 15 to 20 us
-// a call, several times the smallest kernels; here it takes 2 to 4 us.
+// a call, several times the smallest kernels; here it takes 3 us, 2.3 of them the
+// launch, and about 1 us for each tensor it allocates.
 #include <Python.h>
 
 #include <ATen/ATen.h>
@@ -80,6 +81,8 @@ Geometry geometry(const Tensor &t, const char *name) {
   return {n[1], n[0] > 1 ? s[0] : 0, n[1] > 1 ? s[1] : 0, (int)n[0], (int)n[3] * 16, (int)n[2], (int)(n[4] / 9)};
 }
 
+int64_t block_bytes(const Geometry &g) { return (int64_t)g.heads * g.tpb * g.dim / 16 * 9; }
+
 int dtype_code(at::ScalarType t, const char *name) {
   if (t == at::kBFloat16) return FKV_DTYPE_BF16;
   if (t == at::kHalf) return FKV_DTYPE_FP16;
@@ -106,6 +109,22 @@ Rows rows(const Tensor &t, const char *name, int64_t tokens, int64_t heads, int6
   on_device(t, name, dev);
   if (t.stride(2) != 1) refuse(name, ": the channels of a head must be contiguous");
   return {tokens > 1 ? 2 * t.stride(0) : 0, heads > 1 ? 2 * t.stride(1) : 0};
+}
+
+// What a call writes must not overlap itself.
+void rows_apart(const Tensor &t, const char *name) {
+  const int64_t token = t.stride(0), head = t.stride(1), D = t.size(2), n = t.size(0), heads = t.size(1);
+  if (n <= 1 && heads <= 1) return;
+  const bool heads_inside = heads <= 1 || (head >= D && (n <= 1 || token >= (heads - 1) * head + D));
+  const bool tokens_inside = n <= 1 || (token >= D && (heads <= 1 || head >= (n - 1) * token + D));
+  if (!heads_inside && !tokens_inside) refuse(name, ": rows overlap");
+}
+void blocks_apart(const Tensor &t, int64_t block, const char *name) {
+  const int64_t kv = t.stride(0), blk = t.stride(1), n = t.size(1), sides = t.size(0);
+  if (n <= 1 && sides <= 1) return;
+  const bool sides_inside = sides <= 1 || (kv >= block && (n <= 1 || blk >= (sides - 1) * kv + block));
+  const bool blocks_inside = n <= 1 || (blk >= block && (sides <= 1 || kv >= (n - 1) * blk + block));
+  if (!sides_inside && !blocks_inside) refuse(name, ": blocks overlap");
 }
 
 void no_grad(std::initializer_list<const Tensor *> ts) {
@@ -163,6 +182,7 @@ PyObject *write(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const int dt = dtype_code(k.scalar_type(), "k");
     const Rows rk = rows(k, "k", tokens, g.heads, g.dim, k.scalar_type(), dev);
     const Rows rv = v ? rows(*v, "v", tokens, g.heads, g.dim, k.scalar_type(), dev) : Rows{};
+    blocks_apart(layer, block_bytes(g), "layer");
     const c10::cuda::CUDAGuard guard(dev);
     const Tensor ids = slots.contiguous();
     check(lib.write(layer.data_ptr(), g.kv, g.blocks, g.tpb, g.heads, g.dim, g.kv_stride, g.block_stride, k.data_ptr(),
@@ -199,6 +219,10 @@ PyObject *read(PyObject *, PyObject *const *args, Py_ssize_t n) {
     }
     const Rows rk = rows(k, "k", tokens, g.heads, g.dim, type, dev);
     const Rows rv = v.defined() ? rows(v, "v", tokens, g.heads, g.dim, type, dev) : Rows{};
+    if (args[3] != Py_None) {
+      rows_apart(k, "k");
+      if (v.defined()) rows_apart(v, "v");
+    }
     const Tensor ids = slots.contiguous();
     check(lib.read(layer.data_ptr(), g.kv, g.blocks, g.tpb, g.heads, g.dim, g.kv_stride, g.block_stride, k.data_ptr(),
                        v.defined() ? v.data_ptr() : nullptr, rk.token, rk.head, rv.token, rv.head, dt,
@@ -251,6 +275,10 @@ PyObject *convert(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const int dt = dtype_code(k0.scalar_type(), "a 16-bit layer");
     if (k0.stride(4) != 1 || (g.heads > 1 && k0.stride(3) != g.dim) || k0.stride(2) != (int64_t)g.heads * g.dim)
       refuse("a block of a 16-bit layer must be contiguous");
+    if (pack)
+      blocks_apart(f0, block_bytes(g), "fp4_layers");
+    else
+      blocks_apart(k0, (int64_t)g.tpb * g.heads * g.dim, "kv_layers");
     std::vector<void *> kp(layers), fp(layers);
     for (Py_ssize_t i = 0; i < layers; ++i) {
       const Tensor &f = tensor(PySequence_Fast_GET_ITEM(fps, i), "an entry of fp4_layers");
@@ -336,6 +364,7 @@ PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
                  : cu  ? at::zeros({n, q_heads, g.dim}, q.options())
                        : at::empty({n, q_heads, g.dim}, q.options());
     const Rows ro = rows(out, "out", n, q_heads, g.dim, q.scalar_type(), dev);
+    if (given) rows_apart(out, "out");
     Tensor lse;
     if (want_lse) lse = at::full({n, q_heads}, -INFINITY, q.options().dtype(at::kFloat));
     const Tensor t = tables.size(1) > 1 && tables.stride(1) != 1 ? tables.contiguous() : tables;

@@ -35,8 +35,8 @@ struct RowsArgsOf {
   int tokens_per_block;
   int upb;                // units (16 tokens) of a block
   int groups;             // groups (16 channels) of a head
-  uint64_t upb_magic, groups_magic;  // x / upb = (x * upb_magic) >> 40 for x < 2^28 and a divisor up to 2^12
-  bool far;               // more units than that in the 4-bit layer, or in a block
+  Divisor by_upb, by_groups;
+  bool far;               // more units in the 4-bit layer, or in a block, than by_upb is for
   int64_t num_rows;       // tokens of the call (blocks * tokens_per_block for the block form)
   int64_t num_slots;      // slots of the 4-bit layer
   int64_t num_blocks, num_row_blocks;  // of the 4-bit and of the 16-bit side (block form)
@@ -83,6 +83,13 @@ __device__ __forceinline__ void store_group(uint8_t *p, const uint32_t (&r)[8]) 
 // they and the rows divide the CTA's threads evenly: a thread then keeps its
 // row and group through all heads and looks its slot up once.  0: at run time,
 // a place for each group.
+//
+// Bound by memory: 2 + 9/16 bytes a value.  Measured (B200, heads of 128): 256
+// blocks of 16 tokens, 8 heads, 32 layers packed and unpacked again in 214 us, 6.4
+// TB/s, 98 % of a copy's rate; a call that reads 32768 tokens 30.6 us, 5.6 TB/s.
+// With divisions for each group's place and true ones in the rounding, 9 blocks of
+// 28 layers there and back took 9.9 us instead of 6.9, and quantising was bound by
+// the issue of 315 instructions a group.
 template <bool WRITE, bool BF16, bool BLOCKS, bool WIDE, int NG, int R>
 __global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constant__ RowsArgs<BLOCKS> a) {
   const int ng = NG ? NG : a.groups, D = 16 * ng;
@@ -101,7 +108,7 @@ __global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constan
     if (BLOCKS) {
       // a block's rows are multiples of 16, R = 16: row 0 says which block
       const int64_t u = row0 >> 4;
-      const int64_t blk = a.far ? u / a.upb : (int64_t)(((uint64_t)u * a.upb_magic) >> 40);
+      const int64_t blk = a.far ? u / a.upb : divide((int)u, a.by_upb);
       const int in = (int)(u - blk * a.upb);
       const int64_t fb = a.fp4_ids[blk], rb = a.row_ids[blk];
       if (fb < 0 || fb >= a.num_blocks || rb < 0 || rb >= a.num_row_blocks) return;
@@ -113,7 +120,7 @@ __global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constan
       const int64_t slot = a.fp4_ids[i];
       if (slot < 0 || slot >= a.num_slots) return;
       const int64_t u = slot >> 4;
-      const int64_t blk = a.far ? u / a.upb : (int64_t)(((uint64_t)u * a.upb_magic) >> 40);
+      const int64_t blk = a.far ? u / a.upb : divide((int)u, a.by_upb);
       off = (int)(slot & 15);
       unit = fp4 + blk * a.fp4_block_stride + (u - blk * a.upb) * (9 * D);
     }
@@ -173,7 +180,7 @@ __global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constan
         const int w = w0 + k * kThreads;
         unit[k] = row[k] = nullptr, off[k] = 0;
         if (w >= work) continue;
-        const int q = (int)(((uint64_t)w * a.groups_magic) >> 40), h = q / R;  // w / ng
+        const int q = divide(w, a.by_groups), h = q / R;  // w < 2^24
         g[k] = w - q * ng;
         find(q % R, unit[k], row[k], off[k]);
         if (row[k]) row[k] += h * head_stride;
@@ -232,8 +239,9 @@ template <bool WRITE, bool BLOCKS>
 int run_rows(RowsArgs<BLOCKS> &a, int num_layers, int head_size, int dtype, bool wide, cudaStream_t s) {
   const int ng = head_size / 16, r = a.num_rows < 16 ? 1 : 16;
   a.upb = a.tokens_per_block / 16, a.groups = ng;
-  a.upb_magic = ((uint64_t)1 << 40) / a.upb + 1, a.groups_magic = ((uint64_t)1 << 40) / ng + 1;
   a.far = a.num_slots >> 32 || a.num_rows >> 32 || a.upb > 4096;
+  if (!a.far) a.by_upb = divisor_of(a.upb);
+  a.by_groups = divisor_of(ng);
   // grid.x counts row groups: 2^31 - 1 of them is the launch limit
   const int64_t gx = (a.num_rows + r - 1) / r;
   if (gx > INT32_MAX) return fail(FKV_ERR_INVALID_ARG, "more than 2^31 groups of rows in one call");

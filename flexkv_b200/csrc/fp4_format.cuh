@@ -9,6 +9,20 @@
 
 namespace fkv {
 
+// x / d for 0 <= x < 2^28 and 0 < d <= 2^12 as one product: with 2^c >= d and
+// mul = (2^(28 + c) + e) / d, 0 < e <= d, the product is x e / 2^(28 + c) of a
+// d-th too large, less than one.  mul is at most 2^29.
+struct Divisor {
+  uint32_t mul;
+  int shift;
+};
+inline Divisor divisor_of(int d) {
+  int shift = 28;
+  while (d > 1 << (shift - 28)) ++shift;
+  return {(uint32_t)(((uint64_t)1 << shift) / d + 1), shift};
+}
+__device__ __forceinline__ int divide(int x, const Divisor &by) { return (int)(((uint64_t)(uint32_t)x * by.mul) >> by.shift); }
+
 // The scale code nearest to v >= 0 (ties to the even code), at most 226,
 // which is 10240: 6 * 10240 is below the largest half.
 __device__ __forceinline__ uint32_t scale_code(float v) {

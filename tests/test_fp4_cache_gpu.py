@@ -630,3 +630,68 @@ def test_another_device():
     slots = torch.arange(40, device="cuda:1")
     k, _ = fp4_cache.fp4_read(layer, slots)
     assert torch.cuda.current_device() == 0 and np.array_equal(f64(k), M.held(layer.cpu().numpy())[0][:40])
+
+
+def test_slots_past_2_to_the_28():
+    """Rows in a pool whose units pass 2^24, two heads a block: each in its place, and nothing anywhere else."""
+    blocks, heads, dim = 2 ** 24 + 2, 2, 16
+    layer = torch.zeros(1, blocks, heads, 1, 9 * dim, dtype=torch.uint8, device="cuda")
+    slots = np.array([2 ** 28 + 17, 5, 2 ** 28 - 1, 2 ** 28, blocks * 16])
+    k = torch.randn(len(slots), heads, dim, device="cuda").bfloat16()
+    fp4_cache.fp4_write(layer, k, None, torch.from_numpy(slots).cuda())
+    held = np.unique(slots[:4] // 16)
+    want = np.zeros((1, len(held), heads, 1, 9 * dim), dtype=np.uint8)
+    M.write(want, [f64(k)[:4]], np.searchsorted(held, slots[:4] // 16) * 16 + slots[:4] % 16)
+    there = layer[:, torch.from_numpy(held).cuda()]
+    assert np.array_equal(M.held(there.cpu().numpy()), M.held(want))
+    got = f64(fp4_cache.fp4_read(layer, torch.from_numpy(slots).cuda())[0])
+    assert np.array_equal(got[:4], M.dequantise(*M.quantise(f64(k)[:4]))) and not got[4].any()
+    nonzero = sum(int(torch.count_nonzero(x)) for x in layer[0].split(2 ** 22))
+    assert nonzero == int(torch.count_nonzero(there))
+
+
+@pytest.mark.parametrize("new", [1, 3, 40])
+@pytest.mark.parametrize("tpb", [16, 48])
+def test_positions_past_2_to_the_28(new, tpb):
+    """A sequence whose pages are outside the pool but for one at the start and those behind 2^28 tokens: the same
+    as one of these pages alone."""
+    far = 2 ** 28 // tpb + 1
+    layer = torch.from_numpy(written(2, 9, 2, tpb, 64, 3)).cuda()
+    tables = torch.full((1, far + 7), -1, dtype=torch.int32, device="cuda")
+    few = torch.tensor([[4, 0, 8, 3, 1, 7, 2, 6]], dtype=torch.int32, device="cuda")
+    tables[0, 5], tables[0, far:] = few[0, 0], few[0, 1:]
+    length = torch.tensor([far * tpb + 6 * tpb + 5], dtype=torch.int32, device="cuda")
+    q = torch.randn(new, 4, 64, device="cuda").bfloat16()
+    out, lse = fp4_cache.fp4_attention(layer, q, tables, length, return_lse=True)
+    short = length - (far - 1) * tpb
+    want, wlse, weight, size = M.attention(layer.cpu().numpy(), f64(q), few.cpu().numpy(), short.cpu().numpy(),
+                                           np.array([0, new]), 0.125, True, tpb)
+    assert (np.abs(f64(out) - want) <= M.attention_bounds(weight, size, want, 64, "bf16")).all()
+    assert np.abs(f64(lse) - wlse).max() < 1e-4
+
+
+def test_what_is_written_must_not_overlap():
+    layer, slots = garbage(2, 4, 2, 16, 64), torch.arange(5, device="cuda")
+    x = torch.zeros(5, 2, 64, dtype=torch.bfloat16, device="cuda")
+    for bad in (x[:1].expand(5, 2, 64), x[:, :1].expand(5, 2, 64), torch.zeros(900, dtype=x.dtype, device="cuda").as_strided((5, 2, 64), (64, 64, 1))):
+        fp4_cache.fp4_write(layer, bad, bad, slots)  # to read from is fine
+        with pytest.raises(RuntimeError, match="rows overlap"):
+            fp4_cache.fp4_read(layer, slots, out=(x, bad))
+        with pytest.raises(RuntimeError, match="rows overlap"):
+            fp4_cache.fp4_attention(layer, x[:, :2], torch.zeros(1, 1, dtype=torch.int32, device="cuda"),
+                                    torch.ones(1, dtype=torch.int32, device="cuda"), out=bad)
+    for bad in (layer[:, :1].expand(2, 4, 2, 1, 576), layer[:1].expand(2, 4, 2, 1, 576)):
+        with pytest.raises(RuntimeError, match="blocks overlap"):
+            fp4_cache.fp4_write(bad, x, x, slots)
+        fp4_cache.fp4_read(bad, slots)
+        kv, ids = torch.zeros(2, 4, 16, 2, 64, dtype=x.dtype, device="cuda"), torch.arange(2)
+        with pytest.raises(RuntimeError, match="blocks overlap"):
+            fp4_cache.fp4_pack_blocks([kv], [bad], ids, ids)
+        fp4_cache.fp4_unpack_blocks([bad], [kv], ids, ids)
+        with pytest.raises(RuntimeError, match="blocks overlap"):
+            fp4_cache.fp4_unpack_blocks([layer], [kv[:, :1].expand(2, 4, 16, 2, 64)], ids, ids)
+    # sides within a block, and heads outside of tokens
+    inner = torch.zeros(4, 2, 2, 1, 576, dtype=torch.uint8, device="cuda").transpose(0, 1)
+    fp4_cache.fp4_write(inner, x, x, slots)
+    y = torch.zeros(2, 5, 64, dtype=x.dtype, device="cuda").transpose(0, 1)
+    fp4_cache.fp4_read(inner, slots, out=(y, x))
