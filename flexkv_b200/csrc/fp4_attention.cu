@@ -41,6 +41,7 @@ struct AttnArgs {
   int num_seqs;
   float scale;
   int causal;
+  int fill_rest;  // rows of no sequence: zeros, lse -inf
 };
 
 __device__ __forceinline__ float natural_lse(float m, float l) {  // m: in powers of two
@@ -74,6 +75,23 @@ __device__ __forceinline__ void store_row(const AttnArgs &a, int64_t first, int 
     *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
   }
   if (a.lse && c == 0) a.lse[(first + i) * (a.kv_heads * a.group) + qh] = natural_lse(m, l);
+}
+
+// Rows before the first sequence and behind the last, this CTA's share of them,
+// by `n` of its threads (a kernel of its own before the call took 16 us for
+// 12000 rows of 32 heads of 128, all of which the sequences then wrote).
+__device__ __forceinline__ void fill_rest(const AttnArgs &a, int D, int thread, int n) {
+  const int64_t lo = min((int64_t)max(a.cu[0], 0), a.num_q);
+  const int64_t hi = max(min((int64_t)max(a.cu[a.num_seqs], 0), a.num_q), lo), rest = lo + a.num_q - hi;
+  const int heads = a.kv_heads * a.group, pieces = heads * (D / 8);
+  for (int64_t i = blockIdx.x; i < rest; i += gridDim.x) {
+    const int64_t row = i < lo ? i : hi + i - lo;
+    for (int j = thread; j < pieces; j += n) {
+      const int h = j / (D / 8), c = j - h * (D / 8);
+      *reinterpret_cast<uint4 *>(a.out + row * a.o_token_stride + h * a.o_head_stride + 16 * c) = make_uint4(0, 0, 0, 0);
+      if (a.lse && c == 0) a.lse[row * heads + h] = -INFINITY;
+    }
+  }
 }
 
 // ---- few rows: decoding, and checking a handful of proposed tokens ----------
@@ -426,6 +444,7 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
   const Cut cut = find_cut<R, kWarps>(a);
   const int64_t begin = cut.begin;
   const int units_here = (int)(cut.end - begin);
+  if (a.fill_rest) fill_rest(a, D, threadIdx.x, kWarps * 32);
   if (units_here <= 0) return;
   // the first warps have a unit more, or all there are
   const int share = units_here / kWarps, rest = units_here - share * kWarps;
@@ -1083,7 +1102,10 @@ fp4_many_kernel(const __grid_constant__ AttnArgs a, int blocks, int splits, floa
   const int h = blockIdx.x % a.kv_heads, of = blockIdx.x / a.kv_heads, at = of / splits, split = of - at * splits;
 
   int b, rb;
-  if (!find_block<R>(a, at, blocks, b, rb)) return;  // the grid is an upper bound
+  if (!find_block<R>(a, at, blocks, b, rb)) {  // the grid is an upper bound
+    if (a.fill_rest) fill_rest(a, D, threadIdx.x, kManyThreads);
+    return;
+  }
   const Item it = item_of<R>(a, b);
   const int row0 = rb * R, nrows = it.rows * a.group;
   const int tiles = nrows - row0 > 128 ? 2 : 1;
@@ -1371,6 +1393,7 @@ fp4_many_kernel(const __grid_constant__ AttnArgs a, int blocks, int splits, floa
         unit = keep;
       }
     }
+    if (a.fill_rest) fill_rest(a, D, threadIdx.x - 128 * kTiles, kFillWarps * 32);
   } else {
     // ---- the products: a warp for each tile ----
     // In loops and not straight code: these warps share their instruction caches with three busier ones each.  The
@@ -1581,7 +1604,7 @@ int fkv_fp4_attention(const void *layer, int64_t num_blocks, int tokens_per_bloc
                       int64_t q_token_stride_in_bytes, int64_t q_head_stride_in_bytes, int64_t out_token_stride_in_bytes,
                       int64_t out_head_stride_in_bytes, int dtype, int64_t num_q_tokens, int num_q_heads,
                       const int32_t *block_tables, int64_t block_table_stride, int max_blocks, const int32_t *seq_lens,
-                      const int32_t *cu_seqlens_q, int num_seqs, int max_q_len, float softmax_scale, int causal,
+                      const int32_t *cu_seqlens_q, int num_seqs, int max_q_len, float softmax_scale, int flags,
                       void *workspace, int64_t workspace_bytes, void *stream) {
   clear_error();
   const char *w = "fkv_fp4_attention: ";
@@ -1614,7 +1637,8 @@ int fkv_fp4_attention(const void *layer, int64_t num_blocks, int tokens_per_bloc
   a.out = (uint8_t *)out, a.o_token_stride = out_token_stride_in_bytes, a.o_head_stride = out_head_stride_in_bytes;
   a.lse = lse, a.num_q = num_q_tokens, a.tables = block_tables, a.table_stride = block_table_stride;
   a.max_blocks = max_blocks, a.seq_lens = seq_lens, a.cu = cu_seqlens_q, a.num_seqs = num_seqs;
-  a.scale = softmax_scale, a.causal = causal;
+  a.scale = softmax_scale, a.causal = flags & FKV_FP4_CAUSAL;
+  a.fill_rest = cu_seqlens_q && (flags & FKV_FP4_FILL_REST);
   a.rows_each = (int)(num_q_tokens / num_seqs);
   a.table_tokens = (int)std::min<int64_t>((int64_t)max_blocks * tokens_per_block, INT32_MAX - 255);  // positions are ints
   ThreadDeviceCtx *ctx;

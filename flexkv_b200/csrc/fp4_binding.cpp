@@ -359,14 +359,17 @@ PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     const int causal = PyObject_IsTrue(args[7]), want_lse = PyObject_IsTrue(args[9]);
     if (causal < 0 || want_lse < 0) return nullptr;
     const c10::cuda::CUDAGuard guard(dev);
-    // without cu_seqlens_q every row belongs to a sequence
-    Tensor out = given ? *given
-                 : cu  ? at::zeros({n, q_heads, g.dim}, q.options())
-                       : at::empty({n, q_heads, g.dim}, q.options());
+    // without cu_seqlens_q every row belongs to a sequence, and without a sequence nothing is launched
+    const bool fill = !given && cu && seqs;
+    Tensor out = given           ? *given
+                 : cu && !seqs ? at::zeros({n, q_heads, g.dim}, q.options())
+                                 : at::empty({n, q_heads, g.dim}, q.options());
     const Rows ro = rows(out, "out", n, q_heads, g.dim, q.scalar_type(), dev);
     if (given) rows_apart(out, "out");
     Tensor lse;
-    if (want_lse) lse = at::full({n, q_heads}, -INFINITY, q.options().dtype(at::kFloat));
+    if (want_lse)
+      lse = cu && !fill ? at::full({n, q_heads}, -INFINITY, q.options().dtype(at::kFloat))
+                        : at::empty({n, q_heads}, q.options().dtype(at::kFloat));
     const Tensor t = tables.size(1) > 1 && tables.stride(1) != 1 ? tables.contiguous() : tables;
     const Tensor l = lens.contiguous();
     std::optional<Tensor> c;
@@ -378,7 +381,8 @@ PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     check(lib.attention(layer.data_ptr(), g.blocks, g.tpb, g.heads, g.dim, g.kv_stride, g.block_stride, q.data_ptr(),
                             out.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr, rq.token, rq.head, ro.token, ro.head,
                             dt, n, (int)q_heads, t.data_ptr<int32_t>(), t.stride(0), (int)t.size(1), l.data_ptr<int32_t>(),
-                            c ? c->data_ptr<int32_t>() : nullptr, (int)seqs, (int)longest, (float)scale, causal,
+                            c ? c->data_ptr<int32_t>() : nullptr, (int)seqs, (int)longest, (float)scale,
+                            (causal ? FKV_FP4_CAUSAL : 0) | (fill ? FKV_FP4_FILL_REST : 0),
                             bytes > 0 ? workspace.data_ptr() : nullptr, bytes, stream_of(dev)),
           "fp4_attention");
     PyObject *po = given ? Py_NewRef(args[8]) : THPVariable_Wrap(out);

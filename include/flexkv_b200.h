@@ -657,14 +657,18 @@ int fkv_fp4_unpack_blocks(int num_layers, void *const *fp4_layer_ptrs, void *con
  * seq_lens[b] tokens in the cache, the new ones among them, and its token j in
  * block block_tables[b * block_table_stride + j / tokens_per_block], of
  * max_blocks entries.  Its row i sees the keys up to position seq_lens[b] -
- * rows + i (causal != 0) or all of them.  A row that sees nothing gives zeros.
- * Tokens past the table (or past 2^31 - 256), or in a block outside the pool,
- * count as hidden.  cu_seqlens_q must not decrease.  Rows of no sequence are left as they were.  max_q_len: the most rows of a
- * sequence, which only chooses the kernel.  lse (optional): float [num_q_tokens,
+ * rows + i (flag FKV_FP4_CAUSAL) or all of them.  A row that sees nothing gives
+ * zeros.  Tokens past the table (or past 2^31 - 256), or in a block outside the
+ * pool, count as hidden.  cu_seqlens_q must not decrease.  Rows before the first
+ * sequence and behind the last are left as they were, or become zeros (lse:
+ * -inf) with flag FKV_FP4_FILL_REST where there is a sequence at all.
+ * max_q_len: the most rows of a sequence, which only chooses the kernel.  lse (optional): float [num_q_tokens,
  * num_q_heads], the natural logarithm of the sum of exponentials, -inf for a
  * row that sees nothing.  workspace: device memory of at least
  * fkv_fp4_attention_workspace bytes, 16-byte aligned, that nothing else uses
  * until the call has run; its content does not matter. */
+#define FKV_FP4_CAUSAL 1
+#define FKV_FP4_FILL_REST 2
 int64_t fkv_fp4_attention_workspace(int64_t num_q_tokens, int num_q_heads, int num_kv_heads,
                                     int head_size, int num_seqs, int max_q_len);
 int fkv_fp4_attention(const void *layer, int64_t num_blocks, int tokens_per_block, int num_kv_heads,
@@ -674,7 +678,7 @@ int fkv_fp4_attention(const void *layer, int64_t num_blocks, int tokens_per_bloc
                       int64_t out_head_stride_in_bytes, int dtype, int64_t num_q_tokens,
                       int num_q_heads, const int32_t *block_tables, int64_t block_table_stride,
                       int max_blocks, const int32_t *seq_lens, const int32_t *cu_seqlens_q,
-                      int num_seqs, int max_q_len, float softmax_scale, int causal, void *workspace,
+                      int num_seqs, int max_q_len, float softmax_scale, int flags, void *workspace,
                       int64_t workspace_bytes, void *stream);
 
 /* Waits between the warps of an attention kernel that ran out of their limit

@@ -695,3 +695,23 @@ def test_what_is_written_must_not_overlap():
     fp4_cache.fp4_write(inner, x, x, slots)
     y = torch.zeros(2, 5, 64, dtype=x.dtype, device="cuda").transpose(0, 1)
     fp4_cache.fp4_read(inner, slots, out=(y, x))
+
+
+@pytest.mark.parametrize("before,new,behind", [(2, 1, 0), (0, 1, 700), (400, 3, 300), (3, 90, 500), (0, 0, 4), (5, 0, 0)])
+def test_rows_of_no_sequence(before, new, behind):
+    """Zeros and -inf in a new output, whatever its memory held, strided heads or not; as they were in a given one."""
+    layer, _, tables, lens, cu = decode_state(4, new=new)
+    n = before + new * 4 + behind
+    q = torch.randn(n, 8, 128, device="cuda").bfloat16()
+    given = torch.full((8, n, 128), 3.0, dtype=q.dtype, device="cuda").transpose(0, 1)
+    fp4_cache.fp4_attention(layer, q, tables, lens, cu + before, max(new, 1), out=given)
+    rows = torch.cat([torch.arange(before), torch.arange(n - behind, n)]).cuda()
+    assert bool((given[rows] == 3.0).all())
+    for _ in range(2):
+        dirt = [torch.full((n, 8, 128), float("nan"), dtype=q.dtype, device="cuda"), torch.full((n, 8), 7.0, device="cuda")]
+        del dirt
+        out, lse = fp4_cache.fp4_attention(layer, q, tables, lens, cu + before, max(new, 1), return_lse=True)
+        assert not bool(out[rows].any()) and bool(torch.isneginf(lse[rows]).all())
+        assert torch.equal(out[before:n - behind], given[before:n - behind])
+    none = fp4_cache.fp4_attention(layer, q, tables[:0], lens[:0], cu[:1] + before, return_lse=True)
+    assert not bool(none[0].any()) and bool(torch.isneginf(none[1]).all())
