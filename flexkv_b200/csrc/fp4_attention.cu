@@ -15,6 +15,7 @@
 
 #include "fkv_common.h"
 #include "fp4_format.cuh"
+#include "fp4_launch.cuh"
 
 namespace fkv {
 namespace {
@@ -440,6 +441,7 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
   extern __shared__ __align__(128) uint8_t smem_raw[];
   auto &sm = *reinterpret_cast<DecodeSmem<D, NT> *>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  after_previous();
   if (lane < 2) sm.meta[warp][lane].there = 0;
   const Cut cut = find_cut<R, kWarps>(a);
   const int64_t begin = cut.begin;
@@ -1100,6 +1102,7 @@ fp4_many_kernel(const __grid_constant__ AttnArgs a, int blocks, int splits, floa
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // a block's heads, and the parts of its keys, run together
   const int h = blockIdx.x % a.kv_heads, of = blockIdx.x / a.kv_heads, at = of / splits, split = of - at * splits;
+  after_previous();
 
   int b, rb;
   if (!find_block<R>(a, at, blocks, b, rb)) {  // the grid is an upper bound
@@ -1458,6 +1461,7 @@ __global__ void __launch_bounds__(256) fp4_merge_kernel(const __grid_constant__ 
   constexpr int R = kTiles * 128, kVec = D / 32;  // floats of a lane
   const int h = blockIdx.x % a.kv_heads, at = blockIdx.x / a.kv_heads, lane = threadIdx.x & 31;
   const int r = blockIdx.y * 8 + (threadIdx.x >> 5);
+  after_previous();
   int b, rb;
   if (!find_block<R>(a, at, blocks, b, rb)) return;
   const Item it = item_of<R>(a, b);
@@ -1519,8 +1523,7 @@ int launch_decode(const AttnArgs &a, int ctas, void *workspace, cudaStream_t s) 
   FKV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   float *slots = (float *)workspace;
   auto *arrived = (unsigned long long *)(slots + (int64_t)ctas * 2 * slot_floats<D>(8 * NT));
-  kernel<<<ctas, DecodeShape<D, NT>::kWarps * 32, smem, s>>>(a, slots, arrived, next_call());
-  FKV_CUDA(cudaGetLastError());
+  FKV_CUDA(launch_next(kernel, dim3(ctas), DecodeShape<D, NT>::kWarps * 32, smem, s, a, slots, arrived, next_call()));
   note_launch();
   return FKV_OK;
 }
@@ -1555,13 +1558,12 @@ int launch_many(const AttnArgs &a, const ManyPlan &p, void *workspace, cudaStrea
   FKV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   if (p.blocks * a.kv_heads * p.splits > INT32_MAX)
     return fail(FKV_ERR_INVALID_ARG, "fkv_fp4_attention: 2^31 blocks of rows or more");
-  kernel<<<(unsigned)(p.blocks * a.kv_heads * p.splits), kManyThreads, smem, s>>>(a, (int)p.blocks, p.splits, (float *)workspace);
-  FKV_CUDA(cudaGetLastError());
+  FKV_CUDA(launch_next(kernel, dim3((unsigned)(p.blocks * a.kv_heads * p.splits)), kManyThreads, smem, s, a, (int)p.blocks,
+                       p.splits, (float *)workspace));
   note_launch();
   if (p.splits > 1) {
-    fp4_merge_kernel<D, BF16><<<dim3((unsigned)(p.blocks * a.kv_heads), kTiles * 128 / 8), 256, 0, s>>>(
-        a, (int)p.blocks, p.splits, (const float *)workspace);
-    FKV_CUDA(cudaGetLastError());
+    FKV_CUDA(launch_next(fp4_merge_kernel<D, BF16>, dim3((unsigned)(p.blocks * a.kv_heads), kTiles * 128 / 8), 256, 0, s, a,
+                         (int)p.blocks, p.splits, (const float *)workspace));
     note_launch();
   }
   return FKV_OK;

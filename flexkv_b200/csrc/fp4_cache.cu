@@ -19,6 +19,7 @@
 
 #include "fkv_common.h"
 #include "fp4_format.cuh"
+#include "fp4_launch.cuh"
 
 namespace fkv {
 namespace {
@@ -92,6 +93,7 @@ __device__ __forceinline__ void store_group(uint8_t *p, const uint32_t (&r)[8]) 
 // the issue of 315 instructions a group.
 template <bool WRITE, bool BF16, bool BLOCKS, bool WIDE, int NG, int R>
 __global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constant__ RowsArgs<BLOCKS> a) {
+  after_previous();
   const int ng = NG ? NG : a.groups, D = 16 * ng;
   const int layer = a.kv_dim == 1 ? blockIdx.y : blockIdx.y >> 1, side = a.kv_dim == 1 ? 0 : blockIdx.y & 1;
   const int64_t row0 = (int64_t)blockIdx.x * R;
@@ -195,27 +197,25 @@ __global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constan
 }
 
 template <bool WRITE, bool BF16, bool BLOCKS, bool WIDE, int R>
-void launch_ng(const RowsArgs<BLOCKS> &a, dim3 grid, int ng, cudaStream_t s) {
+cudaError_t launch_ng(const RowsArgs<BLOCKS> &a, dim3 grid, int ng, cudaStream_t s) {
   switch (ng) {
-    case 4: fp4_rows_kernel<WRITE, BF16, BLOCKS, WIDE, 4, R><<<grid, kThreads, 0, s>>>(a); break;
-    case 8: fp4_rows_kernel<WRITE, BF16, BLOCKS, WIDE, 8, R><<<grid, kThreads, 0, s>>>(a); break;
-    case 16: fp4_rows_kernel<WRITE, BF16, BLOCKS, WIDE, 16, R><<<grid, kThreads, 0, s>>>(a); break;
-    default: fp4_rows_kernel<WRITE, BF16, BLOCKS, WIDE, 0, R><<<grid, kThreads, 0, s>>>(a); break;
+    case 4: return launch_next(fp4_rows_kernel<WRITE, BF16, BLOCKS, WIDE, 4, R>, grid, kThreads, 0, s, a);
+    case 8: return launch_next(fp4_rows_kernel<WRITE, BF16, BLOCKS, WIDE, 8, R>, grid, kThreads, 0, s, a);
+    case 16: return launch_next(fp4_rows_kernel<WRITE, BF16, BLOCKS, WIDE, 16, R>, grid, kThreads, 0, s, a);
+    default: return launch_next(fp4_rows_kernel<WRITE, BF16, BLOCKS, WIDE, 0, R>, grid, kThreads, 0, s, a);
   }
 }
 template <bool WRITE, bool BF16, bool BLOCKS, bool WIDE>
-void launch_r(const RowsArgs<BLOCKS> &a, int rows_at_once, dim3 grid, int ng, cudaStream_t s) {
+cudaError_t launch_r(const RowsArgs<BLOCKS> &a, int rows_at_once, dim3 grid, int ng, cudaStream_t s) {
   if (BLOCKS || rows_at_once == 16)
-    launch_ng<WRITE, BF16, BLOCKS, WIDE, 16>(a, grid, ng, s);
-  else
-    launch_ng<WRITE, BF16, BLOCKS, WIDE, BLOCKS ? 16 : 1>(a, grid, ng, s);
+    return launch_ng<WRITE, BF16, BLOCKS, WIDE, 16>(a, grid, ng, s);
+  return launch_ng<WRITE, BF16, BLOCKS, WIDE, BLOCKS ? 16 : 1>(a, grid, ng, s);
 }
 template <bool WRITE, bool BLOCKS>
-void launch_rows(const RowsArgs<BLOCKS> &a, bool bf16, bool wide, int r, dim3 grid, int ng, cudaStream_t s) {
+cudaError_t launch_rows(const RowsArgs<BLOCKS> &a, bool bf16, bool wide, int r, dim3 grid, int ng, cudaStream_t s) {
   if (bf16)
-    wide ? launch_r<WRITE, true, BLOCKS, true>(a, r, grid, ng, s) : launch_r<WRITE, true, BLOCKS, false>(a, r, grid, ng, s);
-  else
-    wide ? launch_r<WRITE, false, BLOCKS, true>(a, r, grid, ng, s) : launch_r<WRITE, false, BLOCKS, false>(a, r, grid, ng, s);
+    return wide ? launch_r<WRITE, true, BLOCKS, true>(a, r, grid, ng, s) : launch_r<WRITE, true, BLOCKS, false>(a, r, grid, ng, s);
+  return wide ? launch_r<WRITE, false, BLOCKS, true>(a, r, grid, ng, s) : launch_r<WRITE, false, BLOCKS, false>(a, r, grid, ng, s);
 }
 
 int check_geometry(const char *who, int kv_dim, int64_t num_blocks, int tpb, int heads, int head_size, int dtype) {
@@ -245,8 +245,7 @@ int run_rows(RowsArgs<BLOCKS> &a, int num_layers, int head_size, int dtype, bool
   // grid.x counts row groups: 2^31 - 1 of them is the launch limit
   const int64_t gx = (a.num_rows + r - 1) / r;
   if (gx > INT32_MAX) return fail(FKV_ERR_INVALID_ARG, "more than 2^31 groups of rows in one call");
-  launch_rows<WRITE, BLOCKS>(a, dtype == FKV_DTYPE_BF16, wide, r, dim3((unsigned)gx, num_layers * a.kv_dim), ng, s);
-  FKV_CUDA(cudaGetLastError());
+  FKV_CUDA((launch_rows<WRITE, BLOCKS>(a, dtype == FKV_DTYPE_BF16, wide, r, dim3((unsigned)gx, num_layers * a.kv_dim), ng, s)));
   note_launch();
   return FKV_OK;
 }

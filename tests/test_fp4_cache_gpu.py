@@ -715,3 +715,57 @@ def test_rows_of_no_sequence(before, new, behind):
         assert torch.equal(out[before:n - behind], given[before:n - behind])
     none = fp4_cache.fp4_attention(layer, q, tables[:0], lens[:0], cu[:1] + before, return_lse=True)
     assert not bool(none[0].any()) and bool(torch.isneginf(none[1]).all())
+
+
+@pytest.mark.parametrize("new", [1, 3, 40])
+def test_forked_streams(new):
+    """Write, then attention on two streams at once, with other kernels before, between and beside them, captured
+    and eager: each call sees what was before it on its stream and at the joins."""
+    layer, q, tables, lens, cu = decode_state(1, lens=(170, 1000, 0, 133), new=new)
+    src, k = torch.empty_like(q), torch.empty(4 * new, 2, 128, dtype=q.dtype, device="cuda")
+    late, at = torch.empty_like(k), torch.arange(4 * new, device="cuda") % new
+    slots = torch.where(at < 16, tables[:, 0].long().repeat_interleave(new) * 16 + at, -1)
+    side = torch.cuda.Stream()
+
+    def run():
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        q.zero_()
+        with torch.cuda.stream(side):
+            x = torch.ones(2048, 2048, device="cuda")
+            late.copy_(k + (x @ x)[:1, :1].bfloat16() * 0)
+        q.copy_(src)
+        main.wait_stream(side)
+        fp4_cache.fp4_write(layer, late, late, slots)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            outs = [fp4_cache.fp4_attention(layer, q, tables, lens, cu, new)]
+        outs.append(fp4_cache.fp4_attention(layer, q, tables, lens, cu, new))
+        outs.append(fp4_cache.fp4_read(layer, slots)[0])
+        main.wait_stream(side)
+        late.zero_()
+        return outs
+
+    for x in (src, k):
+        x.normal_()
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = run()
+    for turn in range(4):
+        for x in (src, k):
+            x.normal_()
+        layer.fill_(0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in captured]
+        held = torch.where((slots >= 0)[:, None, None], torch.from_numpy(M.dequantise(*M.quantise(f64(k)))).cuda(), 0.0)
+        assert torch.equal(got[2].double(), held)
+        want = fp4_cache.fp4_attention(layer, src, tables, lens, cu, new)
+        layer.fill_(0)
+        eager = run()
+        torch.cuda.synchronize()
+        for x in (got, eager):
+            assert torch.equal(x[0], want) and torch.equal(x[1], want) and torch.equal(x[2], got[2])
