@@ -1142,174 +1142,175 @@ fp4_many_kernel(const __grid_constant__ AttnArgs a, int blocks, int splits, floa
   auto s_at = [&](int t, int i) { return tmem + (kTiles + t) * 128 + i * kKeys; };
   Patience patience;
 
-  if (warp < 4 * kTiles) {
+  if (warp < 4 * tiles) {
     // ---- a thread for each row ----
     const int t = warp >> 2, r = (warp & 3) * 32 + lane, row = row0 + t * 128 + r;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // the warp's 32 lanes of tensor memory
-    if (t < tiles) {
-      const bool valid = row < nrows;
-      const int i0 = valid ? row / a.group : 0;
-      float mul = 0;
-      {
-        const uint8_t *p = a.q + (it.first + i0) * a.q_token_stride + (h * a.group + row - i0 * a.group) * a.q_head_stride;
-        float amax = 0;
-        uint4 x[D / 8];
+    const bool valid = row < nrows;
+    const int i0 = valid ? row / a.group : 0;
+    float mul = 0;
+    {
+      const uint8_t *p = a.q + (it.first + i0) * a.q_token_stride + (h * a.group + row - i0 * a.group) * a.q_head_stride;
+      float amax = 0;
+      uint4 x[D / 8];
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) x[i] = valid ? reinterpret_cast<const uint4 *>(p)[i] : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < D / 8; ++i) x[i] = valid ? reinterpret_cast<const uint4 *>(p)[i] : make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+      for (int i = 0; i < D / 8; ++i) {
+        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 f = pair_to_float2<BF16>(w[j]);
-            amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
-          }
-        }
-        const float f = row_factor(amax), fs = a.scale < 0.0f ? -f : f;
-        mul = fmaxf(fabsf(a.scale) * 1.4426950408889634f * (1.0f / f), 1e-37f);
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-          uint32_t y[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 z = pair_to_float2<BF16>(w[j]);
-            y[j] = pack_half2(z.x * fs, z.y * fs);
-          }
-          *reinterpret_cast<uint4 *>(&sm.q[t][i / 8][r * 128 + ((i % 8) ^ (r & 7)) * 16]) = make_uint4(y[0], y[1], y[2], y[3]);
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = pair_to_float2<BF16>(w[j]);
+          amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
         }
       }
-      fence_async();
-      mbar_arrive(&sm.q_full);
-
-      const int end = valid ? end_of(row) : 0;
-      const int lowest = __reduce_min_sync(~0u, valid ? end : INT32_MAX);
-      float base = kNone, bar = -INFINITY, l[4] = {0, 0, 0, 0};
-      for (int j = 0; j < chunks; ++j) {
-        patience.wait(&sm.s_full[t][j & 1], (j >> 1) & 1);
-        fence_after();
-        const uint32_t S = s_at(t, j & 1) + lanes;
-        uint32_t x[2][32];
-        tmem_load32(x[0], S), tmem_load32(x[1], S + 32);
-        const uint32_t bad = *(volatile uint32_t *)sm.bad[j & (2 * kRing - 1)];
-        tmem_wait_load(x[0]), tmem_wait_load(x[1]);
-        const int key0 = (chunk0 + j) * kKeys;
-        if (key0 + kKeys > lowest || bad) {  // only what the row sees
+      const float f = row_factor(amax), fs = a.scale < 0.0f ? -f : f;
+      mul = fmaxf(fabsf(a.scale) * 1.4426950408889634f * (1.0f / f), 1e-37f);
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
+      for (int i = 0; i < D / 8; ++i) {
+        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+        uint32_t y[4];
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (key0 + 32 * c + i >= end || ((bad >> (8 * (2 * c + i / 16))) & 1)) x[c][i] = 0xFF800000u;
+        for (int j = 0; j < 4; ++j) {
+          const float2 z = pair_to_float2<BF16>(w[j]);
+          y[j] = pack_half2(z.x * fs, z.y * fs);
         }
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        *reinterpret_cast<uint4 *>(&sm.q[t][i / 8][r * 128 + ((i % 8) ^ (r & 7)) * 16]) = make_uint4(y[0], y[1], y[2], y[3]);
+      }
+    }
+    fence_async();
+    mbar_arrive(&sm.q_full);
+
+    const int end = valid ? end_of(row) : 0;
+    const int lowest = __reduce_min_sync(~0u, valid ? end : INT32_MAX);
+    float base = kNone, bar = -INFINITY, l[4] = {0, 0, 0, 0};
+    for (int j = 0; j < chunks; ++j) {
+      patience.wait(&sm.s_full[t][j & 1], (j >> 1) & 1);
+      fence_after();
+      const uint32_t S = s_at(t, j & 1) + lanes;
+      uint32_t x[2][32];
+      tmem_load32(x[0], S), tmem_load32(x[1], S + 32);
+      const uint32_t bad = *(volatile uint32_t *)sm.bad[j & (2 * kRing - 1)];
+      tmem_wait_load(x[0]), tmem_wait_load(x[1]);
+      const int key0 = (chunk0 + j) * kKeys;
+      if (key0 + kKeys > lowest || bad) {  // only what the row sees
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[c][i]));
-        const float most_here = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-        if (__any_sync(~0u, most_here > bar)) {  // rare after the first chunks
-          float f = 1.0f;
-          if (most_here > bar) {  // other rows stay: a row does not depend on its neighbours
-            const float to = most_here * mul - kLift;
-            f = exp2_fast(base - to);
-            base = to;
-            bar = __fdividef(to + kMove, mul);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) l[i] *= f;
-          if (j > 0) {
-            patience.wait(&sm.o_done[t], (j - 1) & 1);
-            fence_after();
-#pragma unroll 1
-            for (int c = 0; c < D / 16; ++c) {
-              uint32_t y[16];
-              tmem_load16(y, o_at(t) + lanes + 16 * c);
-              tmem_wait_load(y);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
-              tmem_store16(o_at(t) + lanes + 16 * c, y);
-            }
-          }
-        }
-        const uint64_t mul2 = pair(mul, mul), base2 = pair(-base, -base);
-        uint64_t l01 = pair(l[0], l[1]), l23 = pair(l[2], l[3]);
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t p[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 y = unpair(fma2(pair(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])), mul2, base2));
-            const float u = exp2_fast(y.x), v = exp2_fast(y.y);
-            if (i & 1)
-              l23 = add2(l23, pair(u, v));
-            else
-              l01 = add2(l01, pair(u, v));
-            p[i] = pack_half2(u, v);
-          }
-          tmem_store16(S + 16 * c, p);
-        }
-        const float2 la = unpair(l01), lb = unpair(l23);
-        l[0] = la.x, l[1] = la.y, l[2] = lb.x, l[3] = lb.y;
-        tmem_wait_store();
-        fence_before();
-        mbar_arrive(&sm.p_full[t][j & 1]);
+          for (int i = 0; i < 32; ++i)
+            if (key0 + 32 * c + i >= end || ((bad >> (8 * (2 * c + i / 16))) & 1)) x[c][i] = 0xFF800000u;
       }
-
-      // O / l
-      if (chunks) {
-        patience.wait(&sm.all_done[t], 0);
-        fence_after();
-      }
-      const int tok_head = h * a.group + row - i0 * a.group;
-      const float sum = (l[0] + l[1]) + (l[2] + l[3]);
-      if (splits > 1) {  // for the kernel below to join
-        float *part = parts + (int64_t)blockIdx.x * split_floats<D>(), *o = part + (t * 128 + r) * D;
-        if (chunks) {
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[c][i]));
+      const float most_here = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      if (__any_sync(~0u, most_here > bar)) {  // rare after the first chunks
+        float f = 1.0f;
+        if (most_here > bar) {  // other rows stay: a row does not depend on its neighbours
+          const float to = most_here * mul - kLift;
+          f = exp2_fast(base - to);
+          base = to;
+          bar = __fdividef(to + kMove, mul);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l[i] *= f;
+        if (j > 0) {
+          patience.wait(&sm.o_done[t], (j - 1) & 1);
+          fence_after();
 #pragma unroll 1
           for (int c = 0; c < D / 16; ++c) {
-            uint32_t x[16];
-            tmem_load16(x, o_at(t) + lanes + 16 * c);
-            tmem_wait_load(x);
+            uint32_t y[16];
+            tmem_load16(y, o_at(t) + lanes + 16 * c);
+            tmem_wait_load(y);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) reinterpret_cast<uint4 *>(o)[4 * c + i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+            for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
+            tmem_store16(o_at(t) + lanes + 16 * c, y);
           }
         }
-        reinterpret_cast<float2 *>(part + kTiles * 128 * D)[t * 128 + r] = make_float2(base, sum);
-      } else {
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        uint8_t *dst = a.out + (it.first + i0) * a.o_token_stride + tok_head * a.o_head_stride;
+      }
+      const uint64_t mul2 = pair(mul, mul), base2 = pair(-base, -base);
+      uint64_t l01 = pair(l[0], l[1]), l23 = pair(l[2], l[3]);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t p[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float2 y = unpair(fma2(pair(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])), mul2, base2));
+          const float u = exp2_fast(y.x), v = exp2_fast(y.y);
+          if (i & 1)
+            l23 = add2(l23, pair(u, v));
+          else
+            l01 = add2(l01, pair(u, v));
+          p[i] = pack_half2(u, v);
+        }
+        tmem_store16(S + 16 * c, p);
+      }
+      const float2 la = unpair(l01), lb = unpair(l23);
+      l[0] = la.x, l[1] = la.y, l[2] = lb.x, l[3] = lb.y;
+      tmem_wait_store();
+      fence_before();
+      mbar_arrive(&sm.p_full[t][j & 1]);
+    }
+
+    // O / l
+    if (chunks) {
+      patience.wait(&sm.all_done[t], 0);
+      fence_after();
+    }
+    const int tok_head = h * a.group + row - i0 * a.group;
+    const float sum = (l[0] + l[1]) + (l[2] + l[3]);
+    if (splits > 1) {  // for the kernel below to join
+      float *part = parts + (int64_t)blockIdx.x * split_floats<D>(), *o = part + (t * 128 + r) * D;
+      if (chunks) {
 #pragma unroll 1
         for (int c = 0; c < D / 16; ++c) {
           uint32_t x[16];
-          if (chunks) {
-            tmem_load16(x, o_at(t) + lanes + 16 * c);
-            tmem_wait_load(x);
-          }
-          if (valid) {
-            uint32_t y[8];
+          tmem_load16(x, o_at(t) + lanes + 16 * c);
+          tmem_wait_load(x);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const float u = sum == 0.0f ? 0.0f : __uint_as_float(x[2 * k]) * inv;
-              const float v = sum == 0.0f ? 0.0f : __uint_as_float(x[2 * k + 1]) * inv;
-              if (BF16) {
-                const __nv_bfloat162 z = __floats2bfloat162_rn(u, v);
-                y[k] = *reinterpret_cast<const uint32_t *>(&z);
-              } else {
-                y[k] = pack_half2(u, v);
-              }
-            }
-            reinterpret_cast<uint4 *>(dst)[2 * c] = make_uint4(y[0], y[1], y[2], y[3]);
-            reinterpret_cast<uint4 *>(dst)[2 * c + 1] = make_uint4(y[4], y[5], y[6], y[7]);
-          }
+          for (int i = 0; i < 4; ++i) reinterpret_cast<uint4 *>(o)[4 * c + i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
         }
-        if (a.lse && valid) a.lse[(it.first + i0) * (a.kv_heads * a.group) + tok_head] = natural_lse(base, sum);
       }
+      reinterpret_cast<float2 *>(part + kTiles * 128 * D)[t * 128 + r] = make_float2(base, sum);
+    } else {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      uint8_t *dst = a.out + (it.first + i0) * a.o_token_stride + tok_head * a.o_head_stride;
+#pragma unroll 1
+      for (int c = 0; c < D / 16; ++c) {
+        uint32_t x[16];
+        if (chunks) {
+          tmem_load16(x, o_at(t) + lanes + 16 * c);
+          tmem_wait_load(x);
+        }
+        if (valid) {
+          uint32_t y[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float u = sum == 0.0f ? 0.0f : __uint_as_float(x[2 * k]) * inv;
+            const float v = sum == 0.0f ? 0.0f : __uint_as_float(x[2 * k + 1]) * inv;
+            if (BF16) {
+              const __nv_bfloat162 z = __floats2bfloat162_rn(u, v);
+              y[k] = *reinterpret_cast<const uint32_t *>(&z);
+            } else {
+              y[k] = pack_half2(u, v);
+            }
+          }
+          reinterpret_cast<uint4 *>(dst)[2 * c] = make_uint4(y[0], y[1], y[2], y[3]);
+          reinterpret_cast<uint4 *>(dst)[2 * c + 1] = make_uint4(y[4], y[5], y[6], y[7]);
+        }
+      }
+      if (a.lse && valid) a.lse[(it.first + i0) * (a.kv_heads * a.group) + tok_head] = natural_lse(base, sum);
     }
   } else if (warp < 4 * kTiles + kFillWarps) {
     // ---- K and V into shared memory ----
     // Warp w brings unit w of a chunk, 8 tokens at a time, a quarter of a row a lane: 8 lanes that store together
     // have 8 rows, so the swizzle spreads them over all banks.
-    const int w = warp - 4 * kTiles, tok = lane & 7, quarter = lane >> 3;
+    // Where there is no second tile its warps take every second step: four warps alone need 1500 cycles for one,
+    // more than a tile's scores, softmax and products (64 sequences of 4000 tokens, 64 rows: 313 us, so 232).
+    const int w = warp & 3, tok = lane & 7, quarter = lane >> 3;
+    const int by = 3 - tiles, first = warp < 4 * kTiles ? -1 : -2;
     constexpr int kWords = D / 32;  // of a lane's piece, 8 channels each
     const int at_row = tok * (D / 2) + quarter * (D / 8), at_scale = 8 * D + tok * (D / 16) + quarter * (D / 64);
     uint32_t at_chunk[kWords];  // a lane's pieces of a row in shared memory
@@ -1331,7 +1332,7 @@ fp4_many_kernel(const __grid_constant__ AttnArgs a, int blocks, int splits, floa
       const bool good = page >= 0 && page < a.num_blocks;
       unit = good ? a.layer + page * a.block_stride + ((int64_t)h * a.upb + u - e * a.upb) * (9 * D) : nullptr;
       bad = !good && u * 16 < most;
-      page = page_of(j + 1);
+      page = page_of(j + by);
     };
     auto fetch = [&](int j, int side) {
       const uint8_t *p = unit + side * a.kv_stride;
@@ -1372,31 +1373,31 @@ fp4_many_kernel(const __grid_constant__ AttnArgs a, int blocks, int splits, floa
     };
     const uint32_t k_at = smem_addr(sm.k[0]), v_at = smem_addr(sm.v[0]);
     constexpr uint32_t kStage = D / 64 * ManySmem<D>::kCols;
-    // Steps i from -2 on: K of chunk i + 2, then V of chunk i.  Their pieces are loaded a step ahead.
+    // Steps i from -2 on: K of chunk i + 2, then V of chunk i.  Their pieces are loaded a step of the warp's ahead.
     const uint8_t *units[3];  // of the chunks i, i + 1, i + 2
-    page = page_of(0);
-    if (chunks) find(0), fetch(0, 0);
+    page = page_of(first + 2);
+    if (first + 2 < chunks) find(first + 2), fetch(first + 2, 0);
 #pragma unroll 1
-    for (int i = chunks ? -2 : 0; i < chunks; ++i) {
+    for (int i = chunks ? first : 0; i < chunks; i += by) {
       const int slot = (i + 2) & (kRing - 1);
       if (i + 2 >= kRing) patience.wait(&sm.empty[slot], ((i + 2) / kRing + 1) & 1);
       units[0] = units[1], units[1] = units[2], units[2] = unit;
       if (i + 2 < chunks) {
         put(k_at + slot * kStage, 0);
         if (lane == 0) sm.bad[(i + 2) & (2 * kRing - 1)][w] = (uint8_t)bad;  // read before the chunk 2 kRing on gets here
-        if (i + 3 < chunks) find(i + 3), fetch(i + 3, 0);
+        if (i + 2 + by < chunks) find(i + 2 + by), fetch(i + 2 + by, 0);
       }
       if (i >= 0) put(v_at + (i & (kRing - 1)) * kStage, 1);
       fence_async();
       mbar_arrive(&sm.full[slot]);
-      if (i + 1 >= 0 && i + 1 < chunks) {
+      if (i + by >= 0 && i + by < chunks) {
         const uint8_t *keep = unit;
-        unit = units[1];
-        fetch(i + 1, 1);
+        unit = by == 1 ? units[1] : units[2];
+        fetch(i + by, 1);
         unit = keep;
       }
     }
-    if (a.fill_rest) fill_rest(a, D, threadIdx.x - 128 * kTiles, kFillWarps * 32);
+    if (a.fill_rest && warp >= 4 * kTiles) fill_rest(a, D, threadIdx.x - 128 * kTiles, kFillWarps * 32);
   } else {
     // ---- the products: a warp for each tile ----
     // In loops and not straight code: these warps share their instruction caches with three busier ones each.  The
@@ -1570,8 +1571,8 @@ int launch_many(const AttnArgs &a, const ManyPlan &p, void *workspace, cudaStrea
 }
 
 // Rows of a key head up to which the few-rows kernel runs, 16 at a time.  16
-// sequences of 4000 tokens, 8 key heads of 128: 32 rows 62 us there and 82 us in
-// the many-rows kernel (64 sequences: 176 and 315 us), 64 rows 100 and 82 us.
+// sequences of 4000 tokens, 8 key heads of 128: 32 rows 57 us there, 59 in the
+// many-rows kernel (64 sequences: 172 and 232 us); 64 rows 100 and 59 us.
 constexpr int kFewRows = 32;
 int row_tiles(int64_t rows) { return rows <= 8 ? 1 : 2; }
 

@@ -2,8 +2,8 @@
 // the C ABI (include/flexkv_b200.h).  A CPython module on torch's C++ tensors
 // and not ctypes, because these run once per layer and token: reading the
 // tensors' shapes in Python and converting up to 29 arguments took 15 to 20 us
-// a call, several times the smallest kernels; here it takes 3 us, 2.3 of them the
-// launch, and about 1 us for each tensor it allocates.
+// a call, several times the smallest kernels; here it takes 2.5 us, nearly all of
+// them the launch, and about 1 us for each tensor it allocates.
 #include <Python.h>
 
 #include <ATen/ATen.h>
