@@ -1622,6 +1622,7 @@ int fkv_fp4_attention(const void *layer, int64_t num_blocks, int tokens_per_bloc
     return bad("the query heads must be a multiple of the key heads");
   if (num_blocks < 0 || num_q_tokens < 0 || num_seqs < 0 || max_blocks < 0) return bad("counts must be non-negative");
   if (!std::isfinite(softmax_scale)) return bad("softmax_scale must be finite");
+  if (flags & ~(FKV_FP4_CAUSAL | FKV_FP4_FILL_REST)) return bad("unknown flags");
   if (num_q_tokens == 0 || num_seqs == 0) return FKV_OK;
   if (num_q_tokens > INT32_MAX || num_q_tokens * num_q_heads >= INT32_MAX - 65536)
     return bad("2^31 (token, head) rows or more in one call");

@@ -7,6 +7,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -221,7 +222,11 @@ PyObject *read(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const Rows rv = v.defined() ? rows(v, "v", tokens, g.heads, g.dim, type, dev) : Rows{};
     if (args[3] != Py_None) {
       rows_apart(k, "k");
-      if (v.defined()) rows_apart(v, "v");
+      if (v.defined()) {
+        rows_apart(v, "v");
+        const auto both = at::get_overlap_status(k, v);
+        if (tokens && (both == at::MemOverlapStatus::Partial || both == at::MemOverlapStatus::Full)) refuse("k and v overlap");
+      }
     }
     const Tensor ids = slots.contiguous();
     check(lib.read(layer.data_ptr(), g.kv, g.blocks, g.tpb, g.heads, g.dim, g.kv_stride, g.block_stride, k.data_ptr(),
@@ -365,7 +370,11 @@ PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
                  : cu && !seqs ? at::zeros({n, q_heads, g.dim}, q.options())
                                  : at::empty({n, q_heads, g.dim}, q.options());
     const Rows ro = rows(out, "out", n, q_heads, g.dim, q.scalar_type(), dev);
-    if (given) rows_apart(out, "out");
+    if (given) {
+      rows_apart(out, "out");
+      if (at::get_overlap_status(out, q) == at::MemOverlapStatus::Partial)
+        refuse("out may be q itself, but must not overlap it otherwise");
+    }
     Tensor lse;
     if (want_lse)
       lse = cu && !fill ? at::full({n, q_heads}, -INFINITY, q.options().dtype(at::kFloat))

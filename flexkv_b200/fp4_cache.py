@@ -141,7 +141,8 @@ def fp4_attention(layer: torch.Tensor, q: torch.Tensor, block_tables: torch.Tens
     heads, head_size 64 or 128, ``softmax_scale`` 1 / sqrt(head_size) unless
     given.
 
-    Returns ``out`` [tokens, num_q_heads, head_size] of q's type, with
+    Returns ``out`` [tokens, num_q_heads, head_size] of q's type (a given one
+    may be q itself), with
     ``return_lse`` also the natural logarithm of each row's sum of exponentials,
     float32 [tokens, num_q_heads], -inf where it sees nothing.  Rows that belong
     to no sequence are left as they were in a given ``out``, and are zeros

@@ -157,3 +157,9 @@ def test_python_refuses_host_tensors():
             fp4_cache._native().write(*args)
     with pytest.raises(RuntimeError, match="torch.Tensor"):
         fp4_cache.fp4_write([layer], x, x, slots)
+
+
+@pytest.mark.parametrize("flags", [4, -1, 7])
+def test_attention_refuses_unknown_flags(flags):
+    assert _lib.load().fkv_fp4_attention(*attention_args(causal=flags)) == INV
+    assert b"flags" in _lib.load().fkv_last_error()

@@ -769,3 +769,40 @@ def test_forked_streams(new):
         torch.cuda.synchronize()
         for x in (got, eager):
             assert torch.equal(x[0], want) and torch.equal(x[1], want) and torch.equal(x[2], got[2])
+
+
+def test_outputs_that_share_memory_are_refused():
+    layer, slots = garbage(2, 4, 2, 16, 64), torch.arange(5, device="cuda")
+    flat = torch.zeros(6, 2, 64, dtype=torch.bfloat16, device="cuda")
+    tables, lens = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="out may be q"):
+        fp4_cache.fp4_attention(layer, flat[:5], tables, lens, out=flat[1:])
+    assert fp4_cache.fp4_attention(layer, flat[:5], tables, lens, out=flat[:5]) is not None
+    for v in (flat[:5], flat[1:]):
+        with pytest.raises(RuntimeError, match="k and v overlap"):
+            fp4_cache.fp4_read(layer, slots, out=(flat[:5], v))
+    # interleaved sides of one tensor do not overlap
+    both = torch.zeros(5, 2, 2, 64, dtype=torch.bfloat16, device="cuda")
+    fp4_cache.fp4_read(layer, slots, out=(both[:, 0], both[:, 1]))
+
+
+@pytest.mark.parametrize("new", [1, 3, 80])
+def test_graphs_of_one_pool(new):
+    """Two graphs captured into one memory pool, so that they share workspaces, replayed in turn between eager calls."""
+    states = [decode_state(s, lens=(3000, 170), new=new) for s in range(2)]
+    want = [fp4_cache.fp4_attention(*st, new) for st in states]
+    outs = [torch.zeros_like(w) for w in want]
+    torch.cuda.synchronize()
+    graphs = []
+    for st, out in zip(states, outs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if graphs else None):
+            fp4_cache.fp4_attention(*st, new, out=out)
+        graphs.append(graph)
+    for turn in range(6):
+        for out in outs:
+            out.zero_()
+        for i in (0, 1, 1, 0):
+            graphs[i].replay()
+            assert torch.equal(fp4_cache.fp4_attention(*states[i], new), want[i])
+        assert all(torch.equal(out, w) for out, w in zip(outs, want))
