@@ -886,7 +886,8 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
 // on the other, and K and V are converted once for both.  A tile has two
 // buffers for S, so that the next scores are there when a softmax ends.
 // Tensor memory (512 columns): O of both tiles, two S of both; P lies over S.
-// Where the blocks of rows are fewer than the SMs, several CTAs share a block's
+// A block of 128 rows or fewer has one tile; the other's warps help to bring K
+// and V in.  Where the blocks of rows are fewer than the SMs, several CTAs share a block's
 // keys, and a second kernel joins what they have.
 //
 // Measured (B200, bfloat16, heads of 128, 4 query heads to a key head): three

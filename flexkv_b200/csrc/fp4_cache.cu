@@ -11,7 +11,7 @@
 // and is exact in half and bfloat16.  16 tokens of one head are a unit of
 // 9 * D bytes: 16 rows of D / 2 payload bytes (even channel in the low four
 // bits), then 16 rows of D / 16 scale bytes.  A unit is one contiguous,
-// 16-byte aligned piece, so attention fetches it with one bulk copy; a block
+// 16-byte aligned piece, which attention fetches in 16-byte copies; a block
 // holds its units head after head, so a head's share of a block (and a
 // tensor-parallel rank's) is one piece too.
 #include <cuda_bf16.h>
