@@ -45,17 +45,24 @@ struct AttnArgs {
   int fill_rest;  // rows of no sequence: zeros, lse -inf
 };
 
-__device__ __forceinline__ float natural_lse(float m, float l) {  // m: in powers of two
-  return l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
+// A row's sum of weights 2^((s - centre) * mul + kLift) over its scores s, whole or of a part of its keys.
+// What is joined has the row's mul in common; without a key the centre is -inf and the sum 0.
+struct alignas(16) RowSum {
+  float centre, l, mul, unused;
+};
+constexpr float kLift = 7.0f;  // see fp4_decode_kernel's weights
+
+__device__ __forceinline__ float natural_lse(const RowSum &r) {
+  return r.l == 0.0f ? -INFINITY : (fmaf(r.centre, r.mul, -kLift) + __log2f(r.l)) * 0.6931471805599453f;
 }
 
 // N channels from c on of (token, head) row `row` of a sequence.
 template <bool BF16, int N>
 __device__ __forceinline__ void store_row(const AttnArgs &a, int64_t first, int h, int row, int nrows, int c,
-                                          const float (&v)[N], float m, float l) {
+                                          const float (&v)[N], const RowSum &sum) {
   if (row >= nrows) return;
   const int i = row / a.group, qh = h * a.group + row - i * a.group;
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const float inv = sum.l == 0.0f ? 0.0f : 1.0f / sum.l;
   uint32_t w[N / 2];
 #pragma unroll
   for (int k = 0; k < N / 2; ++k) {
@@ -75,7 +82,7 @@ __device__ __forceinline__ void store_row(const AttnArgs &a, int64_t first, int 
   } else {
     *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
   }
-  if (a.lse && c == 0) a.lse[(first + i) * (a.kv_heads * a.group) + qh] = natural_lse(m, l);
+  if (a.lse && c == 0) a.lse[(first + i) * (a.kv_heads * a.group) + qh] = natural_lse(sum);
 }
 
 // Rows before the first sequence and behind the last, this CTA's share of them,
@@ -148,12 +155,16 @@ struct DecodeShape {
   static constexpr int kUps = NT == 2 && D == 64 ? 4 : 2, kStages = 3;
 };
 
-constexpr float kNone = -1e30f;  // a row's base before any key
-// A weight is 2^(score - base).  The base is set 7 below the largest score and
-// moves when one passes it by 15: the largest weight of a row lies between
+// A weight is 2^((s - centre) * mul + kLift): s the sum q k, mul what turns it
+// into a power of two.  The centre is the largest sum when it was set; it moves
+// when one passes it by 8 powers of two: the largest weight of a row lies between
 // 2^7 and 2^15, so its rounding to half (a step of 2^-24 at the least) takes
-// at most 2^-32 of the sum of weights from any weight, however small.
-constexpr float kLift = 7.0f, kMove = 15.0f;
+// at most 2^-32 of the sum of weights from any weight, however small.  The
+// difference is taken first and is nearly exact, in joins too: a product rounded
+// before it, s * mul - base, is off by powers of two where scores pass 2^24, and
+// weights overflowed half there.
+constexpr float kMove = 15.0f;
+constexpr float kLowest = -3.4e38f;  // below every centre but that of a row without keys
 
 struct Item {     // what a warp needs of one sequence
   int len;        // tokens that can be seen: the table's end at most
@@ -352,6 +363,28 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   return r;
 }
 
+// Two floats in a register pair, as the packed instructions take them.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // The power of two that brings a row's largest value to [2^10, 2^11), within
 // what a float holds; its inverse is exact too.
 __device__ __forceinline__ float row_factor(float amax) {
@@ -362,12 +395,23 @@ __device__ __forceinline__ float row_factor(float amax) {
   return __uint_as_float((uint32_t)(k + 127) << 23);
 }
 
+// From a row's q k to powers of two; its bounds keep 0 * mul and s * mul numbers.
+__device__ __forceinline__ float row_mul(float scale, float factor) {
+  return fminf(fmaxf(fabsf(scale) * 1.4426950408889634f * (1.0f / factor), 1e-37f), 3e38f);
+}
+// The sum past which the centre moves: not above centre + 8 / mul, lest a weight pass 2^15.
+__device__ __forceinline__ float bar_of(float centre, float mul) {
+  return __fadd_rd(centre, __fdividef(kMove - kLift, mul));
+}
+// What weights around `from` are around `to`, which is not below it.
+__device__ __forceinline__ float moved(float from, float to, float mul) { return exp2_fast((from - to) * mul); }
+
 // What a warp has of a (sequence, head, row block) that it does not hold whole.
 template <int D, int NT>
 struct Part {
   static constexpr int kPad = D + 4;  // floats of a row: quads store 16-byte pieces of rows 2 t and 2 t + 1
   alignas(16) float o[8 * NT][kPad];
-  float m[8 * NT], l[8 * NT];
+  RowSum sum[8 * NT];
 };
 // The rows a part belongs to, and its place in the line of work.
 struct PartMeta {
@@ -389,7 +433,7 @@ struct DecodeSmem {
 };
 
 template <int D>
-__host__ __device__ constexpr int slot_floats(int rows) { return rows * (D + 2); }
+__host__ __device__ constexpr int slot_floats(int rows) { return rows * (D + 4); }  // and their RowSums
 
 // Joins `count` consecutive warps' parts from that of warp w0 on, whose part
 // is the one in its ring when `ring`: into rows of the output, or into a slot
@@ -403,21 +447,23 @@ __device__ __forceinline__ void join_parts(const AttnArgs &a, const DecodeSmem<D
   };
   for (int i = threadIdx.x; i < R * (D / 4); i += kWarps * 32) {
     const int r = i / (D / 4), c = i % (D / 4) * 4;
-    float M = kNone, L = 0, acc[4] = {};
+    float to = kLowest, acc[4] = {};
 #pragma unroll 4
-    for (int k = 0; k < count; ++k) M = fmaxf(M, part(k).m[r]);
+    for (int k = 0; k < count; ++k) to = fmaxf(to, part(k).sum[r].centre);
+    RowSum all{to, 0, part(0).sum[r].mul};
 #pragma unroll 2
     for (int k = 0; k < count; ++k) {
-      const float f = exp2_fast(part(k).m[r] - M);
+      const RowSum of = part(k).sum[r];
+      const float f = moved(of.centre, to, of.mul);
       const float4 v = *reinterpret_cast<const float4 *>(&part(k).o[r][c]);
-      L += part(k).l[r] * f;
+      all.l += of.l * f;
       acc[0] += v.x * f, acc[1] += v.y * f, acc[2] += v.z * f, acc[3] += v.w * f;
     }
     if (slot) {
       *reinterpret_cast<float4 *>(slot + r * D + c) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-      if (c == 0) slot[R * D + 2 * r] = M, slot[R * D + 2 * r + 1] = L;
+      if (c == 0) reinterpret_cast<RowSum *>(slot + R * D)[r] = all;
     } else {
-      store_row<BF16>(a, pm.first, pm.h, pm.row0 + r, pm.nrows, c, acc, M, L);
+      store_row<BF16>(a, pm.first, pm.h, pm.row0 + r, pm.nrows, c, acc, all);
     }
   }
 }
@@ -551,7 +597,7 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
       const int row0 = cur.rb * R, nrows = cur.it.rows * a.group;  // of the sequence's (token, head) rows
       // queries in half; multiplier and end of the rows 2 t, 2 t + 1
       uint32_t qf[NT][KS][2];
-      float mul[NT][2], bar[NT][2];  // bar: the sum q k past which the row's base moves
+      float mul[NT][2], bar[NT][2];  // bar: the sum q k past which the row's centre moves
       int end[NT][2], lowest = INT32_MAX, highest = 0;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -573,7 +619,7 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
             const float2 y = pair_to_float2<BF16>(x[2 * k + j]);
             qf[n][k][j] = pack_half2(y.x * fs, y.y * fs);
           }
-        const float mine = fmaxf(fabsf(a.scale) * 1.4426950408889634f * (1.0f / f), 1e-37f);
+        const float mine = row_mul(a.scale, f);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           mul[n][j] = __shfl_sync(~0u, mine, (2 * t + j) * 4);
@@ -595,14 +641,14 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
         highest = max(highest, __shfl_xor_sync(~0u, highest, i));
       }
 
-      float o[NT][KS][4], m[NT][2], l[NT][2];
+      float o[NT][KS][4], centre[NT][2], l[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[n][k][i] = 0;
-        m[n][0] = m[n][1] = kNone;
+        centre[n][0] = centre[n][1] = 0;
         l[n][0] = l[n][1] = 0;
       }
 
@@ -690,9 +736,10 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
 #pragma unroll
               for (int i = 4; i < 32; i <<= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, i));
               if (x > bar[n][j]) {  // others stay: a row does not depend on its neighbours
-                const float to = x * mul[n][j] - kLift, f = exp2_fast(m[n][j] - to);
-                m[n][j] = to;
-                bar[n][j] = __fdividef(to + kMove, mul[n][j]);
+                // a row without a key so far has no sums to move, and its centre may lie above
+                const float f = fminf(moved(centre[n][j], x, mul[n][j]), 1.0f);
+                centre[n][j] = x;
+                bar[n][j] = bar_of(x, mul[n][j]);
                 l[n][j] *= f;
 #pragma unroll
                 for (int k = 0; k < KS; ++k) o[n][k][j] *= f, o[n][k][j + 2] *= f;
@@ -706,8 +753,14 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const float x = exp2_fast(fmaf(s[u][n][2 * i], mul[n][0], -m[n][0]));
-              const float y = exp2_fast(fmaf(s[u][n][2 * i + 1], mul[n][1], -m[n][1]));
+              float2 e;
+              if constexpr (NT == 1)  // in pairs: 48 long 133.8 us one by one, 132.0 so; with two tiles 100.4 and 102.6 (64 x 4000, 16 rows)
+                e = unpair(fma2(add2(pair(s[u][n][2 * i], s[u][n][2 * i + 1]), pair(-centre[n][0], -centre[n][1])),
+                                pair(mul[n][0], mul[n][1]), pair(kLift, kLift)));
+              else
+                e = make_float2(fmaf(s[u][n][2 * i] - centre[n][0], mul[n][0], kLift),
+                                fmaf(s[u][n][2 * i + 1] - centre[n][1], mul[n][1], kLift));
+              const float x = exp2_fast(e.x), y = exp2_fast(e.y);
               l[n][0] += x, l[n][1] += y;
               p[n][i] = transpose8(pack_half2(x, y));
             }
@@ -748,17 +801,18 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
 #pragma unroll
           for (int i = 4; i < 32; i <<= 1) sum += __shfl_xor_sync(~0u, sum, i);
           const int rr = n * 8 + 2 * t + j;
+          const RowSum all{bar[n][j] == -INFINITY ? -INFINITY : centre[n][j], sum, mul[n][j]};
           if (starts && ends) {
             float v[D / 8];
 #pragma unroll
             for (int k = 0; k < KS; ++k) v[2 * k] = o[n][k][j], v[2 * k + 1] = o[n][k][j + 2];
-            store_row<BF16>(a, cur.it.first, h, row0 + rr, nrows, g * (D / 8), v, m[n][j], sum);
+            store_row<BF16>(a, cur.it.first, h, row0 + rr, nrows, g * (D / 8), v, all);
           } else {
 #pragma unroll
             for (int k = 0; k < KS; k += 2)
               *reinterpret_cast<float4 *>(&part.o[rr][g * (D / 8) + 2 * k]) =
                   make_float4(o[n][k][j], o[n][k][j + 2], o[n][k + 1][j], o[n][k + 1][j + 2]);
-            if (g == 0) part.m[rr] = m[n][j], part.l[rr] = sum;
+            if (g == 0) part.sum[rr] = all;
           }
         }
       if (!(starts && ends) && lane == 0) {
@@ -818,25 +872,26 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
         for (int n8 = 0; n8 < NT; ++n8) {
           constexpr int kLanes = D / 4, kRows = 32 / kLanes;  // D 64: two rows at a time
           const int c = lane % kLanes * 4;
-          float acc[8 / kRows][4], M[8 / kRows], L[8 / kRows];
+          float acc[8 / kRows][4];
+          RowSum all[8 / kRows];
 #pragma unroll
-          for (int r = 0; r < 8 / kRows; ++r) M[r] = kNone, L[r] = 0, acc[r][0] = acc[r][1] = acc[r][2] = acc[r][3] = 0;
+          for (int r = 0; r < 8 / kRows; ++r) all[r] = {kLowest, 0, 0}, acc[r][0] = acc[r][1] = acc[r][2] = acc[r][3] = 0;
 #pragma unroll 1
           for (int k = warp; k < count; k += kWarps) {
             const float *slot = slot_of(k0 + k * step);
-            float2 ml[8 / kRows];
+            float4 of[8 / kRows];  // a RowSum
             float4 v[8 / kRows];
 #pragma unroll
             for (int r = 0; r < 8 / kRows; ++r) {
               const int rr = n8 * 8 + r * kRows + lane / kLanes;
-              ml[r] = __ldcg(reinterpret_cast<const float2 *>(slot + R * D + 2 * rr));
+              of[r] = __ldcg(reinterpret_cast<const float4 *>(slot + R * D) + rr);
               v[r] = __ldcg(reinterpret_cast<const float4 *>(slot + rr * D + c));
             }
 #pragma unroll
             for (int r = 0; r < 8 / kRows; ++r) {
-              const float m = fmaxf(M[r], ml[r].x), f = exp2_fast(M[r] - m), y = exp2_fast(ml[r].x - m);
-              M[r] = m;
-              L[r] = L[r] * f + ml[r].y * y;
+              const float mul = of[r].z, to = fmaxf(all[r].centre, of[r].x);
+              const float f = moved(all[r].centre, to, mul), y = moved(of[r].x, to, mul);
+              all[r] = {to, all[r].l * f + of[r].y * y, mul};
               acc[r][0] = acc[r][0] * f + v[r].x * y, acc[r][1] = acc[r][1] * f + v[r].y * y;
               acc[r][2] = acc[r][2] * f + v[r].z * y, acc[r][3] = acc[r][3] * f + v[r].w * y;
             }
@@ -845,7 +900,7 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
           for (int r = 0; r < 8 / kRows; ++r) {
             const int rr = n8 * 8 + r * kRows + lane / kLanes;
             *reinterpret_cast<float4 *>(&mine.o[rr][c]) = make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
-            if (c == 0) mine.m[rr] = M[r], mine.l[rr] = L[r];
+            if (c == 0) mine.sum[rr] = all[r];
           }
         }
       }
@@ -879,8 +934,8 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
 //  * one thread for each tile of 128 rows issues its products: S into tensor
 //    memory, and O += P V with P read from there;
 //  * four warps for each tile of rows take S, a thread a row: weights
-//    2^(score - base) in half go back over S as P, their sum stays in the
-//    thread.  The base moves only when a score passes it by kMove, as in the
+//    in half go back over S as P, their sum stays in the thread.  A row's
+//    centre moves only when a score passes it by 8 powers of two, as in the
 //    kernel above: then O is scaled in place.
 // Two tiles of rows alternate: while one is in softmax the tensor core works
 // on the other, and K and V are converted once for both.  A tile has two
@@ -989,27 +1044,6 @@ __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::aft
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// Two floats in a register pair, as the packed instructions take them.
-__device__ __forceinline__ uint64_t pair(float x, float y) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ float2 unpair(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 #define FKV_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
 #define FKV_W8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
 // 16 or 32 columns of the warp's 32 lanes.
@@ -1089,10 +1123,10 @@ __device__ __forceinline__ bool find_block(const AttnArgs &a, int at, int blocks
   return false;
 }
 
-// A row's share of the workspace where the keys are split: its sums, then base
-// and sum of weights.
+// A block's share of the workspace where the keys are split: its rows' O, then
+// their RowSums.
 template <int D>
-__host__ __device__ constexpr int split_floats() { return kTiles * 128 * (D + 2); }
+__host__ __device__ constexpr int split_floats() { return kTiles * 128 * (D + 4); }
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kManyThreads, 1)
@@ -1166,7 +1200,7 @@ fp4_many_kernel(const __grid_constant__ AttnArgs a, int blocks, int splits, floa
         }
       }
       const float f = row_factor(amax), fs = a.scale < 0.0f ? -f : f;
-      mul = fmaxf(fabsf(a.scale) * 1.4426950408889634f * (1.0f / f), 1e-37f);
+      mul = row_mul(a.scale, f);
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) {
         const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
@@ -1184,7 +1218,7 @@ fp4_many_kernel(const __grid_constant__ AttnArgs a, int blocks, int splits, floa
 
     const int end = valid ? end_of(row) : 0;
     const int lowest = __reduce_min_sync(~0u, valid ? end : INT32_MAX);
-    float base = kNone, bar = -INFINITY, l[4] = {0, 0, 0, 0};
+    float centre = 0, bar = -INFINITY, l[4] = {0, 0, 0, 0};
     for (int j = 0; j < chunks; ++j) {
       patience.wait(&sm.s_full[t][j & 1], (j >> 1) & 1);
       fence_after();
@@ -1210,10 +1244,9 @@ fp4_many_kernel(const __grid_constant__ AttnArgs a, int blocks, int splits, floa
       if (__any_sync(~0u, most_here > bar)) {  // rare after the first chunks
         float f = 1.0f;
         if (most_here > bar) {  // other rows stay: a row does not depend on its neighbours
-          const float to = most_here * mul - kLift;
-          f = exp2_fast(base - to);
-          base = to;
-          bar = __fdividef(to + kMove, mul);
+          f = fminf(moved(centre, most_here, mul), 1.0f);  // 1: a row without a key so far
+          centre = most_here;
+          bar = bar_of(centre, mul);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) l[i] *= f;
@@ -1231,14 +1264,15 @@ fp4_many_kernel(const __grid_constant__ AttnArgs a, int blocks, int splits, floa
           }
         }
       }
-      const uint64_t mul2 = pair(mul, mul), base2 = pair(-base, -base);
+      const uint64_t mul2 = pair(mul, mul), from2 = pair(-centre, -centre), lift2 = pair(kLift, kLift);
       uint64_t l01 = pair(l[0], l[1]), l23 = pair(l[2], l[3]);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         uint32_t p[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float2 y = unpair(fma2(pair(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])), mul2, base2));
+          const float2 y =
+              unpair(fma2(add2(pair(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])), from2), mul2, lift2));
           const float u = exp2_fast(y.x), v = exp2_fast(y.y);
           if (i & 1)
             l23 = add2(l23, pair(u, v));
@@ -1274,7 +1308,7 @@ fp4_many_kernel(const __grid_constant__ AttnArgs a, int blocks, int splits, floa
           for (int i = 0; i < 4; ++i) reinterpret_cast<uint4 *>(o)[4 * c + i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
         }
       }
-      reinterpret_cast<float2 *>(part + kTiles * 128 * D)[t * 128 + r] = make_float2(base, sum);
+      reinterpret_cast<RowSum *>(part + kTiles * 128 * D)[t * 128 + r] = {bar == -INFINITY ? -INFINITY : centre, sum, mul};
     } else {
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
       uint8_t *dst = a.out + (it.first + i0) * a.o_token_stride + tok_head * a.o_head_stride;
@@ -1302,7 +1336,7 @@ fp4_many_kernel(const __grid_constant__ AttnArgs a, int blocks, int splits, floa
           reinterpret_cast<uint4 *>(dst)[2 * c + 1] = make_uint4(y[4], y[5], y[6], y[7]);
         }
       }
-      if (a.lse && valid) a.lse[(it.first + i0) * (a.kv_heads * a.group) + tok_head] = natural_lse(base, sum);
+      if (a.lse && valid) a.lse[(it.first + i0) * (a.kv_heads * a.group) + tok_head] = natural_lse({centre, sum, mul});
     }
   } else if (warp < 4 * kTiles + kFillWarps) {
     // ---- K and V into shared memory ----
@@ -1469,23 +1503,24 @@ __global__ void __launch_bounds__(256) fp4_merge_kernel(const __grid_constant__ 
   const Item it = item_of<R>(a, b);
   const int row = rb * R + r, nrows = it.rows * a.group;
   if (row >= nrows) return;
-  float M = kNone, L = 0, acc[kVec] = {};
+  RowSum all{kLowest, 0, 0};
+  float acc[kVec] = {};
 #pragma unroll 4
   for (int s = 0; s < splits; ++s) {
     const float *part = parts + ((int64_t)(at * splits + s) * a.kv_heads + h) * split_floats<D>();
-    const float2 ml = reinterpret_cast<const float2 *>(part + R * D)[r];
+    const RowSum of = reinterpret_cast<const RowSum *>(part + R * D)[r];
     float v[kVec] = {};
-    if (ml.y != 0.0f) {  // a part without keys has no sums
+    if (of.l != 0.0f) {  // a part without keys has no sums
 #pragma unroll
       for (int i = 0; i < kVec; ++i) v[i] = part[r * D + lane * kVec + i];
     }
-    const float to = fmaxf(M, ml.x), f = exp2_fast(M - to), y = exp2_fast(ml.x - to);
-    M = to, L = L * f + ml.y * y;
+    const float to = fmaxf(all.centre, of.centre), f = moved(all.centre, to, of.mul), y = moved(of.centre, to, of.mul);
+    all = {to, all.l * f + of.l * y, of.mul};
 #pragma unroll
     for (int i = 0; i < kVec; ++i) acc[i] = acc[i] * f + v[i] * y;
   }
   const int i0 = row / a.group, qh = h * a.group + row - i0 * a.group;
-  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  const float inv = all.l == 0.0f ? 0.0f : 1.0f / all.l;
   uint8_t *dst = a.out + (it.first + i0) * a.o_token_stride + qh * a.o_head_stride + lane * kVec * 2;
 #pragma unroll
   for (int i = 0; i < kVec; i += 2) {
@@ -1494,7 +1529,7 @@ __global__ void __launch_bounds__(256) fp4_merge_kernel(const __grid_constant__ 
     else
       reinterpret_cast<uint32_t *>(dst)[i / 2] = pack_half2(acc[i] * inv, acc[i + 1] * inv);
   }
-  if (a.lse && lane == 0) a.lse[(it.first + i0) * (a.kv_heads * a.group) + qh] = natural_lse(M, L);
+  if (a.lse && lane == 0) a.lse[(it.first + i0) * (a.kv_heads * a.group) + qh] = natural_lse(all);
 }
 
 // A number of 48 bits for each launch, from a start that differs between processes.
