@@ -205,6 +205,12 @@ _SIGNATURES = {
     "fkv_fp4_unpack_blocks": (
         c_int, [c_int, c_vp, c_vp, c_int, c_int, c_int, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64,
                 c_int, c_vp, c_vp, c_i64, c_vp]),
+    "fkv_fp4_pack_blocks_listed": (
+        c_int, [c_int, c_vp, c_vp, c_int, c_int, c_int, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64,
+                c_int, c_vp, c_vp, c_i64, c_int, c_vp]),
+    "fkv_fp4_unpack_blocks_listed": (
+        c_int, [c_int, c_vp, c_vp, c_int, c_int, c_int, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64,
+                c_int, c_vp, c_vp, c_i64, c_int, c_vp]),
     "fkv_fp4_wait_timeouts": (c_int, [P_i64]),
     "fkv_fp4_attention_workspace": (c_i64, [c_i64, c_int, c_int, c_int, c_int, c_int]),
     "fkv_fp4_attention": (

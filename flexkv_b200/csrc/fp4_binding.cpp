@@ -35,6 +35,8 @@ struct {
   decltype(&::fkv_fp4_read) read;
   decltype(&::fkv_fp4_pack_blocks) pack_blocks;
   decltype(&::fkv_fp4_unpack_blocks) unpack_blocks;
+  decltype(&::fkv_fp4_pack_blocks_listed) pack_blocks_listed;
+  decltype(&::fkv_fp4_unpack_blocks_listed) unpack_blocks_listed;
   decltype(&::fkv_fp4_attention_workspace) attention_workspace;
   decltype(&::fkv_fp4_attention) attention;
 } lib;
@@ -242,7 +244,7 @@ PyObject *read(PyObject *, PyObject *const *args, Py_ssize_t n) {
   });
 }
 
-// Block ids on the device; host ids are checked first.
+// Block ids, contiguous, where they are; host ids are checked.
 Tensor block_ids(const Tensor &t, const char *name, int64_t pool, const at::Device &dev, bool distinct) {
   if (t.scalar_type() != at::kLong || t.dim() != 1) refuse(name, " must be a 1-D ", at::kLong, " tensor");
   if (t.is_cuda()) {
@@ -258,7 +260,7 @@ Tensor block_ids(const Tensor &t, const char *name, int64_t pool, const at::Devi
     std::sort(ids.begin(), ids.end());
     if (std::adjacent_find(ids.begin(), ids.end()) != ids.end()) refuse(name, ": a block id appears twice");
   }
-  return c.to(dev);
+  return c;
 }
 
 // convert(pack, kv_layers, fp4_layers, kv_block_ids, fp4_block_ids)
@@ -300,17 +302,22 @@ PyObject *convert(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const c10::cuda::CUDAGuard guard(dev);
     const Tensor kids = block_ids(ka, "kv_block_ids", k0.size(1), dev, !pack);
     const Tensor fids = block_ids(fa, "fp4_block_ids", g.blocks, dev, pack);
+    const int host = (kids.is_cuda() ? 0 : FKV_FP4_KV_IDS) | (fids.is_cuda() ? 0 : FKV_FP4_FP4_IDS);
     const int64_t ks = g.kv > 1 ? 2 * k0.stride(0) : 0, kb = k0.size(1) > 1 ? 2 * k0.stride(1) : 0;
-    if (pack)
-      check(lib.pack_blocks((int)layers, kp.data(), fp.data(), g.kv, g.tpb, g.heads, g.dim, k0.size(1), ks, kb, g.blocks,
-                                g.kv_stride, g.block_stride, dt, kids.data_ptr<int64_t>(), fids.data_ptr<int64_t>(),
-                                kids.numel(), stream_of(dev)),
-            "fp4_pack_blocks");
+    const int64_t n = kids.numel(), *ki = kids.data_ptr<int64_t>(), *fi = fids.data_ptr<int64_t>();
+    void *const stream = stream_of(dev);
+    const char *const who = pack ? "fp4_pack_blocks" : "fp4_unpack_blocks";
+    auto call = [&](auto pack_blocks, auto unpack_blocks, auto... lists) {
+      check(pack ? pack_blocks((int)layers, kp.data(), fp.data(), g.kv, g.tpb, g.heads, g.dim, k0.size(1), ks, kb, g.blocks,
+                               g.kv_stride, g.block_stride, dt, ki, fi, n, lists..., stream)
+                 : unpack_blocks((int)layers, fp.data(), kp.data(), g.kv, g.tpb, g.heads, g.dim, g.blocks, g.kv_stride,
+                                 g.block_stride, k0.size(1), ks, kb, dt, fi, ki, n, lists..., stream),
+            who);
+    };
+    if (host)
+      call(lib.pack_blocks_listed, lib.unpack_blocks_listed, host);
     else
-      check(lib.unpack_blocks((int)layers, fp.data(), kp.data(), g.kv, g.tpb, g.heads, g.dim, g.blocks, g.kv_stride,
-                                  g.block_stride, k0.size(1), ks, kb, dt, fids.data_ptr<int64_t>(),
-                                  kids.data_ptr<int64_t>(), kids.numel(), stream_of(dev)),
-            "fp4_unpack_blocks");
+      call(lib.pack_blocks, lib.unpack_blocks);
     Py_RETURN_NONE;
   });
   Py_XDECREF(fps);

@@ -17,6 +17,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "fkv_common.h"
 #include "fp4_format.cuh"
 #include "fp4_launch.cuh"
@@ -25,11 +27,19 @@ namespace fkv {
 namespace {
 
 constexpr int kMaxLayers = 128;  // layers of one launch: their pointers travel in the kernel's parameters
+constexpr int kMaxListed = 256;  // pairs of blocks of one launch whose ids travel there too
 constexpr int kThreads = 256;
 constexpr int kUnroll = 4;
 
-// LAYERS: what the call's pointers need; they are copied with every launch.
-template <int LAYERS>
+// Tokens by slot; blocks whose ids are in device memory; blocks of which one
+// list of ids or both come from the host, in the parameters: nothing has to be
+// copied to the device first, and a captured launch keeps its ids.  9 blocks of 28
+// layers there and back take 8.4 us so, with ids on the device 7.4 (the larger
+// parameters); 1000 blocks of one layer, four launches each way, 40 and 26.
+enum Form { kTokens, kBlocks, kListed };
+
+// LAYERS, PAIRS: what the call's pointers and ids need; they are copied with every launch.
+template <int LAYERS, int PAIRS>
 struct RowsArgsOf {
   int num_heads;
   int kv_dim;
@@ -44,13 +54,14 @@ struct RowsArgsOf {
   int64_t fp4_kv_stride, fp4_block_stride;
   int64_t token_stride[2], head_stride[2];        // bytes, 16-bit side
   int64_t row_block_stride;                        // bytes, block form
-  const int64_t *fp4_ids;                          // slots (token form) or blocks
-  const int64_t *row_ids;                          // blocks of the 16-bit side (block form)
+  const int64_t *fp4_ids;                          // slots (token form) or blocks; null: listed[0]
+  const int64_t *row_ids;                          // blocks of the 16-bit side (block form); null: listed[1]
   uint8_t *fp4[LAYERS];
   uint8_t *rows[2][LAYERS];
+  int64_t listed[2][PAIRS];
 };
-template <bool BLOCKS>
-using RowsArgs = RowsArgsOf<BLOCKS ? kMaxLayers : 1>;
+template <int FORM>
+using RowsArgs = RowsArgsOf<FORM == kTokens ? 1 : kMaxLayers, FORM == kListed ? kMaxListed : 1>;
 
 // 32 bytes in one access where the address allows it, else two of 16.
 template <bool WIDE>
@@ -91,8 +102,8 @@ __device__ __forceinline__ void store_group(uint8_t *p, const uint32_t (&r)[8]) 
 // With divisions for each group's place and true ones in the rounding, 9 blocks of
 // 28 layers there and back took 9.9 us instead of 6.9, and quantising was bound by
 // the issue of 315 instructions a group.
-template <bool WRITE, bool BF16, bool BLOCKS, bool WIDE, int NG, int R>
-__global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constant__ RowsArgs<BLOCKS> a) {
+template <bool WRITE, bool BF16, int FORM, bool WIDE, int NG, int R>
+__global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constant__ RowsArgs<FORM> a) {
   after_previous();
   const int ng = NG ? NG : a.groups, D = 16 * ng;
   const int layer = a.kv_dim == 1 ? blockIdx.y : blockIdx.y >> 1, side = a.kv_dim == 1 ? 0 : blockIdx.y & 1;
@@ -107,12 +118,13 @@ __global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constan
     const int64_t i = row0 + t;
     unit = row = nullptr;
     if (i >= a.num_rows) return;
-    if (BLOCKS) {
+    if (FORM != kTokens) {
       // a block's rows are multiples of 16, R = 16: row 0 says which block
       const int64_t u = row0 >> 4;
       const int64_t blk = a.far ? u / a.upb : divide((int)u, a.by_upb);
       const int in = (int)(u - blk * a.upb);
-      const int64_t fb = a.fp4_ids[blk], rb = a.row_ids[blk];
+      const int64_t fb = FORM == kListed && !a.fp4_ids ? a.listed[0][blk] : a.fp4_ids[blk];
+      const int64_t rb = FORM == kListed && !a.row_ids ? a.listed[1][blk] : a.row_ids[blk];
       if (fb < 0 || fb >= a.num_blocks || rb < 0 || rb >= a.num_row_blocks) return;
       off = t;
       unit = fp4 + fb * a.fp4_block_stride + (int64_t)in * (9 * D);
@@ -196,26 +208,26 @@ __global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constan
   }
 }
 
-template <bool WRITE, bool BF16, bool BLOCKS, bool WIDE, int R>
-cudaError_t launch_ng(const RowsArgs<BLOCKS> &a, dim3 grid, int ng, cudaStream_t s) {
+template <bool WRITE, bool BF16, int FORM, bool WIDE, int R>
+cudaError_t launch_ng(const RowsArgs<FORM> &a, dim3 grid, int ng, cudaStream_t s) {
   switch (ng) {
-    case 4: return launch_next(fp4_rows_kernel<WRITE, BF16, BLOCKS, WIDE, 4, R>, grid, kThreads, 0, s, a);
-    case 8: return launch_next(fp4_rows_kernel<WRITE, BF16, BLOCKS, WIDE, 8, R>, grid, kThreads, 0, s, a);
-    case 16: return launch_next(fp4_rows_kernel<WRITE, BF16, BLOCKS, WIDE, 16, R>, grid, kThreads, 0, s, a);
-    default: return launch_next(fp4_rows_kernel<WRITE, BF16, BLOCKS, WIDE, 0, R>, grid, kThreads, 0, s, a);
+    case 4: return launch_next(fp4_rows_kernel<WRITE, BF16, FORM, WIDE, 4, R>, grid, kThreads, 0, s, a);
+    case 8: return launch_next(fp4_rows_kernel<WRITE, BF16, FORM, WIDE, 8, R>, grid, kThreads, 0, s, a);
+    case 16: return launch_next(fp4_rows_kernel<WRITE, BF16, FORM, WIDE, 16, R>, grid, kThreads, 0, s, a);
+    default: return launch_next(fp4_rows_kernel<WRITE, BF16, FORM, WIDE, 0, R>, grid, kThreads, 0, s, a);
   }
 }
-template <bool WRITE, bool BF16, bool BLOCKS, bool WIDE>
-cudaError_t launch_r(const RowsArgs<BLOCKS> &a, int rows_at_once, dim3 grid, int ng, cudaStream_t s) {
-  if (BLOCKS || rows_at_once == 16)
-    return launch_ng<WRITE, BF16, BLOCKS, WIDE, 16>(a, grid, ng, s);
-  return launch_ng<WRITE, BF16, BLOCKS, WIDE, BLOCKS ? 16 : 1>(a, grid, ng, s);
+template <bool WRITE, bool BF16, int FORM, bool WIDE>
+cudaError_t launch_r(const RowsArgs<FORM> &a, int rows_at_once, dim3 grid, int ng, cudaStream_t s) {
+  if (FORM != kTokens || rows_at_once == 16)
+    return launch_ng<WRITE, BF16, FORM, WIDE, 16>(a, grid, ng, s);
+  return launch_ng<WRITE, BF16, FORM, WIDE, FORM != kTokens ? 16 : 1>(a, grid, ng, s);
 }
-template <bool WRITE, bool BLOCKS>
-cudaError_t launch_rows(const RowsArgs<BLOCKS> &a, bool bf16, bool wide, int r, dim3 grid, int ng, cudaStream_t s) {
+template <bool WRITE, int FORM>
+cudaError_t launch_rows(const RowsArgs<FORM> &a, bool bf16, bool wide, int r, dim3 grid, int ng, cudaStream_t s) {
   if (bf16)
-    return wide ? launch_r<WRITE, true, BLOCKS, true>(a, r, grid, ng, s) : launch_r<WRITE, true, BLOCKS, false>(a, r, grid, ng, s);
-  return wide ? launch_r<WRITE, false, BLOCKS, true>(a, r, grid, ng, s) : launch_r<WRITE, false, BLOCKS, false>(a, r, grid, ng, s);
+    return wide ? launch_r<WRITE, true, FORM, true>(a, r, grid, ng, s) : launch_r<WRITE, true, FORM, false>(a, r, grid, ng, s);
+  return wide ? launch_r<WRITE, false, FORM, true>(a, r, grid, ng, s) : launch_r<WRITE, false, FORM, false>(a, r, grid, ng, s);
 }
 
 int check_geometry(const char *who, int kv_dim, int64_t num_blocks, int tpb, int heads, int head_size, int dtype) {
@@ -235,8 +247,8 @@ int check_geometry(const char *who, int kv_dim, int64_t num_blocks, int tpb, int
 bool aligned(int64_t v, int64_t to) { return v % to == 0; }
 bool aligned(const void *p, int64_t to) { return (uintptr_t)p % to == 0; }
 
-template <bool WRITE, bool BLOCKS>
-int run_rows(RowsArgs<BLOCKS> &a, int num_layers, int head_size, int dtype, bool wide, cudaStream_t s) {
+template <bool WRITE, int FORM>
+int run_rows(RowsArgs<FORM> &a, int num_layers, int head_size, int dtype, bool wide, cudaStream_t s) {
   const int ng = head_size / 16, r = a.num_rows < 16 ? 1 : 16;
   a.upb = a.tokens_per_block / 16, a.groups = ng;
   a.far = a.num_slots >> 32 || a.num_rows >> 32 || a.upb > 4096;
@@ -245,7 +257,7 @@ int run_rows(RowsArgs<BLOCKS> &a, int num_layers, int head_size, int dtype, bool
   // grid.x counts row groups: 2^31 - 1 of them is the launch limit
   const int64_t gx = (a.num_rows + r - 1) / r;
   if (gx > INT32_MAX) return fail(FKV_ERR_INVALID_ARG, "more than 2^31 groups of rows in one call");
-  FKV_CUDA((launch_rows<WRITE, BLOCKS>(a, dtype == FKV_DTYPE_BF16, wide, r, dim3((unsigned)gx, num_layers * a.kv_dim), ng, s)));
+  FKV_CUDA((launch_rows<WRITE, FORM>(a, dtype == FKV_DTYPE_BF16, wide, r, dim3((unsigned)gx, num_layers * a.kv_dim), ng, s)));
   note_launch();
   return FKV_OK;
 }
@@ -266,7 +278,7 @@ int tokens_call(const char *who, void *layer, int kv_dim, int64_t num_blocks, in
   if (kv_dim == 1 && v) return fail(FKV_ERR_INVALID_ARG, w + ": a latent layer (kv_dim 1) has no values");
   if (!aligned(layer, 16) || !aligned(kv_stride, 16) || !aligned(block_stride, 16))
     return fail(FKV_ERR_MISALIGNED, w + ": the layer and its strides must be multiples of 16 bytes");
-  RowsArgs<false> a{};
+  RowsArgs<kTokens> a{};
   a.num_heads = heads, a.kv_dim = kv_dim, a.tokens_per_block = tpb;
   a.num_rows = num_tokens, a.num_slots = num_blocks * tpb;
   a.fp4_kv_stride = kv_stride, a.fp4_block_stride = block_stride;
@@ -281,20 +293,22 @@ int tokens_call(const char *who, void *layer, int kv_dim, int64_t num_blocks, in
       return fail(FKV_ERR_MISALIGNED, w + ": rows must start on 16-byte boundaries");
     wide = wide && aligned(a.rows[i][0], 32) && aligned(a.token_stride[i], 32) && aligned(a.head_stride[i], 32);
   }
-  return run_rows<WRITE, false>(a, 1, head_size, dtype, wide, (cudaStream_t)stream);
+  return run_rows<WRITE, kTokens>(a, 1, head_size, dtype, wide, (cudaStream_t)stream);
 }
 
-template <bool WRITE>
+// host_lists: which ids are in host memory (kListed)
+template <bool WRITE, int FORM>
 int blocks_call(const char *who, int num_layers, void *const *fp4_layers, void *const *kv_layers, int kv_dim, int tpb,
                 int heads, int head_size, int64_t fp4_num_blocks, int64_t fp4_kv_stride, int64_t fp4_block_stride,
                 int64_t kv_num_blocks, int64_t kv_kv_stride, int64_t kv_block_stride, int dtype, const int64_t *fp4_ids,
-                const int64_t *kv_ids, int64_t num, void *stream) {
+                const int64_t *kv_ids, int64_t num, int host_lists, void *stream) {
   clear_error();
   int rc = check_geometry(who, kv_dim, fp4_num_blocks, tpb, heads, head_size, dtype);
   if (rc != FKV_OK) return rc;
   const std::string w(who);
   if (num < 0 || num_layers < 0 || kv_num_blocks < 0 || num > INT64_MAX / tpb)
     return fail(FKV_ERR_INVALID_ARG, w + ": counts must be non-negative");
+  if (host_lists & ~(FKV_FP4_KV_IDS | FKV_FP4_FP4_IDS)) return fail(FKV_ERR_INVALID_ARG, w + ": unknown host_lists");
   if (num == 0 || num_layers == 0) return FKV_OK;
   if (!fp4_layers || !kv_layers || !fp4_ids || !kv_ids) return fail(FKV_ERR_INVALID_ARG, w + ": null pointer");
   if (!aligned(fp4_kv_stride, 16) || !aligned(fp4_block_stride, 16) || !aligned(kv_kv_stride, 16) ||
@@ -307,13 +321,12 @@ int blocks_call(const char *who, int num_layers, void *const *fp4_layers, void *
       return fail(FKV_ERR_MISALIGNED, w + ": layers must start on 16-byte boundaries");
     wide = wide && aligned(kv_layers[l], 32);
   }
-  RowsArgs<true> a{};
+  RowsArgs<FORM> a{};
   a.num_heads = heads, a.kv_dim = kv_dim, a.tokens_per_block = tpb;
-  a.num_rows = num * tpb, a.num_slots = fp4_num_blocks * tpb, a.num_blocks = fp4_num_blocks, a.num_row_blocks = kv_num_blocks;
+  a.num_slots = fp4_num_blocks * tpb, a.num_blocks = fp4_num_blocks, a.num_row_blocks = kv_num_blocks;
   a.fp4_kv_stride = fp4_kv_stride, a.fp4_block_stride = fp4_block_stride;
   a.row_block_stride = kv_block_stride;
   for (int i = 0; i < 2; ++i) a.head_stride[i] = 2 * head_size, a.token_stride[i] = (int64_t)2 * head_size * heads;
-  a.fp4_ids = fp4_ids, a.row_ids = kv_ids;
   for (int l0 = 0; l0 < num_layers; l0 += kMaxLayers) {
     const int n = num_layers - l0 < kMaxLayers ? num_layers - l0 : kMaxLayers;
     for (int l = 0; l < n; ++l) {
@@ -321,7 +334,16 @@ int blocks_call(const char *who, int num_layers, void *const *fp4_layers, void *
       a.rows[0][l] = (uint8_t *)kv_layers[l0 + l];
       a.rows[1][l] = (uint8_t *)kv_layers[l0 + l] + kv_kv_stride;
     }
-    if ((rc = run_rows<WRITE, true>(a, n, head_size, dtype, wide, (cudaStream_t)stream)) != FKV_OK) return rc;
+    const int64_t step = FORM == kListed ? kMaxListed : num;
+    for (int64_t i = 0; i < num; i += step) {
+      const int64_t pairs = std::min(num - i, step);
+      a.num_rows = pairs * tpb;
+      a.fp4_ids = host_lists & FKV_FP4_FP4_IDS ? nullptr : fp4_ids + i;
+      a.row_ids = host_lists & FKV_FP4_KV_IDS ? nullptr : kv_ids + i;
+      if (FORM == kListed && !a.fp4_ids) std::copy_n(fp4_ids + i, pairs, a.listed[0]);
+      if (FORM == kListed && !a.row_ids) std::copy_n(kv_ids + i, pairs, a.listed[1]);
+      if ((rc = run_rows<WRITE, FORM>(a, n, head_size, dtype, wide, (cudaStream_t)stream)) != FKV_OK) return rc;
+    }
   }
   return FKV_OK;
 }
@@ -356,21 +378,50 @@ int fkv_fp4_pack_blocks(int num_layers, void *const *kv_layer_ptrs, void *const 
                         int64_t kv_kv_stride_in_bytes, int64_t kv_block_stride_in_bytes, int64_t fp4_num_blocks,
                         int64_t fp4_kv_stride_in_bytes, int64_t fp4_block_stride_in_bytes, int dtype,
                         const int64_t *kv_block_ids, const int64_t *fp4_block_ids, int64_t num_blocks, void *stream) {
-  return fkv::blocks_call<true>("fkv_fp4_pack_blocks", num_layers, fp4_layer_ptrs, kv_layer_ptrs, kv_dim,
-                                tokens_per_block, num_heads, head_size, fp4_num_blocks, fp4_kv_stride_in_bytes,
-                                fp4_block_stride_in_bytes, kv_num_blocks, kv_kv_stride_in_bytes,
-                                kv_block_stride_in_bytes, dtype, fp4_block_ids, kv_block_ids, num_blocks, stream);
+  return fkv::blocks_call<true, fkv::kBlocks>("fkv_fp4_pack_blocks", num_layers, fp4_layer_ptrs, kv_layer_ptrs,
+                                              kv_dim, tokens_per_block, num_heads, head_size, fp4_num_blocks,
+                                              fp4_kv_stride_in_bytes, fp4_block_stride_in_bytes, kv_num_blocks,
+                                              kv_kv_stride_in_bytes, kv_block_stride_in_bytes, dtype, fp4_block_ids,
+                                              kv_block_ids, num_blocks, 0, stream);
+}
+
+int fkv_fp4_pack_blocks_listed(int num_layers, void *const *kv_layer_ptrs, void *const *fp4_layer_ptrs, int kv_dim,
+                               int tokens_per_block, int num_heads, int head_size, int64_t kv_num_blocks,
+                               int64_t kv_kv_stride_in_bytes, int64_t kv_block_stride_in_bytes,
+                               int64_t fp4_num_blocks, int64_t fp4_kv_stride_in_bytes,
+                               int64_t fp4_block_stride_in_bytes, int dtype, const int64_t *kv_block_ids,
+                               const int64_t *fp4_block_ids, int64_t num_blocks, int host_lists, void *stream) {
+  return fkv::blocks_call<true, fkv::kListed>("fkv_fp4_pack_blocks_listed", num_layers, fp4_layer_ptrs, kv_layer_ptrs,
+                                              kv_dim, tokens_per_block, num_heads, head_size, fp4_num_blocks,
+                                              fp4_kv_stride_in_bytes, fp4_block_stride_in_bytes, kv_num_blocks,
+                                              kv_kv_stride_in_bytes, kv_block_stride_in_bytes, dtype, fp4_block_ids,
+                                              kv_block_ids, num_blocks, host_lists, stream);
 }
 
 int fkv_fp4_unpack_blocks(int num_layers, void *const *fp4_layer_ptrs, void *const *kv_layer_ptrs, int kv_dim,
                           int tokens_per_block, int num_heads, int head_size, int64_t fp4_num_blocks,
                           int64_t fp4_kv_stride_in_bytes, int64_t fp4_block_stride_in_bytes, int64_t kv_num_blocks,
                           int64_t kv_kv_stride_in_bytes, int64_t kv_block_stride_in_bytes, int dtype,
-                          const int64_t *fp4_block_ids, const int64_t *kv_block_ids, int64_t num_blocks, void *stream) {
-  return fkv::blocks_call<false>("fkv_fp4_unpack_blocks", num_layers, fp4_layer_ptrs, kv_layer_ptrs, kv_dim,
-                                 tokens_per_block, num_heads, head_size, fp4_num_blocks, fp4_kv_stride_in_bytes,
-                                 fp4_block_stride_in_bytes, kv_num_blocks, kv_kv_stride_in_bytes,
-                                 kv_block_stride_in_bytes, dtype, fp4_block_ids, kv_block_ids, num_blocks, stream);
+                          const int64_t *fp4_block_ids, const int64_t *kv_block_ids, int64_t num_blocks,
+                          void *stream) {
+  return fkv::blocks_call<false, fkv::kBlocks>("fkv_fp4_unpack_blocks", num_layers, fp4_layer_ptrs, kv_layer_ptrs,
+                                               kv_dim, tokens_per_block, num_heads, head_size, fp4_num_blocks,
+                                               fp4_kv_stride_in_bytes, fp4_block_stride_in_bytes, kv_num_blocks,
+                                               kv_kv_stride_in_bytes, kv_block_stride_in_bytes, dtype, fp4_block_ids,
+                                               kv_block_ids, num_blocks, 0, stream);
+}
+
+int fkv_fp4_unpack_blocks_listed(int num_layers, void *const *fp4_layer_ptrs, void *const *kv_layer_ptrs, int kv_dim,
+                                 int tokens_per_block, int num_heads, int head_size, int64_t fp4_num_blocks,
+                                 int64_t fp4_kv_stride_in_bytes, int64_t fp4_block_stride_in_bytes,
+                                 int64_t kv_num_blocks, int64_t kv_kv_stride_in_bytes,
+                                 int64_t kv_block_stride_in_bytes, int dtype, const int64_t *fp4_block_ids,
+                                 const int64_t *kv_block_ids, int64_t num_blocks, int host_lists, void *stream) {
+  return fkv::blocks_call<false, fkv::kListed>("fkv_fp4_unpack_blocks_listed", num_layers, fp4_layer_ptrs,
+                                               kv_layer_ptrs, kv_dim, tokens_per_block, num_heads, head_size,
+                                               fp4_num_blocks, fp4_kv_stride_in_bytes, fp4_block_stride_in_bytes,
+                                               kv_num_blocks, kv_kv_stride_in_bytes, kv_block_stride_in_bytes, dtype,
+                                               fp4_block_ids, kv_block_ids, num_blocks, host_lists, stream);
 }
 
 }  // extern "C"

@@ -48,7 +48,8 @@ __all__ = ["allocate_fp4_layers", "fp4_write", "fp4_read", "fp4_pack_blocks", "f
 UNIT_TOKENS = 16
 
 _ENTRY_POINTS = ("fkv_last_error", "fkv_fp4_write", "fkv_fp4_read", "fkv_fp4_pack_blocks",
-                 "fkv_fp4_unpack_blocks", "fkv_fp4_attention_workspace", "fkv_fp4_attention")
+                 "fkv_fp4_unpack_blocks", "fkv_fp4_pack_blocks_listed", "fkv_fp4_unpack_blocks_listed",
+                 "fkv_fp4_attention_workspace", "fkv_fp4_attention")
 _lock = threading.Lock()
 _module = None
 
@@ -109,9 +110,11 @@ def fp4_pack_blocks(kv_layers: Sequence[torch.Tensor], fp4_layers: Sequence[torc
                     kv_block_ids: torch.Tensor, fp4_block_ids: torch.Tensor) -> None:
     """Quantise blocks ``kv_block_ids[i]`` of a 16-bit cache (one tensor [kv,
     blocks, tokens_per_block, num_heads, head_size] per layer) into blocks
-    ``fp4_block_ids[i]`` of ``fp4_layers``, all layers in one launch.  Ids
-    (int64) may be host tensors, which are checked, or device tensors, where a
-    pair with an id outside its pool is skipped.  No destination may repeat."""
+    ``fp4_block_ids[i]`` of ``fp4_layers``, all layers in one launch (128 of
+    them, and with ids on the host 256 blocks).  Ids (int64) may be host
+    tensors, which are checked and read before the call returns (a captured
+    graph keeps them), or device tensors, where a pair with an id outside its
+    pool is skipped.  No destination may repeat."""
     _native().convert(True, kv_layers, fp4_layers, kv_block_ids, fp4_block_ids)
 
 

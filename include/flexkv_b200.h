@@ -600,8 +600,9 @@ int fkv_cache_index_stats(fkv_cache_index *ci, int64_t *out, void *stream);
  *
  * All of these only enqueue work on `stream`, whose device must be current,
  * allocate nothing and can be captured into a graph.  Ids, slots, tables and
- * lengths are device memory and are checked in the kernels: what points
- * outside a pool is skipped as described, never accessed.
+ * lengths are device memory (the _listed calls' ids: host memory) and are
+ * checked in the kernels: what points outside a pool is skipped as described,
+ * never accessed.
  * ---------------------------------------------------------------------- */
 #define FKV_DTYPE_BF16 0
 #define FKV_DTYPE_FP16 1
@@ -648,6 +649,26 @@ int fkv_fp4_unpack_blocks(int num_layers, void *const *fp4_layer_ptrs, void *con
                           int64_t kv_kv_stride_in_bytes, int64_t kv_block_stride_in_bytes, int dtype,
                           const int64_t *fp4_block_ids, const int64_t *kv_block_ids, int64_t num_blocks,
                           void *stream);
+/* Both with ids in host memory: those of the 16-bit side, of the 4-bit side or
+ * of both, as host_lists says.  They are read before the call returns and
+ * travel in the kernels' parameters, 256 pairs a launch: nothing is copied or
+ * waited for, and a captured call keeps its ids. */
+#define FKV_FP4_KV_IDS 1
+#define FKV_FP4_FP4_IDS 2
+int fkv_fp4_pack_blocks_listed(int num_layers, void *const *kv_layer_ptrs, void *const *fp4_layer_ptrs,
+                               int kv_dim, int tokens_per_block, int num_heads, int head_size,
+                               int64_t kv_num_blocks, int64_t kv_kv_stride_in_bytes,
+                               int64_t kv_block_stride_in_bytes, int64_t fp4_num_blocks,
+                               int64_t fp4_kv_stride_in_bytes, int64_t fp4_block_stride_in_bytes,
+                               int dtype, const int64_t *kv_block_ids, const int64_t *fp4_block_ids,
+                               int64_t num_blocks, int host_lists, void *stream);
+int fkv_fp4_unpack_blocks_listed(int num_layers, void *const *fp4_layer_ptrs, void *const *kv_layer_ptrs,
+                                 int kv_dim, int tokens_per_block, int num_heads, int head_size,
+                                 int64_t fp4_num_blocks, int64_t fp4_kv_stride_in_bytes,
+                                 int64_t fp4_block_stride_in_bytes, int64_t kv_num_blocks,
+                                 int64_t kv_kv_stride_in_bytes, int64_t kv_block_stride_in_bytes,
+                                 int dtype, const int64_t *fp4_block_ids, const int64_t *kv_block_ids,
+                                 int64_t num_blocks, int host_lists, void *stream);
 
 /* Attention of new tokens over a 4-bit layer (kv_dim 2), head_size 64 or 128.
  * q and out: num_q_tokens rows of num_q_heads vectors of `dtype` (token and
