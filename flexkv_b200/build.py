@@ -21,6 +21,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_DIR = os.path.join(PKG_DIR, "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libflexkv_b200.so")
 BINDING = os.path.join(CSRC, "fp4_binding.cpp")  # the 4-bit cache's operators on torch tensors
+BINDING_HEADERS = [os.path.join(CSRC, "fp4_overlap.h"), os.path.join(REPO_DIR, "include", "flexkv_b200.h")]
 BINDING_PATH = os.path.join(LIB_DIR, "_fp4.so")
 SOURCES = ["fkv_common.cpp", "transfer.cu", "tp_group.cpp", "xxh64.cu", "engine.cpp", "ipc.cpp", "ssd.cpp",
            "block_index.cu", "fp4_cache.cu", "fp4_attention.cu"]
@@ -75,7 +76,7 @@ def _build_binding(verbose: bool) -> None:
 def _binding_stale() -> bool:
     if not os.path.exists(BINDING_PATH):
         return True
-    deps = [BINDING, os.path.join(REPO_DIR, "include", "flexkv_b200.h"), os.path.abspath(__file__)]
+    deps = [BINDING, *BINDING_HEADERS, os.path.abspath(__file__)]
     return any(os.path.getmtime(d) > os.path.getmtime(BINDING_PATH) for d in deps)
 
 

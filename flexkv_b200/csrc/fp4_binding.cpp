@@ -7,7 +7,6 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
-#include <ATen/MemoryOverlap.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -23,6 +22,7 @@
 #include <vector>
 
 #include "../../include/flexkv_b200.h"
+#include "fp4_overlap.h"
 
 namespace {
 
@@ -121,6 +121,10 @@ void rows_apart(const Tensor &t, const char *name) {
   const bool heads_inside = heads <= 1 || (head >= D && (n <= 1 || token >= (heads - 1) * head + D));
   const bool tokens_inside = n <= 1 || (token >= D && (heads <= 1 || head >= (n - 1) * token + D));
   if (!heads_inside && !tokens_inside) refuse(name, ": rows overlap");
+}
+// The rows of t as a set, for two outputs or an input and an output.
+fkv::RowSet row_set(const Tensor &t, const Rows &r) {
+  return {(uintptr_t)t.data_ptr(), t.size(0), t.size(1), r.token, r.head, 2 * t.size(2)};
 }
 void blocks_apart(const Tensor &t, int64_t block, const char *name) {
   const int64_t kv = t.stride(0), blk = t.stride(1), n = t.size(1), sides = t.size(0);
@@ -226,8 +230,7 @@ PyObject *read(PyObject *, PyObject *const *args, Py_ssize_t n) {
       rows_apart(k, "k");
       if (v.defined()) {
         rows_apart(v, "v");
-        const auto both = at::get_overlap_status(k, v);
-        if (tokens && (both == at::MemOverlapStatus::Partial || both == at::MemOverlapStatus::Full)) refuse("k and v overlap");
+        if (fkv::rows_share_memory(row_set(k, rk), row_set(v, rv))) refuse("k and v overlap");
       }
     }
     const Tensor ids = slots.contiguous();
@@ -379,7 +382,8 @@ PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     const Rows ro = rows(out, "out", n, q_heads, g.dim, q.scalar_type(), dev);
     if (given) {
       rows_apart(out, "out");
-      if (at::get_overlap_status(out, q) == at::MemOverlapStatus::Partial)
+      const fkv::RowSet from = row_set(q, rq), to = row_set(out, ro);
+      if (!from.same_place(to) && fkv::rows_share_memory(from, to))
         refuse("out may be q itself, but must not overlap it otherwise");
     }
     Tensor lse;

@@ -104,3 +104,73 @@ def test_host_ids_in_a_graph(n):
         fp4_cache.fp4_pack_blocks(src, p, a, b)
         fp4_cache.fp4_unpack_blocks(p, d, b, c)
         assert all(torch.equal(x, y) for x, y in zip(packed + dst, p + d))
+
+
+# ---- outputs that share memory --------------------------------------------------------------------------------
+
+
+@pytest.fixture(scope="module")
+def share_memory(tmp_path_factory):
+    """rows_share_memory of csrc/fp4_overlap.h, on plain numbers."""
+    import os
+    import subprocess
+    from flexkv_b200.build import CSRC
+    d = tmp_path_factory.mktemp("overlap")
+    (d / "o.cpp").write_text('#include "fp4_overlap.h"\nextern "C" int share(const int64_t *a, const int64_t *b) {\n'
+                             '  auto s = [](const int64_t *x) { return fkv::RowSet{(uintptr_t)x[0], x[1], x[2], x[3], x[4], x[5]}; };\n'
+                             '  return fkv::rows_share_memory(s(a), s(b));\n}\n')
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-shared", "-fPIC", "-I", CSRC, "-o", str(d / "o.so"), str(d / "o.cpp")], check=True)
+    f = ctypes.CDLL(os.path.join(d, "o.so")).share
+    return lambda a, b: bool(f((ctypes.c_int64 * 6)(*a), (ctypes.c_int64 * 6)(*b)))
+
+
+def pieces(base, tokens, heads, token, head, nbytes):
+    at = base + np.arange(tokens)[:, None] * token + np.arange(heads) * head
+    return set((at.reshape(-1, 1) + np.arange(nbytes)).reshape(-1).tolist())
+
+
+def test_rows_that_share_memory(share_memory):
+    """Against every byte of both sets: equal and unlike strides, interleaved, self-overlapping, single rows."""
+    r = np.random.RandomState(0)
+    seen = [0, 0, 0, 0]
+    for _ in range(6000):
+        tokens, heads, nbytes = r.randint(0, 6), r.randint(1, 5), r.choice([4, 8])
+        strides = lambda: (int(r.randint(0, 12)) * 4 if tokens > 1 else 0, int(r.randint(0, 12)) * 4 if heads > 1 else 0)  # noqa: E731
+        (ta, ha), (tb, hb) = strides(), strides()
+        alike = r.rand() < 0.6
+        if alike:
+            tb, hb = ta, ha
+        a = (1000, tokens, heads, ta, ha, nbytes)
+        b = (1000 + int(r.randint(-20, 21)) * 4, tokens, heads, tb, hb, nbytes)
+        want = bool(pieces(*a) & pieces(*b))
+        assert share_memory(a, b) == want and share_memory(b, a) == want, (a, b, want)
+        seen[2 * want + alike] += 1
+    assert min(seen) > 100
+    far = 1 << 45  # no product passes 64 bits at real sizes
+    assert not share_memory((far, 32768, 8, 12288, 256, 256), (far + 2048, 32768, 8, 12288, 256, 256))
+    assert share_memory((far, 32768, 8, 12288, 256, 256), (far + 12288 * 32767 + 1792, 32768, 8, 12288, 256, 256))
+    assert not share_memory((far, 32768, 8, 12288, 256, 256), (far + 12288 * 32768 + 1792, 32768, 8, 12288, 256, 256))
+    assert share_memory((far, 1 << 25, 2, 256, 128, 128), (far, 1 << 25, 2, 128, 1 << 32, 128))
+
+
+@pytest.mark.gpu
+def test_strided_outputs_that_share_memory_are_refused():
+    layer, slots = torch.zeros(2, 4, 4, 1, 9 * 64, dtype=torch.uint8, device="cuda"), torch.arange(5, device="cuda")
+    buf = torch.zeros(6, 8, 64, dtype=torch.bfloat16, device="cuda")
+    tables, lens = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda")
+
+    def attend(q, out):
+        return fp4_cache.fp4_attention(layer, q, tables, lens, out=out)
+    for q, out in ((buf[:5, :4], buf[1:, :4]), (buf[:5, :4], buf[:5, 2:6]), (buf[:5, ::2], buf[:5, :4]),
+                   (buf[:1, :4], buf[:1, 3:7]), (buf[:4, :4].transpose(0, 1), buf[:4, :4])):
+        with pytest.raises(RuntimeError, match="out may be q"):
+            attend(q, out)
+        with pytest.raises(RuntimeError, match="k and v overlap"):
+            fp4_cache.fp4_read(layer, slots[:q.shape[0]], out=(q, out))
+    with pytest.raises(RuntimeError, match="k and v overlap"):
+        fp4_cache.fp4_read(layer, slots, out=(buf[:5, :4], buf[:5, :4]))
+    # side by side, interleaved, far apart, the same place
+    for q, out in ((buf[:5, :4], buf[:5, 4:]), (buf[:5, ::2], buf[:5, 1::2]), (buf[:2, :4], buf[2:4, :4])):
+        attend(q, out)
+        fp4_cache.fp4_read(layer, slots[:q.shape[0]], out=(q, out))
+    attend(buf[:5, :4], buf[:5, :4])
