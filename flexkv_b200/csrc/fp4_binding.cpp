@@ -300,6 +300,10 @@ PyObject *convert(PyObject *, PyObject *const *args, Py_ssize_t n) {
       no_grad({&k});
       kp[i] = k.data_ptr(), fp[i] = f.data_ptr();
     }
+    std::vector<void *> to = pack ? fp : kp;
+    std::sort(to.begin(), to.end());
+    if ((pack ? f0 : k0).numel() && std::adjacent_find(to.begin(), to.end()) != to.end())
+      refuse(pack ? "fp4_layers" : "kv_layers", ": a layer to write to appears twice");
     const Tensor &ka = tensor(args[3], "kv_block_ids"), &fa = tensor(args[4], "fp4_block_ids");
     if (ka.numel() != fa.numel()) refuse("kv_block_ids and fp4_block_ids differ in length");
     const c10::cuda::CUDAGuard guard(dev);

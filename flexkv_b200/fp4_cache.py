@@ -114,7 +114,7 @@ def fp4_pack_blocks(kv_layers: Sequence[torch.Tensor], fp4_layers: Sequence[torc
     them, and with ids on the host 256 blocks).  Ids (int64) may be host
     tensors, which are checked and read before the call returns (a captured
     graph keeps them), or device tensors, where a pair with an id outside its
-    pool is skipped.  No destination may repeat."""
+    pool is skipped.  No destination may repeat, neither a block nor a layer."""
     _native().convert(True, kv_layers, fp4_layers, kv_block_ids, fp4_block_ids)
 
 

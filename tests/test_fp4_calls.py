@@ -174,3 +174,21 @@ def test_strided_outputs_that_share_memory_are_refused():
         attend(q, out)
         fp4_cache.fp4_read(layer, slots[:q.shape[0]], out=(q, out))
     attend(buf[:5, :4], buf[:5, :4])
+
+
+@pytest.mark.gpu
+def test_a_layer_is_written_once():
+    """The same tensor twice among the layers to write to is refused; to read from it is fine."""
+    src, packed, dst, (a, b, _) = converted(4, 3)
+    for lists in ([packed[0], packed[1], packed[0]], [packed[0], packed[0].view(packed[0].shape), packed[1]]):
+        with pytest.raises(RuntimeError, match="fp4_layers: a layer to write to appears twice"):
+            fp4_cache.fp4_pack_blocks(src, lists, a, b)
+    with pytest.raises(RuntimeError, match="kv_layers: a layer to write to appears twice"):
+        fp4_cache.fp4_unpack_blocks(packed, [dst[2], dst[1], dst[2]], b, a)
+    assert all(bool((x == 255).all()) for x in packed) and all(bool((x == 5.0).all()) for x in dst)
+    fp4_cache.fp4_pack_blocks([src[0], src[0], src[1]], packed, a, b)
+    assert torch.equal(packed[0], packed[1]) and not torch.equal(packed[0], packed[2])
+    fp4_cache.fp4_unpack_blocks([packed[0], packed[0], packed[2]], dst, b, a)
+    assert torch.equal(dst[0], dst[1])
+    empty = [x[:, :0] for x in packed]
+    fp4_cache.fp4_pack_blocks(src, empty, a[:0], b[:0])
