@@ -26,6 +26,7 @@ BINDING_PATH = os.path.join(LIB_DIR, "_fp4.so")
 SOURCES = ["fkv_common.cpp", "transfer.cu", "tp_group.cpp", "xxh64.cu", "engine.cpp", "ipc.cpp", "ssd.cpp",
            "block_index.cu", "fp4_cache.cu", "fp4_attention.cu"]
 HEADERS = [os.path.join(CSRC, "fkv_common.h"), os.path.join(CSRC, "fp4_format.cuh"), os.path.join(CSRC, "fp4_launch.cuh"),
+           os.path.join(CSRC, "fp4_wait.cuh"),
            os.path.join(REPO_DIR, "include", "flexkv_b200.h")]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

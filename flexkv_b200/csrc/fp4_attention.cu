@@ -16,6 +16,7 @@
 #include "fkv_common.h"
 #include "fp4_format.cuh"
 #include "fp4_launch.cuh"
+#include "fp4_wait.cuh"
 
 namespace fkv {
 namespace {
@@ -308,7 +309,6 @@ struct Walk {
   __device__ int chunk_units() const { return min(kUps, u1 - at); }
 };
 
-__device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void copy16(uint32_t dst, const uint8_t *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -972,36 +972,6 @@ struct ManySmem {
   uint32_t tmem;
 };
 
-__device__ __forceinline__ void mbar_init(uint64_t *m, int count) {
-  asm volatile("mbarrier.init.shared.b64 [%0], %1;" ::"r"(smem_addr(m)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t *m) {
-  asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(smem_addr(m)) : "memory");
-}
-__device__ __forceinline__ bool mbar_try(uint64_t *m, int parity) {
-  int ok;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n selp.b32 %0, 1, 0, p;\n}"
-      : "=r"(ok)
-      : "r"(smem_addr(m)), "r"(parity)
-      : "memory");
-  return ok;
-}
-// A wait has a limit (a try that fails lasts 4 us, the whole of them a second).
-// One that runs out is counted (fkv_fp4_wait_timeouts) and the kernel goes on as
-// if it had come, each later wait with a single try: it ends, and its output is
-// not to be used.
-__device__ unsigned long long g_wait_timeouts;
-struct Patience {
-  int tries = 1 << 18;
-  __device__ __forceinline__ void wait(uint64_t *m, int parity) {
-    for (int i = 0; i < tries; ++i)
-      if (mbar_try(m, parity)) return;
-    if (tries > 1) atomicAdd(&g_wait_timeouts, 1ull);
-    tries = 1;
-  }
-};
-
 // A shared memory operand in the 128-byte swizzled layout.  K-major: 8 rows of
 // 128 bytes every 1024 bytes.  MN-major: 8 rows along K every 1024 bytes, the
 // next 64 columns a block of kKeys rows further.
@@ -1623,6 +1593,7 @@ int fkv_fp4_wait_timeouts(int64_t *count) {
   clear_error();
   if (!count) return fail(FKV_ERR_INVALID_ARG, "fkv_fp4_wait_timeouts: null pointer");
   unsigned long long n = 0;
+  FKV_CUDA(cudaDeviceSynchronize());  // the copy alone does not wait for streams that are not blocking
   FKV_CUDA(cudaMemcpyFromSymbol(&n, g_wait_timeouts, sizeof(n)));
   *count = (int64_t)n;
   return FKV_OK;

@@ -43,7 +43,7 @@ from .build import BINDING_PATH
 from .layout import KVCacheLayout, KVCacheLayoutType
 
 __all__ = ["allocate_fp4_layers", "fp4_write", "fp4_read", "fp4_pack_blocks", "fp4_unpack_blocks",
-           "fp4_attention"]
+           "fp4_attention", "fp4_wait_timeouts"]
 
 UNIT_TOKENS = 16
 
@@ -149,6 +149,19 @@ def fp4_attention(layer: torch.Tensor, q: torch.Tensor, block_tables: torch.Tens
     ``return_lse`` also the natural logarithm of each row's sum of exponentials,
     float32 [tokens, num_q_heads], -inf where it sees nothing.  Rows that belong
     to no sequence are left as they were in a given ``out``, and are zeros
-    (lse: -inf) in a new one."""
+    (lse: -inf) in a new one.  Waits inside the kernel have a limit;
+    ``fp4_wait_timeouts`` tells whether one ran out."""
     return _native().attention(layer, q, block_tables, seq_lens, cu_seqlens_q, max_q_len, softmax_scale, causal, out,
                                return_lse)
+
+
+def fp4_wait_timeouts(device=None) -> int:
+    """How many waits between the warps of ``fp4_attention``'s kernels ran out
+    of their limit (about a second) on ``device`` (the current one unless given)
+    since the process began: 0 unless something is wrong.  A kernel whose wait
+    runs out ends all the same, and what it wrote is not to be used.  Waits for
+    the device; not for capturing."""
+    n = ctypes.c_int64()
+    with torch.cuda.device(device):
+        _lib.check(_lib.load().fkv_fp4_wait_timeouts(ctypes.byref(n)), "fp4_wait_timeouts")
+    return n.value

@@ -705,7 +705,7 @@ int fkv_fp4_attention(const void *layer, int64_t num_blocks, int tokens_per_bloc
 /* Waits between the warps of an attention kernel that ran out of their limit
  * (about a second) on the current device so far: 0 unless something is wrong;
  * the output of a call that counts any is not to be used.  Waits for the
- * device. */
+ * device, for what runs on any of its streams. */
 int fkv_fp4_wait_timeouts(int64_t *count);
 
 #ifdef __cplusplus
