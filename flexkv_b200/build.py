@@ -10,10 +10,13 @@ memory per kernel) is written next to it as ptxas.txt.
 from __future__ import annotations
 
 import argparse
+import importlib.metadata
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
+import warnings
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
@@ -22,7 +25,6 @@ LIB_DIR = os.path.join(PKG_DIR, "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libflexkv_b200.so")
 BINDING = os.path.join(CSRC, "fp4_binding.cpp")  # the 4-bit cache's operators on torch tensors
 BINDING_HEADERS = [os.path.join(CSRC, "fp4_overlap.h"), os.path.join(REPO_DIR, "include", "flexkv_b200.h")]
-BINDING_PATH = os.path.join(LIB_DIR, "_fp4.so")
 SOURCES = ["fkv_common.cpp", "transfer.cu", "tp_group.cpp", "xxh64.cu", "engine.cpp", "ipc.cpp", "ssd.cpp",
            "block_index.cu", "fp4_cache.cu", "fp4_attention.cu"]
 HEADERS = [os.path.join(CSRC, "fkv_common.h"), os.path.join(CSRC, "fp4_format.cuh"), os.path.join(CSRC, "fp4_launch.cuh"),
@@ -46,17 +48,47 @@ def _stale() -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def binding_path() -> str:
+    """Where the 4-bit cache's CPython module is for this interpreter and this
+    torch: its layouts of tensors and exceptions are those of the headers it
+    was built with, so another version gets a module of its own."""
+    if "torch" in sys.modules:
+        torch = sys.modules["torch"].__version__
+    else:  # a build with nothing to do need not import it
+        try:
+            torch = importlib.metadata.version("torch")
+        except importlib.metadata.PackageNotFoundError:
+            torch = "none"
+    return os.path.join(LIB_DIR, f"_fp4.{sysconfig.get_config_var('SOABI')}.torch-{torch}.so")
+
+
+def _binding_includes() -> list:
+    import torch.utils.cpp_extension
+
+    return [sysconfig.get_paths()["include"], *torch.utils.cpp_extension.include_paths()]
+
+
+def _binding_lacks() -> str:
+    """What the module cannot be built without and is not there; the library
+    needs neither."""
+    try:
+        inc = _binding_includes()
+    except ImportError as e:
+        return str(e)
+    for header in ("Python.h", os.path.join("torch", "csrc", "autograd", "python_variable.h")):
+        if not any(os.path.exists(os.path.join(d, header)) for d in inc):
+            return f"{header} not found"
+    return ""
+
+
 def _build_binding(verbose: bool) -> None:
     """The CPython module of the 4-bit cache's operators, against this
     interpreter and the installed torch."""
-    import sysconfig
-
     import torch
-    from torch.utils.cpp_extension import include_paths
 
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
-    inc = [sysconfig.get_paths()["include"], *include_paths()]
-    tmp = BINDING_PATH + ".tmp"
+    inc = _binding_includes()
+    tmp = binding_path() + ".tmp"
     # The C++ library has to be the shared one that torch uses: a second copy, linked statically as some
     # compilers' defaults have it, ends the process at the first stream or exception that meets the other.
     cmd = [
@@ -71,20 +103,28 @@ def _build_binding(verbose: bool) -> None:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed ({res.returncode}):\n{res.stderr[-4000:]}")
-    os.replace(tmp, BINDING_PATH)
+    os.replace(tmp, binding_path())
 
 
 def _binding_stale() -> bool:
-    if not os.path.exists(BINDING_PATH):
+    path = binding_path()
+    if not os.path.exists(path):
         return True
     deps = [BINDING, *BINDING_HEADERS, os.path.abspath(__file__)]
-    return any(os.path.getmtime(d) > os.path.getmtime(BINDING_PATH) for d in deps)
+    return any(os.path.getmtime(d) > os.path.getmtime(path) for d in deps)
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
+    """Builds what is out of date; returns the library's path.  Without the
+    headers of Python or torch the library alone is built, with a warning:
+    ``fp4_cache`` then raises ImportError when it is used."""
     lib = _build_lib(force, verbose)
     if force or _binding_stale():
-        _build_binding(verbose)
+        lacks = _binding_lacks()
+        if lacks:
+            warnings.warn(f"flexkv_b200.fp4_cache is not built: {lacks}")
+        else:
+            _build_binding(verbose)
     return lib
 
 

@@ -39,7 +39,7 @@ from typing import List, Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from .build import BINDING_PATH
+from .build import binding_path
 from .layout import KVCacheLayout, KVCacheLayoutType
 
 __all__ = ["allocate_fp4_layers", "fp4_write", "fp4_read", "fp4_pack_blocks", "fp4_unpack_blocks",
@@ -60,10 +60,11 @@ def _native():
     if _module is None:
         with _lock:
             if _module is None:
-                if not os.path.exists(BINDING_PATH):
-                    raise ImportError(f"{BINDING_PATH} not found; build it with `python -m flexkv_b200.build`")
-                loader = importlib.machinery.ExtensionFileLoader("flexkv_b200._fp4", BINDING_PATH)
-                spec = importlib.util.spec_from_file_location("flexkv_b200._fp4", BINDING_PATH, loader=loader)
+                path = binding_path()
+                if not os.path.exists(path):
+                    raise ImportError(f"{path} not found; build it with `python -m flexkv_b200.build`")
+                loader = importlib.machinery.ExtensionFileLoader("flexkv_b200._fp4", path)
+                spec = importlib.util.spec_from_file_location("flexkv_b200._fp4", path, loader=loader)
                 module = importlib.util.module_from_spec(spec)
                 loader.exec_module(module)
                 lib = _lib.load()

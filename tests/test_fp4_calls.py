@@ -192,3 +192,33 @@ def test_a_layer_is_written_once():
     assert torch.equal(dst[0], dst[1])
     empty = [x[:, :0] for x in packed]
     fp4_cache.fp4_pack_blocks(src, empty, a[:0], b[:0])
+
+
+# ---- the module they are in -----------------------------------------------------------------------------------
+
+
+def test_the_module_belongs_to_one_torch_and_python(monkeypatch):
+    """Another version of either is not served by what was built for this one."""
+    import sysconfig
+    from flexkv_b200 import build
+    path = build.binding_path()
+    assert torch.__version__ in path and sysconfig.get_config_var("SOABI") in path
+    assert not build._binding_stale()
+    monkeypatch.setattr(torch, "__version__", "2.99.0+cu999")
+    assert build.binding_path() != path and build._binding_stale()
+    monkeypatch.setattr(fp4_cache, "_module", None)
+    with pytest.raises(ImportError, match="2.99.0.cu999.*flexkv_b200.build"):
+        fp4_cache._native()
+
+
+def test_the_library_is_built_without_torchs_headers(monkeypatch, tmp_path):
+    from flexkv_b200 import build
+    assert build._binding_lacks() == ""
+    monkeypatch.setattr(build, "_binding_stale", lambda: True)
+    monkeypatch.setattr(build, "_binding_includes", lambda: [str(tmp_path)])
+    monkeypatch.setattr(build, "_build_binding", lambda verbose: pytest.fail("built without its headers"))
+    with pytest.warns(UserWarning, match="fp4_cache is not built: Python.h not found"):
+        assert build.build() == build.LIB_PATH
+    (tmp_path / "Python.h").write_text("")
+    with pytest.warns(UserWarning, match="python_variable.h not found"):
+        build.build()
