@@ -140,6 +140,11 @@ void no_grad(std::initializer_list<const Tensor *> ts) {
     if (t && t->requires_grad()) refuse("the 4-bit cache has no gradient: call under torch.no_grad()");
 }
 
+// After a call that writes t: a backward pass that kept its old content must not run.
+void written(const Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 void *stream_of(const at::Device &dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
 
 void *data(const Tensor *t) { return t ? t->data_ptr() : nullptr; }
@@ -195,6 +200,7 @@ PyObject *write(PyObject *, PyObject *const *args, Py_ssize_t n) {
     check(lib.write(layer.data_ptr(), g.kv, g.blocks, g.tpb, g.heads, g.dim, g.kv_stride, g.block_stride, k.data_ptr(),
                         data(v), rk.token, rk.head, rv.token, rv.head, dt, ids.data_ptr<int64_t>(), tokens, stream_of(dev)),
           "fp4_write");
+    written(layer);
     Py_RETURN_NONE;
   });
 }
@@ -238,6 +244,10 @@ PyObject *read(PyObject *, PyObject *const *args, Py_ssize_t n) {
                        v.defined() ? v.data_ptr() : nullptr, rk.token, rk.head, rv.token, rv.head, dt,
                        ids.data_ptr<int64_t>(), tokens, stream_of(dev)),
           "fp4_read");
+    if (args[3] != Py_None) {
+      written(k);
+      if (v.defined()) written(v);
+    }
     PyObject *pk = THPVariable_Wrap(k);
     PyObject *pv = v.defined() ? THPVariable_Wrap(v) : Py_NewRef(Py_None);
     PyObject *out = pk && pv ? PyTuple_Pack(2, pk, pv) : nullptr;
@@ -325,6 +335,7 @@ PyObject *convert(PyObject *, PyObject *const *args, Py_ssize_t n) {
       call(lib.pack_blocks_listed, lib.unpack_blocks_listed, host);
     else
       call(lib.pack_blocks, lib.unpack_blocks);
+    for (Py_ssize_t i = 0; i < layers; ++i) written(tensor(PySequence_Fast_GET_ITEM(pack ? fps : kvs, i), "a layer"));
     Py_RETURN_NONE;
   });
   Py_XDECREF(fps);
@@ -409,6 +420,7 @@ PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
                             (causal ? FKV_FP4_CAUSAL : 0) | (fill ? FKV_FP4_FILL_REST : 0),
                             bytes > 0 ? workspace.data_ptr() : nullptr, bytes, stream_of(dev)),
           "fp4_attention");
+    if (given) written(out);
     PyObject *po = given ? Py_NewRef(args[8]) : THPVariable_Wrap(out);
     if (!want_lse || !po) return po;
     PyObject *pl = THPVariable_Wrap(lse);

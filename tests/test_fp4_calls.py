@@ -222,3 +222,44 @@ def test_the_library_is_built_without_torchs_headers(monkeypatch, tmp_path):
     (tmp_path / "Python.h").write_text("")
     with pytest.warns(UserWarning, match="python_variable.h not found"):
         build.build()
+
+
+# ---- beside autograd ------------------------------------------------------------------------------------------
+
+
+def small():
+    layer = torch.zeros(2, 4, 2, 1, 9 * 64, dtype=torch.uint8, device="cuda")
+    x = torch.randn(5, 2, 64, device="cuda").bfloat16()
+    return layer, x, torch.arange(5, device="cuda"), torch.zeros(1, 1, dtype=torch.int32, device="cuda"), \
+        torch.full((1,), 5, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.gpu
+def test_what_is_written_gets_a_new_version():
+    """A backward pass that kept a tensor which a call has since written is refused by autograd."""
+    layer, x, slots, tables, lens = small()
+    kv, ids = [torch.zeros(2, 4, 16, 2, 64, dtype=x.dtype, device="cuda")], torch.arange(2)
+
+    def writes(t, call):
+        w = torch.ones((), device="cuda", requires_grad=True)
+        y = (w * t).sum()
+        call()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    out, other = torch.zeros_like(x), torch.zeros_like(x)
+    writes(layer, lambda: fp4_cache.fp4_write(layer, x, x, slots))
+    writes(out, lambda: fp4_cache.fp4_read(layer, slots, out=(out, other)))
+    writes(other, lambda: fp4_cache.fp4_read(layer, slots, out=(out, other)))
+    writes(out, lambda: fp4_cache.fp4_attention(layer, x, tables, lens, out=out))
+    writes(layer, lambda: fp4_cache.fp4_pack_blocks(kv, [layer], ids, ids))
+    writes(kv[0], lambda: fp4_cache.fp4_unpack_blocks([layer], kv, ids, ids))
+    # what is only read stays as it was, and tensors of inference mode have no version
+    w = torch.ones((), device="cuda", requires_grad=True)
+    y = (w * x).sum() + (w * layer).sum()
+    fp4_cache.fp4_read(layer, slots)
+    fp4_cache.fp4_attention(layer, x, tables, lens)
+    y.backward()
+    with torch.inference_mode():
+        layer2, x2, *rest = small()
+        fp4_cache.fp4_write(layer2, x2, x2, rest[0])
+        fp4_cache.fp4_read(layer2, rest[0], out=(x2, torch.zeros_like(x2)))
