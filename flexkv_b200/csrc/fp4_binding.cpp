@@ -7,6 +7,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -134,10 +135,14 @@ void blocks_apart(const Tensor &t, int64_t block, const char *name) {
   if (!sides_inside && !blocks_inside) refuse(name, ": blocks overlap");
 }
 
+// Nothing here is differentiable: what records a gradient, or carries a tangent, is refused.
 void no_grad(std::initializer_list<const Tensor *> ts) {
-  if (!c10::GradMode::is_enabled()) return;
-  for (const Tensor *t : ts)
-    if (t && t->requires_grad()) refuse("the 4-bit cache has no gradient: call under torch.no_grad()");
+  const bool backward = c10::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  for (const Tensor *t : ts) {
+    if (!t) continue;
+    if (backward && t->requires_grad()) refuse("the 4-bit cache has no gradient: call under torch.no_grad()");
+    if (forward && t->_fw_grad(0).defined()) refuse("the 4-bit cache has no gradient: an input has a tangent");
+  }
 }
 
 // After a call that writes t: a backward pass that kept its old content must not run.

@@ -263,3 +263,21 @@ def test_what_is_written_gets_a_new_version():
         layer2, x2, *rest = small()
         fp4_cache.fp4_write(layer2, x2, x2, rest[0])
         fp4_cache.fp4_read(layer2, rest[0], out=(x2, torch.zeros_like(x2)))
+
+
+@pytest.mark.gpu
+def test_tangents_are_refused():
+    import torch.autograd.forward_ad as fw
+    layer, x, slots, tables, lens = small()
+    with fw.dual_level():
+        d = fw.make_dual(x, torch.ones_like(x))
+        with torch.no_grad():
+            for call in (lambda: fp4_cache.fp4_write(layer, d, x, slots), lambda: fp4_cache.fp4_write(layer, x, d, slots),
+                         lambda: fp4_cache.fp4_attention(layer, d, tables, lens),
+                         lambda: fp4_cache.fp4_pack_blocks([fw.make_dual(torch.zeros(2, 4, 16, 2, 64, device="cuda").bfloat16(),
+                                                                         torch.ones(2, 4, 16, 2, 64, device="cuda").bfloat16())],
+                                                           [layer], slots[:1], slots[:1])):
+                with pytest.raises(RuntimeError, match="tangent"):
+                    call()
+        fp4_cache.fp4_write(layer, x, x, slots)
+    assert not bool((layer == 0).all())
