@@ -281,3 +281,45 @@ def test_tangents_are_refused():
                     call()
         fp4_cache.fp4_write(layer, x, x, slots)
     assert not bool((layer == 0).all())
+
+
+# ---- several threads ------------------------------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+def test_threads():
+    """Every operator from several threads at once, each on a stream of its own: what one thread alone gets."""
+    import threading
+
+    def work(seed, stream, turns, out):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        with torch.cuda.stream(stream):
+            layer = torch.zeros(2, 70, 2, 1, 9 * 64, dtype=torch.uint8, device="cuda")
+            kv = torch.zeros(2, 70, 16, 2, 64, dtype=torch.bfloat16, device="cuda")
+            tables = torch.randperm(70, generator=g, device="cuda")[:66].view(2, 33).int()
+            lens = torch.tensor([500, 177 + seed], dtype=torch.int32, device="cuda")
+            rows = torch.randn(1120, 2, 64, generator=g, device="cuda").bfloat16()
+            slots = torch.randperm(1120, generator=g, device="cuda")
+            ids = torch.arange(40)
+            for turn in range(turns):
+                fp4_cache.fp4_write(layer, rows, rows, slots)
+                got = [fp4_cache.fp4_attention(layer, torch.randn(2 * n, 4, 64, generator=g, device="cuda").bfloat16(), tables, lens)
+                       for n in (1, 3, 40)]
+                fp4_cache.fp4_unpack_blocks([layer], [kv], ids + turn, ids)
+                fp4_cache.fp4_pack_blocks([kv], [layer], ids.cuda(), ids + turn)
+                got += [*fp4_cache.fp4_read(layer, slots), kv.clone()]
+                out.append(got)
+        stream.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    want = [[] for _ in streams]
+    for i, s in enumerate(streams):
+        work(i, s, 6, want[i])
+    got = [[] for _ in streams]
+    threads = [threading.Thread(target=work, args=(i, s, 6, got[i])) for i, s in enumerate(streams)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for w, g in zip(want, got):
+        assert len(w) == len(g) == 6
+        assert all(torch.equal(x, y) for a, b in zip(w, g) for x, y in zip(a, b))
