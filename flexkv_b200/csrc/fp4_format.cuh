@@ -48,14 +48,7 @@ __device__ __forceinline__ float sixth(float amax) {
 // The half a scale code stands for, in both halves of a register.
 __device__ __forceinline__ uint32_t scale_half2(uint32_t code) { return code * 0x00800080u; }
 
-// Two e2m1 values (a byte, low four bits first) to two halves.
-__device__ __forceinline__ uint32_t e2m1x2_to_half2(uint32_t byte) {
-  uint32_t r;
-  asm("{\n .reg .b8 b;\n cvt.u8.u32 b, %1;\n cvt.rn.f16x2.e2m1x2 %0, b;\n}" : "=r"(r) : "r"(byte));
-  return r;
-}
-
-// The four bytes of a word, each as two halves.
+// The four bytes of a word, two e2m1 values each (low four bits first), as two halves.
 __device__ __forceinline__ void e2m1x8_to_half2(uint32_t w, uint32_t (&r)[4]) {
   asm("{\n .reg .b8 b0, b1, b2, b3;\n mov.b32 {b0, b1, b2, b3}, %4;\n"
       " cvt.rn.f16x2.e2m1x2 %0, b0;\n cvt.rn.f16x2.e2m1x2 %1, b1;\n"
