@@ -7,15 +7,16 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
-#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/Dtype.h>
 
 #include <algorithm>
 #include <cmath>
+#include <functional>
 #include <optional>
 #include <sstream>
 #include <stdexcept>
@@ -137,7 +138,8 @@ void blocks_apart(const Tensor &t, int64_t block, const char *name) {
 
 // Nothing here is differentiable: what records a gradient, or carries a tangent, is refused.
 void no_grad(std::initializer_list<const Tensor *> ts) {
-  const bool backward = c10::GradMode::is_enabled(), forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  const bool backward = c10::GradMode::is_enabled();
+  const bool forward = torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr;  // else there are no tangents
   for (const Tensor *t : ts) {
     if (!t) continue;
     if (backward && t->requires_grad()) refuse("the 4-bit cache has no gradient: call under torch.no_grad()");
@@ -305,6 +307,7 @@ PyObject *convert(PyObject *, PyObject *const *args, Py_ssize_t n) {
     else
       blocks_apart(k0, (int64_t)g.tpb * g.heads * g.dim, "kv_layers");
     std::vector<void *> kp(layers), fp(layers);
+    std::vector<const Tensor *> targets(layers);
     for (Py_ssize_t i = 0; i < layers; ++i) {
       const Tensor &f = tensor(PySequence_Fast_GET_ITEM(fps, i), "an entry of fp4_layers");
       const Tensor &k = tensor(PySequence_Fast_GET_ITEM(kvs, i), "an entry of kv_layers");
@@ -313,10 +316,11 @@ PyObject *convert(PyObject *, PyObject *const *args, Py_ssize_t n) {
       if (k.scalar_type() != k0.scalar_type() || k.sizes() != k0.sizes() || k.strides() != k0.strides() || k.device() != dev)
         refuse("kv_layers[", i, "] must have the type, shape and strides of kv_layers[0] and be on ", dev);
       no_grad({&k});
-      kp[i] = k.data_ptr(), fp[i] = f.data_ptr();
+      kp[i] = k.data_ptr(), fp[i] = f.data_ptr(), targets[i] = pack ? &f : &k;
     }
     std::vector<void *> to = pack ? fp : kp;
-    std::sort(to.begin(), to.end());
+    // layers that are allocated one after another are in order already
+    if (std::adjacent_find(to.begin(), to.end(), std::greater_equal<>()) != to.end()) std::sort(to.begin(), to.end());
     if ((pack ? f0 : k0).numel() && std::adjacent_find(to.begin(), to.end()) != to.end())
       refuse(pack ? "fp4_layers" : "kv_layers", ": a layer to write to appears twice");
     const Tensor &ka = tensor(args[3], "kv_block_ids"), &fa = tensor(args[4], "fp4_block_ids");
@@ -340,7 +344,7 @@ PyObject *convert(PyObject *, PyObject *const *args, Py_ssize_t n) {
       call(lib.pack_blocks_listed, lib.unpack_blocks_listed, host);
     else
       call(lib.pack_blocks, lib.unpack_blocks);
-    for (Py_ssize_t i = 0; i < layers; ++i) written(tensor(PySequence_Fast_GET_ITEM(pack ? fps : kvs, i), "a layer"));
+    for (const Tensor *t : targets) written(*t);
     Py_RETURN_NONE;
   });
   Py_XDECREF(fps);
