@@ -395,6 +395,12 @@ __device__ __forceinline__ float row_factor(float amax) {
   return __uint_as_float((uint32_t)(k + 127) << 23);
 }
 
+// What a row's queries are multiplied by: its factor, with the sign of softmax_scale, so that mul is positive and no
+// score 0 * inf.  A row with an infinite query has the scores inf, -inf and NaN and so no softmax: they all become
+// NaN, lest a row of -inf alone pass for one that sees nothing.
+__device__ __forceinline__ float query_factor(float amax, float factor, float scale) {
+  return amax > 3.4e38f ? __int_as_float(0x7FFFFFFF) : scale < 0.0f ? -factor : factor;
+}
 // From a row's q k to powers of two; its bounds keep 0 * mul and s * mul numbers.
 __device__ __forceinline__ float row_mul(float scale, float factor) {
   return fminf(fmaxf(fabsf(scale) * 1.4426950408889634f * (1.0f / factor), 1e-37f), 3e38f);
@@ -610,8 +616,7 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
         }
         amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
-        // a negative softmax_scale goes into the queries: the multiplier is positive, and so that no score is 0 * inf
-        const float f = row_factor(amax), fs = a.scale < 0.0f ? -f : f;
+        const float f = row_factor(amax), fs = query_factor(amax, f, a.scale);
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
@@ -1182,6 +1187,8 @@ fp4_many_kernel(const __grid_constant__ AttnArgs a, int blocks, int splits, floa
         }
         *reinterpret_cast<uint4 *>(&sm.q[t][i / 8][r * 128 + ((i % 8) ^ (r & 7)) * 16]) = make_uint4(y[0], y[1], y[2], y[3]);
       }
+      // an infinite query as in query_factor; a select there instead takes 717 us in place of 697 for three prompts
+      if (amax > 3.4e38f) *reinterpret_cast<uint4 *>(&sm.q[t][0][r * 128 + (r & 7) * 16]) = make_uint4(~0u, ~0u, ~0u, ~0u);
     }
     fence_async();
     mbar_arrive(&sm.q_full);

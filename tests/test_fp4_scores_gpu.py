@@ -98,3 +98,21 @@ def test_scales_past_float(form):
     k[30:33] = 0.0
     g = torch.Generator().manual_seed(3)
     check(form, k, torch.randn(100, D, generator=g), torch.full((D,), 1e20), 1e30, 1.0)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("where", [float("inf"), -float("inf")])
+def test_infinite_queries_have_no_softmax(form, where):
+    """Scores that are all infinite, of either sign: NaN as in the definition, and zeros where nothing is seen."""
+    g = torch.Generator().manual_seed(5)
+    q = torch.ones(D)
+    q[7] = where
+    out, lse, _, _ = attend(form, torch.rand(100, D, generator=g) + 1, torch.randn(100, D, generator=g), q, 0.1)
+    assert np.isnan(out).all() and np.isnan(lse).all()
+    new, heads, group, seqs = form
+    layer = torch.zeros(2, 3, heads, 1, 9 * D, dtype=torch.uint8, device="cuda")
+    x = q.bfloat16().cuda().expand(seqs * new, heads * group, D)
+    for tables, lens in ((0, 0), (99, 40)):  # no keys; keys in blocks outside the pool
+        out, lse = fp4_cache.fp4_attention(layer, x, torch.full((seqs, 3), tables, dtype=torch.int32, device="cuda"),
+                                           torch.full((seqs,), lens, dtype=torch.int32, device="cuda"), return_lse=True)
+        assert not bool(out.any()) and bool(torch.isneginf(lse).all())
