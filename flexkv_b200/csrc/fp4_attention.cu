@@ -136,15 +136,16 @@ __device__ __forceinline__ void fill_rest(const AttnArgs &a, int D, int thread, 
 // fixed order.
 //
 // Measured (B200, bfloat16, heads of 128): 48 sequences of 6000 to 16384 tokens,
-// 8 key heads, 32 query heads: 133 us for 630 MB, 4.7 TB/s, 73 % of a copy's
-// rate; what bounds it there is the issue of about 310 instructions a unit (64
+// 8 key heads, 32 query heads: 130 us for 630 MB, 4.8 TB/s, 74 % of a copy's
+// rate (call after call, each on other inputs), 144 where other work comes
+// between; what bounds it there is the issue of about 310 instructions a unit (64
 // conversions, 64 multiplications, 16 products; the read alone takes 106 us).
 // Why 12 warps, two units a stage and three stages: one unit and six stages take
 // 144 us, 16 warps with one unit and four stages 138, 8 warps with four units
 // 136, 16 warps with two stages of two 131.5 but 15.3 us instead of 13.2 for one
 // sequence of 1000 tokens (at that time).  Small calls are bound by the chain
 // launch, lengths, pages, keys, joins: that sequence 11 us, one of 131071 tokens
-// 17.4 us.
+// 17.9 us.
 
 // Warps of a CTA, units of a chunk and chunks of a warp's ring, for NT row tiles.
 // Heads of 64 leave registers for more: 64 sequences of 4000 tokens, 8 key heads,
@@ -231,7 +232,7 @@ __device__ __forceinline__ Cut find_cut(const AttnArgs &a) {
   if (a.num_seqs == 1 && total) {
     // All (head, row block)s are as long: cut between them, and into no more than leave a warp kWhole units each
     // while that spares the second step of the join.  1000 tokens, 8 heads: 11.0 us, and 14.0 with every cut at a
-    // unit a warp.
+    // unit a warp.  For one sequence only: two of them, cut at a unit a warp, take 14.5 us and four 15.7.
     constexpr int kWhole = 8;
     const Item it = item_of<R>(a, 0);
     const uint32_t items = it.blocks * a.kv_heads, few = (it.units + kWarps * kWhole - 1) / (kWarps * kWhole);
@@ -951,8 +952,9 @@ fp4_decode_kernel(const __grid_constant__ AttnArgs a, float *__restrict__ slots,
 // keys, and a second kernel joins what they have.
 //
 // Measured (B200, bfloat16, heads of 128, 4 query heads to a key head): three
-// chunks of about 3900 tokens behind 1500 cached ones, 655 GFLOP: 710 us, 920
-// TFLOP/s, 55 % of a library product's rate alone and 66 % of its sustained one.
+// chunks of about 3900 tokens behind 1500 cached ones, 655 GFLOP: 732 us call after
+// call, each on other inputs, 895 TFLOP/s, 54 % of a library product's rate alone
+// and 64 % of its sustained one (706 us where the inputs stay the same).
 // A chunk of 64 keys for both tiles takes about 2000 cycles of an SM: the tensor
 // core is busy for 1300 of them (a product of S with 64 columns takes 48 cycles,
 // its operands being 6 KiB of shared memory, one with P 64), the exponentials for
@@ -1583,9 +1585,12 @@ int launch_many(const AttnArgs &a, const ManyPlan &p, void *workspace, cudaStrea
   return FKV_OK;
 }
 
-// Rows of a key head up to which the few-rows kernel runs, 16 at a time.  16
-// sequences of 4000 tokens, 8 key heads of 128: 32 rows 57 us there, 59 in the
-// many-rows kernel (64 sequences: 172 and 232 us); 64 rows 100 and 59 us.
+// Rows of a key head up to which the few-rows kernel runs, 16 at a time.  8 key
+// heads, sequences of 4000 tokens, us there and in the many-rows kernel:
+//   heads of 128   32 rows: 16 sequences 60 and 60, 64 sequences 175 and 233
+//                  64 rows:              99 and 62,               326 and 235
+//   heads of 64    32 rows:              43 and 53,               114 and 204
+//                  64 rows:              66 and 53,               211 and 205
 constexpr int kFewRows = 32;
 int row_tiles(int64_t rows) { return rows <= 8 ? 1 : 2; }
 

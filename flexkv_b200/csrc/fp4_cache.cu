@@ -97,8 +97,9 @@ __device__ __forceinline__ void store_group(uint8_t *p, const uint32_t (&r)[8]) 
 // a place for each group.
 //
 // Bound by memory: 2 + 9/16 bytes a value.  Measured (B200, heads of 128): 256
-// blocks of 16 tokens, 8 heads, 32 layers packed and unpacked again in 213 us, 6.5
-// TB/s, 99 % of a copy's rate; a call that reads 32768 tokens 30.3 us, 5.7 TB/s.
+// blocks of 16 tokens, 8 heads, 32 layers packed and unpacked again in 215 us, 6.4
+// TB/s, 98 % of a copy's rate (227 us, 93 %, where other work comes between); a call
+// that reads 32768 tokens 30.5 us, 5.7 TB/s.
 // With divisions for each group's place and true ones in the rounding, 9 blocks of
 // 28 layers there and back took 9.9 us instead of 6.9, and quantising was bound by
 // the issue of 315 instructions a group.

@@ -683,9 +683,11 @@ int fkv_fp4_unpack_blocks_listed(int num_layers, void *const *fp4_layer_ptrs, vo
  * pool, count as hidden.  cu_seqlens_q must not decrease.  Rows before the first
  * sequence and behind the last are left as they were, or become zeros (lse:
  * -inf) with flag FKV_FP4_FILL_REST where there is a sequence at all.
- * max_q_len: the most rows of a sequence, which only chooses the kernel.  lse (optional): float [num_q_tokens,
- * num_q_heads], the natural logarithm of the sum of exponentials, -inf for a
- * row that sees nothing.  workspace: device memory of at least
+ * max_q_len: the most rows of a sequence, which only chooses the kernel (too
+ * large, and sequences of few rows take up to three times as long).  out may
+ * be q itself, with its strides, and must not overlap it otherwise.  lse
+ * (optional): float [num_q_tokens, num_q_heads], the natural logarithm of the
+ * sum of exponentials, -inf for a row that sees nothing.  workspace: device memory of at least
  * fkv_fp4_attention_workspace bytes, 16-byte aligned, that nothing else uses
  * until the call has run; its content does not matter. */
 #define FKV_FP4_CAUSAL 1
