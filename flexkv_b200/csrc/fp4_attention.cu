@@ -138,7 +138,7 @@ __device__ __forceinline__ void fill_rest(const AttnArgs &a, int D, int thread, 
 // Measured (B200, bfloat16, heads of 128): 48 sequences of 6000 to 16384 tokens,
 // 8 key heads, 32 query heads: 130 us for 630 MB, 4.8 TB/s, 74 % of a copy's
 // rate (call after call, each on other inputs), 144 where other work comes
-// between; what bounds it there is the issue of about 310 instructions a unit (64
+// between; what bounds it there is the issue of 315 instructions a unit (64
 // conversions, 64 multiplications, 16 products; the read alone takes 106 us).
 // Why 12 warps, two units a stage and three stages: one unit and six stages take
 // 144 us, 16 warps with one unit and four stages 138, 8 warps with four units
